@@ -267,6 +267,99 @@ int s2s_rgb8_device(int batch, int height, int width, const float* d_chw, int pn
 int s2s_forward_image(s2s_handle* h, int batch, int height, int width, const void* samples,
                       int channels, int bit_depth, int png_rows, uint8_t* out, uint8_t* aux);
 
+/* ---- Token operators on device tensors: attention over packed documents and the
+ * rotary positions of its queries and keys. No counterpart in the reference, whose
+ * attention stays inside 8x8 windows; these serve the layers of image and video
+ * transformers whose tokens see a whole image, a run of frames or a packed batch of
+ * images of several sizes.
+ *
+ * Handle-less: work is enqueued on `stream` (NULL = the default stream) of the device
+ * that holds the tensors, whichever device is current, without synchronising, without
+ * workspaces and without allocating: calls may overlap and be captured into graphs.
+ * The arguments are read during the call; the device arrays (offsets, prefixes,
+ * positions, slopes included) when the work runs. Refusals come back as
+ * S2S_ERR_INVALID, the message through s2s_last_error(NULL), before anything is
+ * enqueued. */
+enum { S2S_F16 = 0, S2S_BF16 = 1, S2S_F32 = 2 };
+
+#define S2S_MAX_AXES 3
+#define S2S_ROTARY_MAX_PAIRS 128
+
+/* Rows of heads: value d of head h of token t is data[t * token_stride + h * head_stride
+ * + d], strides in elements. The library's own QKV rows [token][head][q|k|v][dp] are
+ * three of these with token_stride = heads * 3 * dp and head_stride = 3 * dp. */
+typedef struct s2s_heads {
+  void* data;
+  int64_t token_stride;
+  int64_t head_stride; /* not read where heads == 1 */
+  int heads;
+} s2s_heads;
+
+/* Rotary positions: pair p of every head turns by position[axis[p]] * frequency[p]
+ * radians. Plain data: fill it with s2s_rotary_init or by hand (other frequencies, axes
+ * in turn). Pairs are (p, p + pairs) of a head's values, or (2p, 2p + 1) with
+ * `interleaved`; values from 2 * pairs on are copied. */
+typedef struct s2s_rotary {
+  int axes;
+  int pairs;
+  int interleaved;
+  uint8_t axis[S2S_ROTARY_MAX_PAIRS];
+  double frequency[S2S_ROTARY_MAX_PAIRS];
+} s2s_rotary;
+
+/* The geometric series over `sections[a]` pairs for each axis a in order: frequency
+ * base^(-p / pairs) of the pair's place in the whole head, or with `per_axis`
+ * base^(-i / sections[a]) of its place i in its section. Host only. */
+int s2s_rotary_init(s2s_rotary* r, int axes, const int* sections, double base, int per_axis,
+                    int interleaved);
+
+/* y[i] = x[i] turned, for i < n (1..4; q and k in one launch), `dtype` any of the three,
+ * any strides. y[i] may be x[i] itself; otherwise no output may overlap anything else.
+ * d_pos: int32 [axes][tokens], an axis's tokens contiguous, axes pos_stride apart. With
+ * `inverse` the turn is undone (the transposed rotation: also its gradient). Angles are
+ * reduced in 64 bits, products and sums are 32-bit, rounded once. */
+int s2s_rotary_apply(const s2s_rotary* r, int dtype, int head_dim, int tokens, const int* d_pos,
+                     int64_t pos_stride, const s2s_heads* x, const s2s_heads* y, int n,
+                     int inverse, void* stream);
+
+/* Attention of queries over the keys of their own document. Document d holds query rows
+ * [d_q_offsets[d], d_q_offsets[d + 1]) and key rows [d_kv_offsets[d], d_kv_offsets[d + 1]);
+ * offsets do not decrease and stay within the tokens (values that do not are cut to it:
+ * results are then undefined, no other memory is touched). NULL offsets: documents of
+ * equal length (the tokens must divide). Query head h reads key head
+ * h / (q.heads / k.heads). For query i of nq and key j of nk of a document
+ *   z = scale * <q_i, k_j>;  cap > 0: z = cap * tanh(z / cap);
+ *   z -= sum over axes a of |d_slopes[a][h]| * |d_q_pos[a][i] - d_kv_pos[a][j]|
+ * and key j is seen if causal == 0, or j <= i + nk - nq, or j < d_prefix[d] (NULL: none).
+ * out_i = sum of softmax(z)_j v_j over the keys seen, d_lse = log sum exp(z) in fp32; a row
+ * that sees no key (or only scores of minus infinity) gives zeros and minus infinity.
+ * Values at keys that no mask of the row lets through never reach it, NaN and infinities
+ * included. Rows of no document are left as they were. */
+typedef struct s2s_attention {
+  int dtype;     /* S2S_F16 or S2S_BF16, of q, k, v and out */
+  int head_dim;  /* a multiple of 8, at most 128 */
+  int q_tokens, kv_tokens;
+  int documents;
+  int causal;
+  const int* d_q_offsets;  /* [documents + 1] */
+  const int* d_kv_offsets; /* [documents + 1]; NULL only together with d_q_offsets */
+  const int* d_prefix;     /* [documents], causal only */
+  float scale;             /* > 0 */
+  float cap;               /* 0: none */
+  int axes;                /* of the distance bias, 0: none */
+  const float* d_slopes;   /* [axes][q heads] */
+  const int* d_q_pos;      /* [axes][q_tokens] */
+  const int* d_kv_pos;     /* [axes][kv_tokens] */
+  s2s_heads q, k, v, out;  /* 16-byte aligned, strides multiples of 8 elements */
+  float* d_lse;            /* [q heads][q_tokens], may be NULL */
+} s2s_attention;
+
+int s2s_masked_attention(const s2s_attention* a, void* stream);
+
+/* Waits for `device` and says whether a bounded wait of any kernel on it has given up
+ * since the last look (S2S_ERR_TIMEOUT; the synchronous forwards look by themselves). */
+int s2s_device_status(int device);
+
 /* gpu::selftest (src/gpu.rs:889-1265; `--cuda-selftest`, src/main.rs:179-192): with the
  * same arguments as s2s_create, build handles on `device` and check the fast paths
  * against their plain forms on a seeded two-image batch of an odd size

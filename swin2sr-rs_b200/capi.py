@@ -31,8 +31,12 @@ EXPORTS = ("s2s_create", "s2s_forward", "s2s_forward_batch", "s2s_forward_device
            "s2s_band_init_local", "s2s_band_rows", "s2s_forward_band", "s2s_forward_band_host",
            "s2s_band_partition", "s2s_band_halo_ops", "s2s_png_header", "s2s_png_decode",
            "s2s_png_encode_rgb8", "s2s_png_encode_rows", "s2s_free", "s2s_adjust_device",
-           "s2s_rgb8_device", "s2s_forward_image", "s2s_selftest")
+           "s2s_rgb8_device", "s2s_forward_image", "s2s_selftest", "s2s_rotary_init",
+           "s2s_rotary_apply", "s2s_masked_attention", "s2s_device_status")
 BAND_ID_BYTES = 128
+MAX_AXES, ROTARY_MAX_PAIRS = 3, 128
+# element types of the token operators
+DTYPE_CODE = {"float16": 0, "bfloat16": 1, "float32": 2}
 
 
 class S2SConfig(ctypes.Structure):
@@ -45,6 +49,27 @@ class S2SConfig(ctypes.Structure):
 class S2STensor(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char_p), ("data", ctypes.POINTER(ctypes.c_float)),
                 ("ndim", ctypes.c_int), ("shape", ctypes.c_int64 * 4)]
+
+
+class S2SHeads(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64), ("heads", ctypes.c_int)]
+
+
+class S2SRotary(ctypes.Structure):
+    _fields_ = [("axes", ctypes.c_int), ("pairs", ctypes.c_int), ("interleaved", ctypes.c_int),
+                ("axis", ctypes.c_uint8 * ROTARY_MAX_PAIRS),
+                ("frequency", ctypes.c_double * ROTARY_MAX_PAIRS)]
+
+
+class S2SAttention(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int), ("head_dim", ctypes.c_int), ("q_tokens", ctypes.c_int),
+                ("kv_tokens", ctypes.c_int), ("documents", ctypes.c_int), ("causal", ctypes.c_int),
+                ("d_q_offsets", ctypes.c_void_p), ("d_kv_offsets", ctypes.c_void_p),
+                ("d_prefix", ctypes.c_void_p), ("scale", ctypes.c_float), ("cap", ctypes.c_float),
+                ("axes", ctypes.c_int), ("d_slopes", ctypes.c_void_p),
+                ("d_q_pos", ctypes.c_void_p), ("d_kv_pos", ctypes.c_void_p), ("q", S2SHeads),
+                ("k", S2SHeads), ("v", S2SHeads), ("out", S2SHeads), ("d_lse", ctypes.c_void_p)]
 
 
 class S2SError(RuntimeError):
@@ -143,6 +168,18 @@ def load() -> ctypes.CDLL:
     L.s2s_selftest.argtypes = [ctypes.POINTER(S2SConfig), ctypes.POINTER(S2STensor), ctypes.c_int,
                                ctypes.c_int, ctypes.c_char_p, ctypes.c_int]
     L.s2s_selftest.restype = ctypes.c_int
+    hp = ctypes.POINTER(S2SHeads)
+    L.s2s_rotary_init.argtypes = [ctypes.POINTER(S2SRotary), ctypes.c_int, ip, ctypes.c_double,
+                                  ctypes.c_int, ctypes.c_int]
+    L.s2s_rotary_init.restype = ctypes.c_int
+    L.s2s_rotary_apply.argtypes = [ctypes.POINTER(S2SRotary), ctypes.c_int, ctypes.c_int,
+                                   ctypes.c_int, vp, ctypes.c_int64, hp, hp, ctypes.c_int,
+                                   ctypes.c_int, vp]
+    L.s2s_rotary_apply.restype = ctypes.c_int
+    L.s2s_masked_attention.argtypes = [ctypes.POINTER(S2SAttention), vp]
+    L.s2s_masked_attention.restype = ctypes.c_int
+    L.s2s_device_status.argtypes = [ctypes.c_int]
+    L.s2s_device_status.restype = ctypes.c_int
     L.s2s_version.argtypes = []
     L.s2s_version.restype = ctypes.c_char_p
     _lib = L
@@ -445,3 +482,62 @@ def rgb8_device(B: int, h: int, w: int, d_chw: int, d_out: int, png_rows: bool =
     L = load()
     _fail(L, L.s2s_rgb8_device(B, h, w, ctypes.c_void_p(d_chw), int(png_rows),
                                ctypes.c_void_p(d_out), ctypes.c_void_p(stream or None)))
+
+
+# ---- token operators on device pointers (handle-less; enqueued, not synchronised)
+def _dtype(name: str) -> int:
+    try:
+        return DTYPE_CODE[name]
+    except KeyError:
+        raise ValueError(f"dtype must be one of {', '.join(DTYPE_CODE)}, not {name!r}") from None
+
+
+def heads(data: int, token_stride: int, head_stride: int, n: int) -> S2SHeads:
+    """Rows of `n` heads at a device address, strides in elements (s2s_heads): for a torch
+    tensor x [tokens][heads][head_dim] with contiguous values,
+    heads(x.data_ptr(), x.stride(0), x.stride(1), x.shape[1])."""
+    return S2SHeads(data, token_stride, head_stride, n)
+
+
+def rotary_plan(sections, base: float = 10000.0, per_axis: bool = False,
+                interleaved: bool = False) -> S2SRotary:
+    """s2s_rotary_init: the rotary positions over len(sections) axes, sections[a] pairs of
+    each. Made once; `frequency` and `axis` may be changed afterwards."""
+    L = load()
+    r = S2SRotary()
+    s = (ctypes.c_int * len(sections))(*sections)
+    _fail(L, L.s2s_rotary_init(ctypes.byref(r), len(sections), s, base, int(per_axis),
+                               int(interleaved)))
+    return r
+
+
+def rotary(plan: S2SRotary, dtype: str, head_dim: int, tokens: int, d_pos: int, pos_stride: int,
+           tensors, inverse: bool = False, stream: int = 0) -> None:
+    """s2s_rotary_apply: `tensors` is [(x, y), ...] of heads(), x turned into y (the same for
+    in place); d_pos int32 [axes][tokens], axes `pos_stride` apart."""
+    L = load()
+    n = len(tensors)
+    x = (S2SHeads * n)(*[t[0] for t in tensors])
+    y = (S2SHeads * n)(*[t[1] for t in tensors])
+    _fail(L, L.s2s_rotary_apply(plan, _dtype(dtype), head_dim, tokens, d_pos or None, pos_stride,
+                                x, y, n, int(inverse), stream or None))
+
+
+def attention(dtype: str, head_dim: int, scale: float, q: S2SHeads, k: S2SHeads, v: S2SHeads,
+              out: S2SHeads, q_tokens: int, kv_tokens: int, documents: int = 1,
+              d_q_offsets: int = 0, d_kv_offsets: int = 0, causal: bool = False,
+              d_prefix: int = 0, cap: float = 0.0, axes: int = 0, d_slopes: int = 0,
+              d_q_pos: int = 0, d_kv_pos: int = 0, d_lse: int = 0, stream: int = 0) -> None:
+    """s2s_masked_attention on device pointers: queries over the keys of their own document,
+    with capped scores, a bias by distance, causal order and prefixes (include/s2s.h)."""
+    L = load()
+    a = S2SAttention(_dtype(dtype), head_dim, q_tokens, kv_tokens, documents, int(causal),
+                     d_q_offsets, d_kv_offsets, d_prefix, scale, cap, axes, d_slopes, d_q_pos,
+                     d_kv_pos, q, k, v, out, d_lse)
+    _fail(L, L.s2s_masked_attention(a, stream or None))
+
+
+def device_status(device: int = 0) -> None:
+    """s2s_device_status: waits for the device; raises if a bounded wait on it gave up."""
+    L = load()
+    _fail(L, L.s2s_device_status(device))

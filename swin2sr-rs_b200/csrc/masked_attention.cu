@@ -1,0 +1,277 @@
+// Attention of queries over the keys of their own document: capped scores, a bias that
+// falls with the distance along up to three position axes, causal order with a prefix
+// that every query sees. Documents lie one behind another in the token rows.
+//
+// Per head h and query i of a document of nq queries and nk keys
+//   z_j = scale <q_i, k_j>;  z_j = cap tanh(z_j / cap);
+//   z_j -= sum_a |slope[a][h]| |qpos[a][i] - kpos[a][j]|
+//   o_i = sum_{j < seen(i)} exp(z_j - m) v_j / sum_{j < seen(i)} exp(z_j - m)
+// All masks together leave each query a run of its document's first keys:
+//   seen(i) = nk, or with causal order min(nk, max(prefix, i + 1 + nk - nq)).
+// Scores, maxima, sums and outputs are fp32 until the one rounding of o.
+#include "heads.cuh"
+
+namespace s2s {
+namespace {
+
+struct Rows {
+  void* data;
+  int64_t token, head;  // strides
+};
+
+struct AttnArgs {
+  Rows q, k, v, out;
+  float* lse;
+  const int *qoff, *koff, *prefix;
+  const int *qpos, *kpos;
+  const float* slopes;
+  int q_tokens, kv_tokens, documents, causal, axes;
+  int q_heads, kv_heads, group, head_dim;
+  float scale, cap;
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct Doc {
+  int q0, nq, k0, nk, prefix;
+};
+
+// Offsets are device data that the host cannot check: cut to the tokens, so that no row
+// outside the tensors is ever touched.
+__device__ __forceinline__ Doc document(const AttnArgs& A, int d) {
+  Doc D;
+  if (A.qoff) {
+    D.q0 = min(max(A.qoff[d], 0), A.q_tokens);
+    D.nq = min(max(A.qoff[d + 1], D.q0), A.q_tokens) - D.q0;
+    D.k0 = min(max(A.koff[d], 0), A.kv_tokens);
+    D.nk = min(max(A.koff[d + 1], D.k0), A.kv_tokens) - D.k0;
+  } else {
+    D.nq = A.q_tokens / A.documents;
+    D.nk = A.kv_tokens / A.documents;
+    D.q0 = d * D.nq;
+    D.k0 = d * D.nk;
+  }
+  D.prefix = A.prefix ? A.prefix[d] : 0;
+  return D;
+}
+
+// Keys that query i of the document sees.
+__device__ __forceinline__ int seen(const AttnArgs& A, const Doc& D, int i) {
+  if (!A.causal) return D.nk;
+  const long long last = (long long)i + 1 + D.nk - D.nq;
+  return (int)min((long long)D.nk, max(last, (long long)max(D.prefix, 0)));
+}
+
+// The bias of one pair, times log2 e; positions may lie anywhere in 32 bits.
+__device__ __forceinline__ float distance_bias(const AttnArgs& A, int h, int qrow, int krow) {
+  float b = 0.0f;
+  for (int a = 0; a < A.axes; a++) {
+    const long long d = (long long)A.qpos[(int64_t)a * A.q_tokens + qrow] -
+                        A.kpos[(int64_t)a * A.kv_tokens + krow];
+    b -= fabsf(A.slopes[a * A.q_heads + h]) * kLog2e * (float)(d < 0 ? -d : d);
+  }
+  return b;
+}
+
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p) {
+  const uint2 u = *reinterpret_cast<const uint2*>(p);
+  const T* t = reinterpret_cast<const T*>(&u);
+  return make_float4(to_f32(t[0]), to_f32(t[1]), to_f32(t[2]), to_f32(t[3]));
+}
+
+// One query row of one head by one warp, key after key: lane l has the values
+// 4l .. 4l + 3 of the head.
+template <typename T>
+__device__ void attend_row(const AttnArgs& A, const Doc& D, int i, int h, int lane) {
+  const int qrow = D.q0 + i, hk = h / A.group, d = lane * 4;
+  const bool mine = d < A.head_dim;
+  const T* k = static_cast<const T*>(A.k.data) + (int64_t)hk * A.k.head + d;
+  const T* v = static_cast<const T*>(A.v.data) + (int64_t)hk * A.v.head + d;
+  float4 q = make_float4(0, 0, 0, 0), o = q;
+  if (mine)
+    q = load4(static_cast<const T*>(A.q.data) + (int64_t)qrow * A.q.token +
+              (int64_t)h * A.q.head + d);
+  const int n = seen(A, D, i);
+  float m = -INFINITY, l = 0.0f;
+  for (int j = 0; j < n; j++) {
+    const int64_t row = D.k0 + j;
+    float s = 0.0f;
+    if (mine) {
+      const float4 x = load4(k + row * A.k.token);
+      s = q.x * x.x + q.y * x.y + q.z * x.z + q.w * x.w;
+    }
+#pragma unroll
+    for (int w = 16; w; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+    float z = s * A.scale;
+    if (A.cap > 0.0f) z = A.cap * tanhf(z / A.cap);
+    z = z * kLog2e + distance_bias(A, h, qrow, (int)row);
+    if (z == -INFINITY) continue;
+    const float top = fmaxf(m, z), keep = ex2(m - top), p = ex2(z - top);
+    m = top;
+    l = l * keep + p;
+    if (mine) {
+      const float4 x = load4(v + row * A.v.token);
+      o.x = o.x * keep + p * x.x;
+      o.y = o.y * keep + p * x.y;
+      o.z = o.z * keep + p * x.z;
+      o.w = o.w * keep + p * x.w;
+    }
+  }
+  const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+  if (mine) {
+    uint2 u;
+    T* t = reinterpret_cast<T*>(&u);
+    t[0] = from_f32<T>(o.x * inv);
+    t[1] = from_f32<T>(o.y * inv);
+    t[2] = from_f32<T>(o.z * inv);
+    t[3] = from_f32<T>(o.w * inv);
+    *reinterpret_cast<uint2*>(static_cast<T*>(A.out.data) + (int64_t)qrow * A.out.token +
+                              (int64_t)h * A.out.head + d) = u;
+  }
+  if (A.lse && lane == 0)
+    A.lse[(int64_t)h * A.q_tokens + qrow] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+// One warp per (query row, head).
+template <typename T>
+__global__ void __launch_bounds__(256) k_attention_rows(const __grid_constant__ AttnArgs A) {
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (w >= (long long)A.q_tokens * A.q_heads) return;
+  const int row = (int)(w / A.q_heads), h = (int)(w % A.q_heads);
+  int d = 0;
+  if (A.qoff) {  // the last document that begins at or before the row
+    int lo = 0, hi = A.documents;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (A.qoff[mid] <= row) lo = mid + 1;
+      else hi = mid;
+    }
+    d = lo - 1;
+  } else {
+    d = row / (A.q_tokens / A.documents);
+  }
+  if (d < 0) return;
+  const Doc D = document(A, d);
+  if (row < D.q0 || row >= D.q0 + D.nq) return;
+  attend_row<T>(A, D, row - D.q0, h, lane);
+}
+
+template <typename T>
+cudaError_t launch_attention(const AttnArgs& A, cudaStream_t st) {
+  const long long warps = (long long)A.q_tokens * A.q_heads;
+  return launch_pdl(k_attention_rows<T>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, st, A);
+}
+
+}  // namespace
+}  // namespace s2s
+
+extern "C" {
+
+int s2s_masked_attention(const s2s_attention* a, void* stream) {
+  using namespace s2s;
+  return guarded_free([&] {
+    const std::string me = "s2s_masked_attention: ";
+    if (!a) fail(S2S_ERR_INVALID, me + "null argument");
+    if (a->dtype != S2S_F16 && a->dtype != S2S_BF16)
+      fail(S2S_ERR_INVALID, me + "dtype must be S2S_F16 or S2S_BF16");
+    if (a->head_dim < 8 || a->head_dim > 128 || a->head_dim % 8)
+      fail(S2S_ERR_INVALID, me + "head_dim must be a multiple of 8, at most 128");
+    if (a->q_tokens < 0 || a->kv_tokens < 0 || a->documents < 0)
+      fail(S2S_ERR_INVALID, me + "tokens and documents must be >= 0");
+    if (!a->d_q_offsets != !a->d_kv_offsets)
+      fail(S2S_ERR_INVALID, me + "offsets of queries and keys come together");
+    if (!a->d_q_offsets && a->documents > 0 &&
+        (a->q_tokens % a->documents || a->kv_tokens % a->documents))
+      fail(S2S_ERR_INVALID, me + "without offsets the documents must divide the tokens");
+    if (a->d_prefix && !a->causal) fail(S2S_ERR_INVALID, me + "a prefix needs causal order");
+    if (!(a->scale > 0.0f) || !std::isfinite(a->scale))
+      fail(S2S_ERR_INVALID, me + "scale must be positive and finite");
+    if (!(a->cap >= 0.0f) || !std::isfinite(a->cap))
+      fail(S2S_ERR_INVALID, me + "cap must be 0 or positive and finite");
+    if (a->axes < 0 || a->axes > S2S_MAX_AXES)
+      fail(S2S_ERR_INVALID, me + "axes must be 0.." + std::to_string(S2S_MAX_AXES));
+    check_heads("s2s_masked_attention: q", a->q, a->q_tokens, a->head_dim, a->dtype, 8, false);
+    check_heads("s2s_masked_attention: k", a->k, a->kv_tokens, a->head_dim, a->dtype, 8, false);
+    check_heads("s2s_masked_attention: v", a->v, a->kv_tokens, a->head_dim, a->dtype, 8, false);
+    check_heads("s2s_masked_attention: out", a->out, a->q_tokens, a->head_dim, a->dtype, 8, true);
+    if (a->v.heads != a->k.heads || a->out.heads != a->q.heads || a->q.heads % a->k.heads)
+      fail(S2S_ERR_INVALID, me + "k and v, and q and out, must have the same heads, q's a "
+                                 "multiple of k's");
+    if (a->q.heads > 65535) fail(S2S_ERR_INVALID, me + "at most 65535 heads");
+    for (const void* p : {(const void*)a->d_q_offsets, (const void*)a->d_kv_offsets,
+                          (const void*)a->d_prefix, (const void*)a->d_slopes,
+                          (const void*)a->d_q_pos, (const void*)a->d_kv_pos,
+                          (const void*)a->d_lse})
+      if ((uintptr_t)p % 4)
+        fail(S2S_ERR_INVALID, me + "offsets, prefix, slopes, positions and lse must be 4-byte "
+                                   "aligned");
+    if (a->q_tokens == 0 || a->documents == 0) return;
+    if (a->axes && (!a->d_slopes || !a->d_q_pos || (!a->d_kv_pos && a->kv_tokens)))
+      fail(S2S_ERR_INVALID, me + "axes need d_slopes, d_q_pos and d_kv_pos");
+    const bool keys = a->kv_tokens > 0;
+    DeviceScope scope({{"s2s_masked_attention: q", a->q.data},
+                       {"s2s_masked_attention: k", keys ? a->k.data : nullptr},
+                       {"s2s_masked_attention: v", keys ? a->v.data : nullptr},
+                       {"s2s_masked_attention: out", a->out.data},
+                       {"s2s_masked_attention: d_q_offsets", a->d_q_offsets},
+                       {"s2s_masked_attention: d_kv_offsets", a->d_kv_offsets},
+                       {"s2s_masked_attention: d_prefix", a->d_prefix},
+                       {"s2s_masked_attention: d_slopes", a->axes ? a->d_slopes : nullptr},
+                       {"s2s_masked_attention: d_q_pos", a->axes ? a->d_q_pos : nullptr},
+                       {"s2s_masked_attention: d_kv_pos", a->axes && keys ? a->d_kv_pos : nullptr},
+                       {"s2s_masked_attention: d_lse", a->d_lse}}, stream);
+    AttnArgs A;
+    memset(&A, 0, sizeof A);
+    auto rows = [](const s2s_heads& x, int64_t tokens) {
+      const s2s_heads p = plain_strides(x, tokens);
+      return Rows{p.data, p.token_stride, p.head_stride};
+    };
+    A.q = rows(a->q, a->q_tokens);
+    A.k = rows(a->k, a->kv_tokens);
+    A.v = rows(a->v, a->kv_tokens);
+    A.out = rows(a->out, a->q_tokens);
+    A.lse = a->d_lse;
+    A.qoff = a->d_q_offsets;
+    A.koff = a->d_kv_offsets;
+    A.prefix = a->d_prefix;
+    A.axes = a->axes;
+    A.qpos = a->d_q_pos;
+    A.kpos = a->d_kv_pos;
+    A.slopes = a->d_slopes;
+    A.q_tokens = a->q_tokens;
+    A.kv_tokens = a->kv_tokens;
+    A.documents = a->documents;
+    A.causal = a->causal != 0;
+    A.q_heads = a->q.heads;
+    A.kv_heads = a->k.heads;
+    A.group = a->q.heads / a->k.heads;
+    A.head_dim = a->head_dim;
+    A.scale = a->scale;
+    A.cap = a->cap;
+    cudaStream_t st = (cudaStream_t)stream;
+    ck(a->dtype == S2S_F16 ? launch_attention<__half>(A, st) : launch_attention<__nv_bfloat16>(A, st),
+       "masked_attention");
+  });
+}
+
+int s2s_device_status(int device) {
+  using namespace s2s;
+  return guarded_free([&] {
+    int before = 0;
+    ck(cudaGetDevice(&before), "cudaGetDevice");
+    struct Restore {
+      int d;
+      ~Restore() { cudaSetDevice(d); }
+    } restore{before};
+    ck(cudaSetDevice(device), "cudaSetDevice");
+    ck(cudaDeviceSynchronize(), "cudaDeviceSynchronize");
+    check_device_error(nullptr);
+  });
+}
+
+}  // extern "C"

@@ -9,3 +9,5 @@
 #include "engine.cu"
 #include "image.cu"
 #include "noalloc.cu"
+#include "rotary.cu"
+#include "masked_attention.cu"
