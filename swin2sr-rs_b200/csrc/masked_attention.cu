@@ -27,9 +27,11 @@ struct AttnArgs {
   const float* slopes;
   int q_tokens, kv_tokens, documents, causal, axes;
   int q_heads, kv_heads, group, head_dim;
+  int splits;  // CTAs of a cluster that share a tile's keys
   float scale, cap;
 };
 
+constexpr int kMaxSplits = 8;  // the portable cluster size
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -56,6 +58,30 @@ __device__ __forceinline__ Doc document(const AttnArgs& A, int d) {
   return D;
 }
 
+// Tiles of `rows` rows (`mult` rows a query) lie in slots: document d's tiles begin at slot
+// floor(rows before it / rows) + d, which leaves each document room for all of them without
+// a look at the others. The document of a slot by a whole warp, and the slot's tile in it;
+// -1 where there is none.
+__device__ __forceinline__ int find_document(const AttnArgs& A, int slot, int rows, int mult,
+                                             int lane, int* tile) {
+  auto first = [&](int d) -> long long {
+    const long long q = A.qoff ? (long long)min(max(A.qoff[d], 0), A.q_tokens)
+                               : (long long)d * (A.q_tokens / A.documents);
+    return q * mult / rows + d;
+  };
+  int lo = 0, n = A.documents;  // the last d of [lo, lo + n) with first(d) <= slot
+  while (n > 1) {
+    const int step = (n + 31) / 32, at = lo + lane * step;
+    const unsigned ok = __ballot_sync(0xffffffffu, lane * step < n && first(at) <= slot);
+    const int c = max(__popc(ok) - 1, 0) * step;
+    lo += c;
+    n = min(step, n - c);
+  }
+  const long long t = slot - first(lo);
+  *tile = (int)t;
+  return t < 0 ? -1 : lo;
+}
+
 // Keys that query i of the document sees.
 __device__ __forceinline__ int seen(const AttnArgs& A, const Doc& D, int i) {
   if (!A.causal) return D.nk;
@@ -74,6 +100,42 @@ __device__ __forceinline__ float distance_bias(const AttnArgs& A, int h, int qro
   return b;
 }
 
+// Four scores s -> cap2 * tanh(s * to_cap). Up to 1, tanh x = x P(x^2) with P the polynomial
+// of degree 6 of least relative error on [0, 1] (5e-8, by the exchange algorithm); beyond,
+// 1 - 2 / (1 + e^{2x}). The second form costs two more of the special function unit's
+// operations, which softmax is bound by, so a warp takes it only where it has such a score.
+__device__ __forceinline__ float tanh_poly(float x) {
+  const float u = x * x;
+  float p = 0.0010410225950181484f;
+  p = fmaf(p, u, -0.006203379016369581f);
+  p = fmaf(p, u, 0.020289979875087738f);
+  p = fmaf(p, u, -0.05345702916383743f);
+  p = fmaf(p, u, 0.13325203955173492f);
+  p = fmaf(p, u, -0.33332839608192444f);
+  p = fmaf(p, u, 0.9999999403953552f);
+  return x * p;
+}
+__device__ __forceinline__ float tanh_exp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(fabsf(x) * (2.0f * kLog2e))));
+  return copysignf(fmaf(-2.0f, r, 1.0f), x);
+}
+__device__ __forceinline__ void capped(float (&s)[4], float to_cap, float cap2) {
+  float x[4], far = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    x[e] = s[e] * to_cap;
+    far = fmaxf(far, fabsf(x[e]));
+  }
+  if (__any_sync(0xffffffffu, far > 1.0f)) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) s[e] = cap2 * (fabsf(x[e]) > 1.0f ? tanh_exp(x[e]) : tanh_poly(x[e]));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; e++) s[e] = cap2 * tanh_poly(x[e]);
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ float4 load4(const T* p) {
   const uint2 u = *reinterpret_cast<const uint2*>(p);
@@ -82,9 +144,10 @@ __device__ __forceinline__ float4 load4(const T* p) {
 }
 
 // One query row of one head by one warp, key after key: lane l has the values
-// 4l .. 4l + 3 of the head.
+// 4l .. 4l + 3 of the head. For rows that a tile cannot do: it multiplies the values of
+// keys that a row does not see by zero weights, and zero times NaN or infinity is NaN.
 template <typename T>
-__device__ void attend_row(const AttnArgs& A, const Doc& D, int i, int h, int lane) {
+__device__ __noinline__ void attend_row(const AttnArgs& A, const Doc& D, int i, int h, int lane) {
   const int qrow = D.q0 + i, hk = h / A.group, d = lane * 4;
   const bool mine = d < A.head_dim;
   const T* k = static_cast<const T*>(A.k.data) + (int64_t)hk * A.k.head + d;
@@ -134,37 +197,17 @@ __device__ void attend_row(const AttnArgs& A, const Doc& D, int i, int h, int la
     A.lse[(int64_t)h * A.q_tokens + qrow] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
-// One warp per (query row, head).
-template <typename T>
-__global__ void __launch_bounds__(256) k_attention_rows(const __grid_constant__ AttnArgs A) {
-  pdl_trigger();
-  pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (w >= (long long)A.q_tokens * A.q_heads) return;
-  const int row = (int)(w / A.q_heads), h = (int)(w % A.q_heads);
-  int d = 0;
-  if (A.qoff) {  // the last document that begins at or before the row
-    int lo = 0, hi = A.documents;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (A.qoff[mid] <= row) lo = mid + 1;
-      else hi = mid;
-    }
-    d = lo - 1;
-  } else {
-    d = row / (A.q_tokens / A.documents);
-  }
-  if (d < 0) return;
-  const Doc D = document(A, d);
-  if (row < D.q0 || row >= D.q0 + D.nq) return;
-  attend_row<T>(A, D, row - D.q0, h, lane);
-}
+}  // namespace
+}  // namespace s2s
+
+#include "masked_attention_mma.cuh"
+
+namespace s2s {
+namespace {
 
 template <typename T>
-cudaError_t launch_attention(const AttnArgs& A, cudaStream_t st) {
-  const long long warps = (long long)A.q_tokens * A.q_heads;
-  return launch_pdl(k_attention_rows<T>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, st, A);
+cudaError_t launch_attention(AttnArgs& A, cudaStream_t st) {
+  return launch_attention_mma<T>(A, st);
 }
 
 }  // namespace

@@ -1,0 +1,532 @@
+// The attention of masked_attention.cu on mma.sync tiles, for short documents, few queries
+// and small work.
+//
+// A CTA of four warps takes 16 * RW rows of one document and key head - a row is a query and
+// one of the query heads that share the key head, so K and V are read once for all of them -
+// and walks the keys in tiles of 64 through a ring of three cp.async stages. RW warps lie
+// along the rows, 4 / RW along the keys of a tile: one query of eight heads is one row tile,
+// whose keys the four warps share. Every warp keeps a running maximum, sum and output of its
+// own; they are joined once at the end, first within the CTA, then over the CTAs of a cluster
+// among which the keys of the tile were split (through distributed shared memory: a call
+// needs no workspace, and the order of the sums is fixed).
+//
+// Bound: HBM where the keys are long (K and V are read once), latency where they are not.
+#pragma once
+
+namespace s2s {
+namespace {
+
+constexpr int kMmaThreads = 128;
+constexpr int kMmaKeys = 64;    // keys of a tile
+constexpr int kMmaStages = 3;
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) { return pack_h2(lo, hi); }
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <typename T>
+__device__ __forceinline__ void mma_tile(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1);
+template <>
+__device__ __forceinline__ void mma_tile<__half>(float (&c)[4], const uint32_t (&a)[4],
+                                                 uint32_t b0, uint32_t b1) {
+  mma16816(c, a[0], a[1], a[2], a[3], b0, b1);
+}
+template <>
+__device__ __forceinline__ void mma_tile<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4],
+                                                        uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// 16 bytes global -> shared, zeros where `ok` is false (the source is not read then).
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(src)), "r"(ok ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(src)), "r"(ok ? 4 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// ------------------------------------------------------------------------- clusters
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+__device__ __forceinline__ float cluster_load(uint32_t addr, uint32_t rank) {
+  float v;
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\t"
+      "ld.shared::cluster.f32 %0, [a];\n\t}"
+      : "=f"(v)
+      : "r"(addr), "r"(rank));
+  return v;
+}
+__device__ __forceinline__ float4 cluster_load4(uint32_t addr, uint32_t rank) {
+  float4 v;
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\t"
+      "ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [a];\n\t}"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+      : "r"(addr), "r"(rank));
+  return v;
+}
+
+template <int DP, int RW>
+struct MmaCfg {
+  static constexpr int KW = 4 / RW;              // warps along the keys
+  static constexpr int ROWS = 16 * RW;
+  static constexpr int KEYS = kMmaKeys / KW;     // keys of a tile that one warp takes
+  static constexpr int TILE = kMmaKeys * DP * 2; // bytes of a K or V tile
+  static constexpr int POS = S2S_MAX_AXES * kMmaKeys * 4;
+  static constexpr int RING = kMmaStages * (2 * TILE + POS);
+  static constexpr int LD = DP + 4;              // floats of a joined output row
+  static constexpr int JOIN = 4 * 16 * LD * 4;   // the four warps' outputs, over the ring
+  static constexpr int BODY = RING > JOIN ? RING : JOIN;
+  static constexpr int SMEM = BODY + 4 * 16 * 8 + ROWS * 12;  // + maxima and sums, + flags
+};
+
+// Byte offset of 16-byte chunk `c` of row `r` in a [rows][DP] tile: the chunks of a row are
+// permuted so that eight rows' equal chunks lie in different banks.
+template <int DP>
+__device__ __forceinline__ uint32_t tile_at(int r, int c) {
+  const int x = DP == 32 ? (r >> 1) & 3 : r & 7;
+  return (uint32_t)(r * DP * 2 + ((c ^ x) << 4));
+}
+
+template <typename T, int DP, int RW>
+__global__ void __launch_bounds__(kMmaThreads) k_attention_mma(const __grid_constant__ AttnArgs A) {
+  using C = MmaCfg<DP, RW>;
+  constexpr int KW = C::KW, NT = C::KEYS / 8, DN = DP / 8, DK = DP / 16;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rw = warp % RW, kw = warp / RW, g = lane >> 2, t4 = lane & 3;
+  const int S = A.splits;
+  const int split = S > 1 ? (int)cluster_rank() : 0;
+  const unsigned item = blockIdx.x / S;
+  const int slot = item / A.kv_heads, hk = item % A.kv_heads;
+  pdl_trigger();
+  pdl_wait();
+
+  int tile;
+  const int doc = find_document(A, slot, C::ROWS, A.group, lane, &tile);
+  if (doc < 0) return;  // the same for all of a cluster
+  const Doc D = document(A, doc);
+  const long long r0 = (long long)tile * C::ROWS;  // rows of the document: query * group + head
+  const long long nrows = (long long)D.nq * A.group - r0;
+  if (nrows <= 0) return;
+  const int i_first = (int)(r0 / A.group);
+  const int i_last = min(D.nq - 1, (int)((r0 + C::ROWS - 1) / A.group));
+  const int kend = seen(A, D, i_last);           // keys that any row of the tile sees
+  const int ntiles = (kend + kMmaKeys - 1) / kMmaKeys;
+  const int tb = (int)((long long)ntiles * split / S), te = (int)((long long)ntiles * (split + 1) / S);
+  const int hd = A.head_dim;
+
+  // this thread's two rows
+  const T* qp[2];
+  int row_seen[2], row_q[2], row_h[2];
+  bool live[2];
+#pragma unroll
+  for (int e = 0; e < 2; e++) {
+    const long long r = r0 + rw * 16 + g + 8 * e;
+    live[e] = r - r0 < nrows;
+    const int i = live[e] ? (int)(r / A.group) : i_first;
+    row_q[e] = D.q0 + i;
+    row_h[e] = hk * A.group + (live[e] ? (int)(r - (long long)i * A.group) : 0);
+    row_seen[e] = live[e] ? seen(A, D, i) : 0;
+    qp[e] = static_cast<const T*>(A.q.data) + (int64_t)row_q[e] * A.q.token +
+            (int64_t)row_h[e] * A.q.head;
+  }
+  const int open = seen(A, D, i_first);  // every row sees the keys before this one
+
+  // bias: per axis the rows' slopes times log2 e and positions, from the tile's first query
+  float slope[2][S2S_MAX_AXES], qpos[2][S2S_MAX_AXES];
+  int ref[S2S_MAX_AXES];
+  if (A.axes) {
+#pragma unroll
+    for (int a = 0; a < S2S_MAX_AXES; a++)
+      if (a < A.axes) {
+        const int* qa = A.qpos + (int64_t)a * A.q_tokens;
+        ref[a] = qa[D.q0 + i_first];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          slope[e][a] = fabsf(A.slopes[a * A.q_heads + row_h[e]]) * kLog2e;
+          qpos[e][a] = (float)(int)((unsigned)qa[row_q[e]] - (unsigned)ref[a]);
+        }
+      }
+  }
+
+  // K and V tiles into the ring
+  constexpr int CH = DP / 8, STEP = kMmaThreads / CH;  // chunks of a row, rows a pass
+  const int lrow = tid / CH, lch = tid % CH;
+  const bool lok = lch * 8 < hd;
+  const T* kbase = static_cast<const T*>(A.k.data) + (int64_t)D.k0 * A.k.token +
+                   (int64_t)hk * A.k.head + (lok ? lch * 8 : 0);
+  const T* vbase = static_cast<const T*>(A.v.data) + (int64_t)D.k0 * A.v.token +
+                   (int64_t)hk * A.v.head + (lok ? lch * 8 : 0);
+  auto fetch = [&](int t) {
+    const int st = (t - tb) % kMmaStages;
+    const uint32_t kd = smem_u32(smem) + st * (2 * C::TILE + C::POS), vd = kd + C::TILE;
+#pragma unroll
+    for (int r = lrow; r < kMmaKeys; r += STEP) {
+      const int j = t * kMmaKeys + r;
+      const bool ok = lok && j < kend;
+      const int64_t row = ok ? j : 0;
+      cp_async16(kd + tile_at<DP>(r, lch), kbase + row * A.k.token, ok);
+      cp_async16(vd + tile_at<DP>(r, lch), vbase + row * A.v.token, ok);
+    }
+    if (A.axes)
+      for (int u = tid; u < A.axes * kMmaKeys; u += kMmaThreads) {
+        const int a = u / kMmaKeys, j = t * kMmaKeys + u % kMmaKeys;
+        const bool ok = j < kend;
+        cp_async4(vd + C::TILE + u * 4, A.kpos + (int64_t)a * A.kv_tokens + D.k0 + (ok ? j : 0), ok);
+      }
+  };
+#pragma unroll
+  for (int s = 0; s < kMmaStages - 1; s++) {
+    if (tb + s < te) fetch(tb + s);
+    cp_async_commit();
+  }
+
+  // Q fragments straight from global memory
+  uint32_t qf[DK][4];
+#pragma unroll
+  for (int kk = 0; kk < DK; kk++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int d = kk * 16 + 2 * t4 + (e >> 1) * 8;
+      qf[kk][e] = live[e & 1] && d < hd ? *reinterpret_cast<const uint32_t*>(qp[e & 1] + d) : 0u;
+    }
+
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+  float o[DN][4];
+#pragma unroll
+  for (int n = 0; n < DN; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+  const float to_cap = A.cap > 0.0f ? A.scale / A.cap : 0.0f;
+  const float cap2 = A.cap * kLog2e, scale2 = A.scale * kLog2e;
+
+  for (int t = tb; t < te; t++) {
+    cp_async_wait<kMmaStages - 2>();
+    __syncthreads();
+    if (t + kMmaStages - 1 < te) fetch(t + kMmaStages - 1);
+    cp_async_commit();
+    const uint32_t ks = smem_u32(smem) + ((t - tb) % kMmaStages) * (2 * C::TILE + C::POS);
+    const uint32_t vs = ks + C::TILE;
+    const int j0 = t * kMmaKeys + kw * C::KEYS;
+    if (KW > 1 && j0 >= kend) continue;  // no key of this warp is seen
+
+    float s[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+#pragma unroll
+    for (int kk = 0; kk < DK; kk++) {
+      if (kk * 16 >= hd) break;
+#pragma unroll
+      for (int n = 0; n < NT; n += 2) {
+        uint32_t b0, b1, b2, b3;
+        const int r = kw * C::KEYS + n * 8 + (lane & 7) + ((lane >> 4) << 3);
+        ldsm_x4(ks + tile_at<DP>(r, kk * 2 + ((lane >> 3) & 1)), b0, b1, b2, b3);
+        mma_tile<T>(s[n], qf[kk], b0, b1);
+        mma_tile<T>(s[n + 1], qf[kk], b2, b3);
+      }
+    }
+    // scores in units of log 2
+    if (A.cap > 0.0f) {
+#pragma unroll
+      for (int n = 0; n < NT; n++) capped(s[n], to_cap, cap2);
+    } else {
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[n][e] *= scale2;
+    }
+    if (A.axes) {
+      const int* kp = reinterpret_cast<const int*>(
+          smem + ((t - tb) % kMmaStages) * (2 * C::TILE + C::POS) + 2 * C::TILE);
+#pragma unroll
+      for (int a = 0; a < S2S_MAX_AXES; a++)
+        if (a < A.axes)
+#pragma unroll
+          for (int n = 0; n < NT; n++) {
+            const int2 k2 = *reinterpret_cast<const int2*>(kp + a * kMmaKeys + kw * C::KEYS + n * 8 + 2 * t4);
+            const float x0 = (float)(int)((unsigned)k2.x - (unsigned)ref[a]);
+            const float x1 = (float)(int)((unsigned)k2.y - (unsigned)ref[a]);
+            s[n][0] -= slope[0][a] * fabsf(qpos[0][a] - x0);
+            s[n][1] -= slope[0][a] * fabsf(qpos[0][a] - x1);
+            s[n][2] -= slope[1][a] * fabsf(qpos[1][a] - x0);
+            s[n][3] -= slope[1][a] * fabsf(qpos[1][a] - x1);
+          }
+    }
+    if (j0 + C::KEYS > open) {
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (j0 + n * 8 + 2 * t4 + (e & 1) >= row_seen[e >> 1]) s[n][e] = -INFINITY;
+    }
+    // running maximum and sum
+    float keep[2], base[2];
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < NT; n++) top = fmaxf(top, fmaxf(s[n][2 * e], s[n][2 * e + 1]));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      top = fmaxf(top, m[e]);
+      base[e] = top == -INFINITY ? 0.0f : top;  // a row that has seen nothing yet
+      keep[e] = ex2(m[e] - base[e]);
+      m[e] = top;
+      l[e] *= keep[e];
+    }
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        s[n][e] = ex2(s[n][e] - base[e >> 1]);
+        l[e >> 1] += s[n][e];
+      }
+    if (__any_sync(0xffffffffu, keep[0] != 1.0f || keep[1] != 1.0f)) {
+#pragma unroll
+      for (int n = 0; n < DN; n++) {
+        o[n][0] *= keep[0];
+        o[n][1] *= keep[0];
+        o[n][2] *= keep[1];
+        o[n][3] *= keep[1];
+      }
+    }
+    // O += P V; the weights are rounded to the type of v, the sum l is not
+#pragma unroll
+    for (int kk = 0; kk < NT / 2; kk++) {
+      const uint32_t a[4] = {pack2<T>(s[2 * kk][0], s[2 * kk][1]), pack2<T>(s[2 * kk][2], s[2 * kk][3]),
+                             pack2<T>(s[2 * kk + 1][0], s[2 * kk + 1][1]),
+                             pack2<T>(s[2 * kk + 1][2], s[2 * kk + 1][3])};
+#pragma unroll
+      for (int n = 0; n < DN; n += 2) {
+        if (n * 8 >= hd) break;
+        uint32_t b0, b1, b2, b3;
+        const int r = kw * C::KEYS + kk * 16 + (lane & 7) + (((lane >> 3) & 1) << 3);
+        ldsm_x4_t(vs + tile_at<DP>(r, n + (lane >> 4)), b0, b1, b2, b3);
+        mma_tile<T>(o[n], a, b0, b1);
+        mma_tile<T>(o[n + 1], a, b2, b3);
+      }
+    }
+  }
+  cp_async_wait<0>();
+#pragma unroll
+  for (int e = 0; e < 2; e++) {
+    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+  }
+
+  if (KW == 1 && S == 1) {
+    // the warp has its rows to itself
+    unsigned redo = 0;
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const float inv = m[e] == -INFINITY ? 0.0f : 1.0f / l[e];
+      bool bad = false;
+      T* op = static_cast<T*>(A.out.data) + (int64_t)row_q[e] * A.out.token + (int64_t)row_h[e] * A.out.head;
+#pragma unroll
+      for (int n = 0; n < DN; n++) {
+        const float x = m[e] == -INFINITY ? 0.0f : o[n][2 * e] * inv;
+        const float y = m[e] == -INFINITY ? 0.0f : o[n][2 * e + 1] * inv;
+        bad = bad || !(fabsf(x) < INFINITY) || !(fabsf(y) < INFINITY);
+        if (live[e] && n * 8 < hd) *reinterpret_cast<uint32_t*>(op + n * 8 + 2 * t4) = pack2<T>(x, y);
+      }
+      if (live[e] && t4 == 0 && A.lse)
+        A.lse[(int64_t)row_h[e] * A.q_tokens + row_q[e]] =
+            m[e] == -INFINITY ? -INFINITY : (m[e] + log2f(l[e])) * kLn2;
+      // keys that the row does not see were multiplied by zero weights: a NaN or infinity
+      // among their values shows here, and the row is done again without them
+      redo |= __ballot_sync(0xffffffffu, bad && live[e] && row_seen[e] < kend) ? 1u << e : 0u;
+      if (redo >> e & 1) {
+        const unsigned who = __ballot_sync(0xffffffffu, bad && live[e] && row_seen[e] < kend);
+        __syncwarp();
+        for (int q = 0; q < 8; q++)
+          if (who >> (4 * q) & 15u) {
+            const int src = 4 * q;
+            const int i = __shfl_sync(0xffffffffu, row_q[e], src) - D.q0;
+            attend_row<T>(A, D, i, __shfl_sync(0xffffffffu, row_h[e], src), lane);
+          }
+      }
+    }
+    return;
+  }
+
+  // Join: the warps' outputs, maxima and sums in shared memory (over the ring)
+  float* part = reinterpret_cast<float*>(smem);                 // [4][16][LD]
+  float2* ml = reinterpret_cast<float2*>(smem + C::BODY);       // [4][16]
+  float2* mlc = ml + 64;                                        // [ROWS] of the CTA
+  int* flag = reinterpret_cast<int*>(mlc + C::ROWS);            // [ROWS]
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < 2; e++) {
+    float* p = part + (warp * 16 + g + 8 * e) * C::LD + 2 * t4;
+#pragma unroll
+    for (int n = 0; n < DN; n++) *reinterpret_cast<float2*>(p + n * 8) = make_float2(o[n][2 * e], o[n][2 * e + 1]);
+    if (t4 == 0) ml[warp * 16 + g + 8 * e] = make_float2(m[e], l[e]);
+  }
+  if (tid < C::ROWS) flag[tid] = 0;
+  __syncthreads();
+  // the key warps of a row into the first of them
+  constexpr int Q4 = DP / 4;
+  for (int u = tid; u < C::ROWS * Q4; u += kMmaThreads) {
+    const int r = u / Q4, c = (u % Q4) * 4, w = r / 16, rr = r % 16;
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < KW; k++) top = fmaxf(top, ml[(k * RW + w) * 16 + rr].x);
+    const float b = top == -INFINITY ? 0.0f : top;
+    float4 sum = make_float4(0, 0, 0, 0);
+    float total = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KW; k++) {
+      const float2 x = ml[(k * RW + w) * 16 + rr];
+      const float f = ex2(x.x - b);
+      const float4 v = *reinterpret_cast<const float4*>(part + ((k * RW + w) * 16 + rr) * C::LD + c);
+      total += x.y * f;
+      sum.x += v.x * f;
+      sum.y += v.y * f;
+      sum.z += v.z * f;
+      sum.w += v.w * f;
+    }
+    *reinterpret_cast<float4*>(part + (w * 16 + rr) * C::LD + c) = sum;
+    if (c == 0) mlc[r] = make_float2(top, total);
+  }
+  if (S > 1) cluster_sync();
+  else __syncthreads();
+  // the CTAs of the cluster: each finishes every S-th row
+  const int mine = (C::ROWS - split + S - 1) / S;
+  for (int u = tid; u < mine * Q4; u += kMmaThreads) {
+    const int r = split + (u / Q4) * S, c = (u % Q4) * 4;
+    if (r >= nrows) continue;
+    float4 sum;
+    float top, total;
+    if (S > 1) {
+      const uint32_t mla = smem_u32(&mlc[r]), pa = smem_u32(part + r * C::LD + c);
+      top = -INFINITY;
+      for (int k = 0; k < S; k++) top = fmaxf(top, cluster_load(mla, k));
+      const float b = top == -INFINITY ? 0.0f : top;
+      sum = make_float4(0, 0, 0, 0);
+      total = 0.0f;
+      for (int k = 0; k < S; k++) {
+        const float f = ex2(cluster_load(mla, k) - b);
+        const float4 v = cluster_load4(pa, k);
+        total += cluster_load(mla + 4, k) * f;
+        sum.x += v.x * f;
+        sum.y += v.y * f;
+        sum.z += v.z * f;
+        sum.w += v.w * f;
+      }
+    } else {
+      sum = *reinterpret_cast<const float4*>(part + r * C::LD + c);
+      top = mlc[r].x;
+      total = mlc[r].y;
+    }
+    const int i = (int)((r0 + r) / A.group), h = hk * A.group + (int)(r0 + r - (long long)i * A.group);
+    const bool none = top == -INFINITY;
+    const float inv = none ? 0.0f : 1.0f / total;
+    const float4 x = none ? make_float4(0, 0, 0, 0)
+                          : make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+    if (c < hd)
+      *reinterpret_cast<uint2*>(static_cast<T*>(A.out.data) + (int64_t)(D.q0 + i) * A.out.token +
+                                (int64_t)h * A.out.head + c) = make_uint2(pack2<T>(x.x, x.y), pack2<T>(x.z, x.w));
+    if (c == 0 && A.lse)
+      A.lse[(int64_t)h * A.q_tokens + D.q0 + i] = none ? -INFINITY : (top + log2f(total)) * kLn2;
+    if (!(fabsf(x.x) < INFINITY && fabsf(x.y) < INFINITY && fabsf(x.z) < INFINITY && fabsf(x.w) < INFINITY) &&
+        seen(A, D, i) < kend)
+      flag[r] = 1;
+  }
+  __syncthreads();
+  for (int r = warp; r < C::ROWS; r += 4)
+    if (flag[r]) {
+      const int i = (int)((r0 + r) / A.group);
+      attend_row<T>(A, D, i, hk * A.group + (int)(r0 + r - (long long)i * A.group), lane);
+    }
+  if (S > 1) cluster_sync();  // nobody leaves while its shared memory is read
+}
+
+template <typename T, int DP, int RW>
+cudaError_t launch_attention_mma(AttnArgs& A, cudaStream_t st) {
+  using C = MmaCfg<DP, RW>;
+  auto kernel = k_attention_mma<T, DP, RW>;
+  static LaunchSetup setup;
+  int ctas = 0;
+  cudaError_t err = resident_ctas(setup, kernel, kMmaThreads, C::SMEM, &ctas);
+  if (err != cudaSuccess) return err;
+  const long long slots = (long long)A.q_tokens * A.group / C::ROWS + A.documents;
+  const long long items = slots * A.kv_heads;
+  // Few tiles with many keys: the keys of a tile are split over a cluster, until the CTAs
+  // fill the device or have two key tiles each (by the mean length: the host does not know
+  // the offsets).
+  const long long keys = A.kv_tokens / A.documents;
+  int splits = 1;
+  while (splits < kMaxSplits && items * splits * 2 <= ctas && keys >= 4LL * kMmaKeys * splits) splits *= 2;
+  A.splits = splits;
+  const long long grid = items * splits;
+  if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof cfg);
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kMmaThreads);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (splits > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = splits;
+    attr[n].val.clusterDim.y = 1;
+    attr[n++].val.clusterDim.z = 1;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  return cudaLaunchKernelEx(&cfg, kernel, A);
+}
+
+template <typename T, int DP>
+cudaError_t launch_attention_mma(AttnArgs& A, cudaStream_t st) {
+  const long long rows = (long long)A.q_tokens * A.group / A.documents;
+  return rows <= 16   ? launch_attention_mma<T, DP, 1>(A, st)
+         : rows <= 32 ? launch_attention_mma<T, DP, 2>(A, st)
+                      : launch_attention_mma<T, DP, 4>(A, st);
+}
+
+template <typename T>
+cudaError_t launch_attention_mma(AttnArgs& A, cudaStream_t st) {
+  return A.head_dim <= 32   ? launch_attention_mma<T, 32>(A, st)
+         : A.head_dim <= 64 ? launch_attention_mma<T, 64>(A, st)
+                            : launch_attention_mma<T, 128>(A, st);
+}
+
+}  // namespace
+}  // namespace s2s
