@@ -201,13 +201,15 @@ __device__ __noinline__ void attend_row(const AttnArgs& A, const Doc& D, int i, 
 }  // namespace s2s
 
 #include "masked_attention_mma.cuh"
+#include "masked_attention_tc.cuh"
 
 namespace s2s {
 namespace {
 
 template <typename T>
 cudaError_t launch_attention(AttnArgs& A, cudaStream_t st) {
-  return launch_attention_mma<T>(A, st);
+  const bool many = A.q_tokens / A.documents >= 128 && A.kv_tokens > 0;
+  return many ? launch_attention_tc<T>(A, st) : launch_attention_mma<T>(A, st);
 }
 
 }  // namespace

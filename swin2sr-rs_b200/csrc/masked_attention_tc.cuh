@@ -1,0 +1,496 @@
+// The attention of masked_attention.cu on tcgen05, for documents with many queries.
+//
+// A CTA takes 256 query rows of one document and head as two tiles of 128, which share every
+// K and V tile of 128 keys that TMA brings in. Ten warps: two groups of four for the softmax
+// of the two tiles, one that loads, one that issues the MMAs:
+//   S_w = Q_w K_i^T      both operands from shared memory, S_w in TMEM (128 columns)
+//   softmax group w      reads S_w, a row per thread, and writes the weights P_w as 16-bit
+//                        values over the first half of S_w's columns
+//   O_w += P_w V_i       P_w from TMEM, V_i as it lies in memory (keys by values: the MN-major
+//                        operand form), O_w in TMEM
+// While group 0 is at its softmax the tensor core does tile 1's two products and the other way
+// round. The output is scaled again only when a row's maximum grows by more than 2^8 beyond
+// the one its weights refer to (weights then stay below 2^8, in the range of both types, and
+// the sums are 32-bit), which after the first tiles is rare; the group does it itself, as
+// S_w(i) being complete means O_w += P_w V_{i-1} is too.
+#pragma once
+
+namespace s2s {
+namespace {
+
+constexpr int kTcTile = 128;     // rows and keys of a tile
+constexpr int kTcThreads = 320;
+constexpr int kTcPanel = kTcTile * 128;  // bytes of 128 rows of 64 values
+
+template <int NP>  // panels of 64 values: head_dim <= 64 * NP
+struct TcCfg {
+  static constexpr int QB = NP * kTcPanel;  // a Q, K or V tile
+  static constexpr int STAGES = NP == 1 ? 8 : 4;
+  static constexpr int RING = 2 * QB;
+  static constexpr int POS = RING + STAGES * QB;
+  static constexpr int BARS = POS + 2 * 2 * S2S_MAX_AXES * kTcTile * 4;
+  static constexpr int NBARS = 2 * STAGES + 9;
+  static constexpr int SMEM = BARS + NBARS * 8 + 16 + 1024;  // + alignment
+};
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar,
+                                            int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
+// A [rows][64] panel in the 128-byte swizzle read along its rows as the contraction (V: keys
+// contract, values are the N extent): 64-value panels `panel` bytes apart, groups of eight
+// keys 1024 bytes apart.
+__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t panel) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+  d |= (uint64_t)((panel >> 4) & 0x3FFFu) << 16;
+  d |= (uint64_t)(1024u >> 4) << 32;
+  d |= (uint64_t)1u << 46;
+  d |= (uint64_t)2u << 61;
+  return d;
+}
+
+// Instruction descriptor: fp16 or bf16 operands, fp32 sums; B K-major, or MN-major.
+__device__ __forceinline__ uint32_t idesc_16(int M, int N, bool bf16, bool b_mn) {
+  return idesc_f16_f32(M, N) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u);
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+      "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+      "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tc_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// Values of a TMEM load are not used before this point (after the wait for the load).
+__device__ __forceinline__ void loaded(uint32_t (&r)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]),
+                      "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
+}
+
+__device__ __forceinline__ void group_sync(int id) {
+  asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
+}
+
+// PLAIN: no cap, no bias.
+template <typename T, int NP, bool PLAIN>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    k_attention_tc(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap mapQ,
+                   const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV) {
+  using C = TcCfg<NP>;
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* sQ = smem;
+  uint8_t* ring = smem + C::RING;
+  float* spos = reinterpret_cast<float*>(smem + C::POS);  // [group][buffer][axis][key]
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem + C::BARS);
+  uint64_t* kv_empty = kv_full + C::STAGES;
+  uint64_t* q_full = kv_empty + C::STAGES;  // [2], as the rest: one of each tile
+  uint64_t* s_full = q_full + 2;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_full = p_full + 2;
+  uint64_t* fin = o_full + 2;
+  uint32_t* holder = reinterpret_cast<uint32_t*>(fin + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid == 0) {
+    for (int s = 0; s < C::STAGES; s++) {
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_empty[s], 1);
+    }
+    for (int w = 0; w < 2; w++) {
+      mbar_init(&q_full[w], 1);
+      mbar_init(&s_full[w], 1);
+      mbar_init(&p_full[w], 4);
+      mbar_init(&o_full[w], 1);
+    }
+    mbar_init(fin, 1);
+    fence_barrier_init();
+    tma_prefetch_desc(&mapQ);
+    tma_prefetch_desc(&mapK);
+    tma_prefetch_desc(&mapV);
+  }
+  if (warp == 9) {
+    tmem_alloc(holder, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *holder;
+  pdl_trigger();
+  pdl_wait();
+
+  // The slots from the back: in causal order the last tiles have the most keys.
+  const int slots = gridDim.x / A.q_heads;
+  const int slot = slots - 1 - (int)(blockIdx.x / A.q_heads), h = blockIdx.x % A.q_heads;
+  const int hk = h / A.group;
+  int tile = 0;
+  const int doc = find_document(A, slot, 2 * kTcTile, 1, lane, &tile);
+  Doc D = {0, 0, 0, 0, 0};
+  if (doc >= 0) D = document(A, doc);
+  // the CTA's first query; slots behind the document's last tile have none
+  const bool any = doc >= 0 && (long long)tile * (2 * kTcTile) < D.nq;
+  const int i0 = any ? tile * (2 * kTcTile) : D.nq;
+  int rows[2], kend[2], n[2];
+#pragma unroll
+  for (int w = 0; w < 2; w++) {
+    rows[w] = max(0, min(kTcTile, D.nq - i0 - w * kTcTile));
+    kend[w] = rows[w] > 0 ? seen(A, D, i0 + w * kTcTile + rows[w] - 1) : 0;
+    n[w] = (kend[w] + kTcTile - 1) / kTcTile;
+  }
+  const int N = max(n[0], n[1]), kmax = max(kend[0], kend[1]);
+  const int ksteps = (A.head_dim + 15) / 16;
+
+  if (warp == 8) {
+    if (lane == 0) {
+      // ------------------------------------------------------------------ loads
+      auto load = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int head, int row) {
+        mbar_arrive_expect_tx(bar, C::QB);
+#pragma unroll
+        for (int p = 0; p < NP; p++) tma_load_3d(dst + p * kTcPanel, map, bar, p * 64, head, row);
+      };
+      for (int w = 0; w < 2; w++)
+        if (n[w] > 0) load(sQ + w * C::QB, &mapQ, &q_full[w], h, D.q0 + i0 + w * kTcTile);
+      bool ok = true;
+      int it = 0;
+      for (; it < 2 * N; it++) {
+        const int s = it % C::STAGES;
+        if (it >= C::STAGES) ok = mbar_wait(&kv_empty[s], ((it / C::STAGES) - 1) & 1, DEV_TIMEOUT_EMPTY);
+        if (!ok) break;
+        load(ring + s * C::QB, it & 1 ? &mapV : &mapK, &kv_full[s], hk, D.k0 + (it >> 1) * kTcTile);
+      }
+      // no copy is in flight when the CTA ends, also where a wait gave up
+      for (int w = 0; w < 2; w++)
+        if (n[w] > 0) mbar_wait(&q_full[w], 0, DEV_TIMEOUT_FULL);
+      for (int k = max(0, it - C::STAGES); k < it; k++)
+        mbar_wait(&kv_full[k % C::STAGES], (k / C::STAGES) & 1, DEV_TIMEOUT_FULL);
+    }
+  } else if (warp == 9) {
+    // --------------------------------------------------------------------- MMAs
+    const uint32_t id_s = idesc_16(128, 128, BF16, false);
+    const uint32_t id_o = idesc_16(128, ksteps * 16, BF16, true);
+    bool ok = true;
+    auto arrived = [&](int it) {
+      ok = ok && mbar_wait(&kv_full[it % C::STAGES], (it / C::STAGES) & 1, DEV_TIMEOUT_FULL);
+      tc_fence_after();
+    };
+    auto scores = [&](int w, int i) {
+      if (lane == 0) {
+        const uint32_t q = smem_u32(sQ + w * C::QB), k = smem_u32(ring + ((2 * i) % C::STAGES) * C::QB);
+#pragma unroll
+        for (int c = 0; c < 4 * NP; c++) {
+          if (c >= ksteps) break;
+          const uint32_t at = (c >> 2) * kTcPanel + (c & 3) * 32;
+          tc_mma_f16(tmem + w * 128, sw128_desc(q + at), sw128_desc(k + at), id_s, c != 0);
+        }
+        tc_commit(&s_full[w]);
+      }
+      __syncwarp();
+    };
+    if (N > 0) {
+      arrived(0);
+      for (int w = 0; w < 2 && ok; w++)
+        if (n[w] > 0) {
+          ok = mbar_wait(&q_full[w], 0, DEV_TIMEOUT_FULL);
+          tc_fence_after();
+          if (ok) scores(w, 0);
+        }
+      if (ok && lane == 0) tc_commit(&kv_empty[0]);
+    }
+    for (int i = 0; i < N && ok; i++) {
+      const int vs = (2 * i + 1) % C::STAGES;
+      arrived(2 * i + 1);
+      if (!ok) break;
+      // keys that no row sees, and rows of other documents behind them, have zero weights:
+      // what lies there must not reach the product
+      const int valid = min(kTcTile, kmax - i * kTcTile), vsteps = (valid + 15) / 16;
+      if (valid & 15) {
+        for (int p = 0; p < NP; p++)
+          for (int c = lane; c < (vsteps * 16 - valid) * 8; c += 32)
+            *reinterpret_cast<uint4*>(ring + vs * C::QB + p * kTcPanel + valid * 128 + c * 16) =
+                make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      for (int w = 0; w < 2 && ok; w++) {
+        if (i < n[w]) {
+          ok = mbar_wait(&p_full[w], i & 1, DEV_TIMEOUT_ACC);
+          tc_fence_after();
+          if (!ok) break;
+          if (lane == 0) {
+            const uint32_t v = smem_u32(ring + vs * C::QB);
+#pragma unroll
+            for (int c = 0; c < 8; c++) {
+              if (c >= vsteps) break;
+              tc_mma_f16_ta(tmem + 256 + w * 128, tmem + w * 128 + c * 8, sw128_mn_desc(v + c * 2048, kTcPanel),
+                            id_o, (i | c) != 0);
+            }
+            if (i == n[w] - 1) tc_commit(&o_full[w]);
+          }
+          __syncwarp();
+        }
+        if (w == 1 && lane == 0) tc_commit(&kv_empty[vs]);
+        if (i + 1 < N && w == 0) arrived(2 * i + 2);
+        if (ok && i + 1 < n[w]) scores(w, i + 1);
+      }
+      if (ok && i + 1 < N && lane == 0) tc_commit(&kv_empty[(2 * i + 2) % C::STAGES]);
+    }
+    // TMEM is freed when every MMA has retired
+    if (lane == 0) {
+      tc_commit(fin);
+      mbar_wait(fin, 0, DEV_TIMEOUT_ACC);
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax
+    const int w = warp >> 2, r = tid & 127;
+    const int rows_w = w ? rows[1] : rows[0], n_w = w ? n[1] : n[0];
+    const int i = i0 + w * kTcTile + r;       // this thread's query
+    const bool live = r < rows_w;
+    const int mine = live ? seen(A, D, i) : 0;
+    const int open = rows_w > 0 ? seen(A, D, i0 + w * kTcTile) : 0;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t ts = lanes + w * 128, to = lanes + 256 + w * 128;
+    const float scale2 = A.scale * kLog2e, cap2 = A.cap * kLog2e;
+    const float to_cap = A.cap > 0.0f ? A.scale / A.cap : 0.0f;
+    bool ok = true;
+    float m = -INFINITY, l = 0.0f;
+
+    // bias: slope times position for this row's query (from the CTA's first query on) and,
+    // in shared memory, for the keys of a tile, each loaded a tile ahead by one thread
+    float qf[S2S_MAX_AXES], slope[S2S_MAX_AXES];
+    int ref[S2S_MAX_AXES], kraw[S2S_MAX_AXES];
+    float* pos = spos + w * 2 * S2S_MAX_AXES * kTcTile;
+    auto key_positions = [&](int t) {
+      const int j = t * kTcTile + r;
+#pragma unroll
+      for (int a = 0; a < S2S_MAX_AXES; a++)
+        if (a < A.axes) kraw[a] = j < D.nk ? A.kpos[(int64_t)a * A.kv_tokens + D.k0 + j] : ref[a];
+    };
+    if (!PLAIN && n_w > 0) {
+#pragma unroll
+      for (int a = 0; a < S2S_MAX_AXES; a++)
+        if (a < A.axes) {
+          const int* qa = A.qpos + (int64_t)a * A.q_tokens + D.q0;
+          ref[a] = qa[i0];
+          slope[a] = fabsf(A.slopes[a * A.q_heads + h]) * kLog2e;
+          qf[a] = slope[a] * (float)(int)((unsigned)qa[live ? i : i0] - (unsigned)ref[a]);
+        }
+      key_positions(0);
+    }
+
+    for (int t = 0; t < n_w; t++) {
+      const float* kp = pos + (t & 1) * S2S_MAX_AXES * kTcTile;
+      if (!PLAIN && A.axes) {
+#pragma unroll
+        for (int a = 0; a < S2S_MAX_AXES; a++)
+          if (a < A.axes)
+            const_cast<float*>(kp)[a * kTcTile + r] = slope[a] * (float)(int)((unsigned)kraw[a] - (unsigned)ref[a]);
+        group_sync(1 + w);
+        if (t + 1 < n_w) key_positions(t + 1);
+      }
+      // after a wait that gave up the group goes on without waiting, so that its four warps
+      // still meet at their barrier
+      if (ok) ok = mbar_wait(&s_full[w], t & 1, DEV_TIMEOUT_ACC);
+      tc_fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; c++) tmem_ld32_nw(ts + c * 32, s[c]);
+      tc_wait_ld();
+#pragma unroll
+      for (int c = 0; c < 4; c++) loaded(s[c]);
+      auto at = [&](int j) -> float { return __uint_as_float(s[j >> 5][j & 31]); };
+      auto set = [&](int j, float x) { s[j >> 5][j & 31] = __float_as_uint(x); };
+
+      if (!PLAIN) {
+        // scores in units of log 2
+        if (A.cap > 0.0f) {
+#pragma unroll
+          for (int j = 0; j < 128; j += 4) {
+            float x[4] = {at(j), at(j + 1), at(j + 2), at(j + 3)};
+            capped(x, to_cap, cap2);
+#pragma unroll
+            for (int e = 0; e < 4; e++) set(j + e, x[e]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 128; j++) set(j, at(j) * scale2);
+        }
+#pragma unroll
+        for (int a = 0; a < S2S_MAX_AXES; a++)
+          if (a < A.axes) {
+#pragma unroll
+            for (int j = 0; j < 128; j += 4) {
+              const float4 k = *reinterpret_cast<const float4*>(kp + a * kTcTile + j);
+              set(j, at(j) - fabsf(qf[a] - k.x));
+              set(j + 1, at(j + 1) - fabsf(qf[a] - k.y));
+              set(j + 2, at(j + 2) - fabsf(qf[a] - k.z));
+              set(j + 3, at(j + 3) - fabsf(qf[a] - k.w));
+            }
+          }
+      }
+      if ((t + 1) * kTcTile > open) {
+        const int last = mine - t * kTcTile;
+#pragma unroll
+        for (int j = 0; j < 128; j++)
+          if (j >= last) set(j, -INFINITY);
+      }
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int j = 0; j < 128; j++) top[j & 3] = fmaxf(top[j & 3], at(j));
+      float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      const float unit = PLAIN ? scale2 : 1.0f;
+      high *= unit;
+      if (t == 0) {
+        m = high;
+      } else if (__any_sync(0xffffffffu, high > m + 8.0f)) {
+        const float next = fmaxf(m, high), keep = next == -INFINITY ? 1.0f : ex2(m - next);
+        m = next;
+        l *= keep;
+        for (int c = 0; c < ksteps * 16; c += 16) {
+          uint32_t o[16];
+          tmem_ld16(to + c, o);
+#pragma unroll
+          for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+          tmem_st16(to + c, o);
+        }
+      }
+      const float base = m == -INFINITY ? 0.0f : m;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        uint32_t p[32];
+#pragma unroll
+        for (int j = 0; j < 32; j++) {
+          const float x = ex2(fmaf(at(64 * c + 2 * j), unit, -base));
+          const float y = ex2(fmaf(at(64 * c + 2 * j + 1), unit, -base));
+          sum[(2 * j) & 3] += x;
+          sum[(2 * j + 1) & 3] += y;
+          p[j] = pack2<T>(x, y);
+        }
+        tmem_st32(ts + c * 32, p);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[w]);
+    }
+
+    // ------------------------------------------------------------------- output
+    if (n_w > 0 && ok) ok = mbar_wait(&o_full[w], 0, DEV_TIMEOUT_ACC);
+    tc_fence_after();
+    const bool none = m == -INFINITY;
+    const float inv = none ? 0.0f : 1.0f / l;
+    bool bad = false;
+    T* out = static_cast<T*>(A.out.data) + (int64_t)(D.q0 + i) * A.out.token + (int64_t)h * A.out.head;
+    if (rows_w > 0)
+      for (int c = 0; c < ksteps * 16; c += 16) {
+        uint32_t o[16];
+        if (n_w > 0) tmem_ld16(to + c, o);
+        uint32_t v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float x = none ? 0.0f : __uint_as_float(o[2 * e]) * inv;
+          const float y = none ? 0.0f : __uint_as_float(o[2 * e + 1]) * inv;
+          bad = bad || !(fabsf(x) < INFINITY) || !(fabsf(y) < INFINITY);
+          v[e] = pack2<T>(x, y);
+        }
+        if (live) {
+          *reinterpret_cast<uint4*>(out + c) = make_uint4(v[0], v[1], v[2], v[3]);
+          if (c + 8 < A.head_dim) *reinterpret_cast<uint4*>(out + c + 8) = make_uint4(v[4], v[5], v[6], v[7]);
+        }
+      }
+    if (live && A.lse)
+      A.lse[(int64_t)h * A.q_tokens + D.q0 + i] = none ? -INFINITY : (m + log2f(l)) * kLn2;
+    // keys of the document that this row does not see had zero weights: a NaN or infinity
+    // among their values shows here, and the row is done again without them
+    unsigned redo = __ballot_sync(0xffffffffu, bad && live && mine < kmax);
+    __syncwarp();
+    while (redo) {
+      const int src = __ffs(redo) - 1;
+      redo &= redo - 1;
+      attend_row<T>(A, D, i0 + w * kTcTile + (warp & 3) * 32 + src, h, lane);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+// Rows of heads as a [tokens][heads][head_dim] tensor, in boxes of `rows` tokens, one head and
+// 64 values (zeros beyond head_dim and beyond the tokens).
+inline bool make_map_heads(CUtensorMap* map, const Rows& x, bool bf16, int64_t tokens, int heads,
+                           int head_dim, int rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)heads, (cuuint64_t)tokens};
+  // a stride that is never used still has to be a valid one
+  cuuint64_t strides[2] = {(cuuint64_t)(heads > 1 ? x.head : head_dim) * 2,
+                           (cuuint64_t)(tokens > 1 ? x.token : head_dim) * 2};
+  cuuint32_t box[3] = {64, 1, (cuuint32_t)rows};
+  cuuint32_t es[3] = {1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, x.data,
+            dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int NP, bool PLAIN>
+cudaError_t launch_attention_tc(const AttnArgs& A, cudaStream_t st) {
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  using C = TcCfg<NP>;
+  auto kernel = k_attention_tc<T, NP, PLAIN>;
+  static LaunchSetup setup;
+  int ctas = 0;
+  const cudaError_t err = resident_ctas(setup, kernel, kTcThreads, C::SMEM, &ctas);
+  if (err != cudaSuccess) return err;
+  CUtensorMap q, k, v;
+  if (!make_map_heads(&q, A.q, BF16, A.q_tokens, A.q_heads, A.head_dim, kTcTile) ||
+      !make_map_heads(&k, A.k, BF16, A.kv_tokens, A.kv_heads, A.head_dim, kTcTile) ||
+      !make_map_heads(&v, A.v, BF16, A.kv_tokens, A.kv_heads, A.head_dim, kTcTile))
+    return cudaErrorInvalidValue;
+  const long long slots = (long long)A.q_tokens / (2 * kTcTile) + A.documents;
+  const long long grid = slots * A.q_heads;
+  if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+  return launch_pdl(kernel, dim3((unsigned)grid), dim3(kTcThreads), C::SMEM, st, A, q, k, v);
+}
+
+template <typename T>
+cudaError_t launch_attention_tc(const AttnArgs& A, cudaStream_t st) {
+  const bool plain = A.cap == 0.0f && A.axes == 0;
+  if (A.head_dim <= 64)
+    return plain ? launch_attention_tc<T, 1, true>(A, st) : launch_attention_tc<T, 1, false>(A, st);
+  return plain ? launch_attention_tc<T, 2, true>(A, st) : launch_attention_tc<T, 2, false>(A, st);
+}
+
+}  // namespace
+}  // namespace s2s
