@@ -27,11 +27,14 @@ struct AttnArgs {
   const float* slopes;
   int q_tokens, kv_tokens, documents, causal, axes;
   int q_heads, kv_heads, group, head_dim;
-  int splits;  // CTAs of a cluster that share a tile's keys
+  int splits;      // CTAs of a cluster that share a tile's keys
+  int slots;       // of row tiles (find_document)
+  int cta_slots;   // slots that a CTA takes, one after the other
+  int cta_heads;   // key heads that a CTA takes, one after the other
   float scale, cap;
 };
 
-constexpr int kMaxSplits = 8;  // the portable cluster size
+constexpr int kMaxSplits = 16;  // the largest cluster
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -58,28 +61,37 @@ __device__ __forceinline__ Doc document(const AttnArgs& A, int d) {
   return D;
 }
 
-// Tiles of `rows` rows (`mult` rows a query) lie in slots: document d's tiles begin at slot
-// floor(rows before it / rows) + d, which leaves each document room for all of them without
-// a look at the others. The document of a slot by a whole warp, and the slot's tile in it;
-// -1 where there is none.
-__device__ __forceinline__ int find_document(const AttnArgs& A, int slot, int rows, int mult,
-                                             int lane, int* tile) {
+// Tiles of `rows` rows (`mult` rows a query) lie in `slots` slots: document d's tiles begin at
+// slot floor(rows before it / rows) + d, which leaves each document room for all of them
+// without a look at the others. The document of a slot, by a whole warp, and the slot's tile
+// in it; false where there is none. Documents of about one length are found at the first
+// guess, in one round of loads; others by a search of 32 places a round.
+__device__ __forceinline__ bool find_document(const AttnArgs& A, int slot, int slots, int rows,
+                                              int mult, int lane, Doc* D, int* tile) {
   auto first = [&](int d) -> long long {
     const long long q = A.qoff ? (long long)min(max(A.qoff[d], 0), A.q_tokens)
                                : (long long)d * (A.q_tokens / A.documents);
     return q * mult / rows + d;
   };
+  int d = (int)min((long long)A.documents - 1, (long long)slot * A.documents / slots);
+  *D = document(A, d);
+  const long long at = first(d), next = d + 1 < A.documents ? first(d + 1) : (long long)slot + 1;
+  if (at <= slot && slot < next) {
+    *tile = (int)(slot - at);
+    return true;
+  }
   int lo = 0, n = A.documents;  // the last d of [lo, lo + n) with first(d) <= slot
   while (n > 1) {
-    const int step = (n + 31) / 32, at = lo + lane * step;
-    const unsigned ok = __ballot_sync(0xffffffffu, lane * step < n && first(at) <= slot);
+    const int step = (n + 31) / 32, x = lo + lane * step;
+    const unsigned ok = __ballot_sync(0xffffffffu, lane * step < n && first(x) <= slot);
     const int c = max(__popc(ok) - 1, 0) * step;
     lo += c;
     n = min(step, n - c);
   }
+  *D = document(A, lo);
   const long long t = slot - first(lo);
   *tile = (int)t;
-  return t < 0 ? -1 : lo;
+  return t >= 0;
 }
 
 // Keys that query i of the document sees.
@@ -100,40 +112,58 @@ __device__ __forceinline__ float distance_bias(const AttnArgs& A, int h, int qro
   return b;
 }
 
-// Four scores s -> cap2 * tanh(s * to_cap). Up to 1, tanh x = x P(x^2) with P the polynomial
-// of degree 6 of least relative error on [0, 1] (5e-8, by the exchange algorithm); beyond,
-// 1 - 2 / (1 + e^{2x}). The second form costs two more of the special function unit's
-// operations, which softmax is bound by, so a warp takes it only where it has such a score.
-__device__ __forceinline__ float tanh_poly(float x) {
-  const float u = x * x;
-  float p = 0.0010410225950181484f;
-  p = fmaf(p, u, -0.006203379016369581f);
-  p = fmaf(p, u, 0.020289979875087738f);
-  p = fmaf(p, u, -0.05345702916383743f);
-  p = fmaf(p, u, 0.13325203955173492f);
-  p = fmaf(p, u, -0.33332839608192444f);
-  p = fmaf(p, u, 0.9999999403953552f);
-  return x * p;
+using F2 = unsigned long long;  // two fp32 lanes of the packed operations
+__device__ __forceinline__ F2 f2_both(float x) { return f2_pack(x, x); }
+
+// Scores s -> cap2 * tanh(s * to_cap). Up to 1, tanh x = x P(x^2) with P the polynomial of
+// degree 6 of least relative error on [0, 1] (5e-8, by the exchange algorithm), two scores an
+// instruction; beyond, 1 - 2 / (1 + e^{2x}). The second form costs two more operations of the
+// special function unit, which softmax is bound by, so a warp takes it only where it has such
+// a score.
+__device__ __forceinline__ F2 tanh_poly(F2 x) {
+  const F2 u = f2_mul(x, x);
+  F2 p = f2_fma(f2_both(0.0010410225950181484f), u, f2_both(-0.006203379016369581f));
+  p = f2_fma(p, u, f2_both(0.020289979875087738f));
+  p = f2_fma(p, u, f2_both(-0.05345702916383743f));
+  p = f2_fma(p, u, f2_both(0.13325203955173492f));
+  p = f2_fma(p, u, f2_both(-0.33332839608192444f));
+  p = f2_fma(p, u, f2_both(0.9999999403953552f));
+  return f2_mul(x, p);
 }
-__device__ __forceinline__ float tanh_exp(float x) {
+__device__ __forceinline__ float tanh_far(float x, float near) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(fabsf(x) * (2.0f * kLog2e))));
-  return copysignf(fmaf(-2.0f, r, 1.0f), x);
+  return fabsf(x) > 1.0f ? copysignf(fmaf(-2.0f, r, 1.0f), x) : near;
 }
-__device__ __forceinline__ void capped(float (&s)[4], float to_cap, float cap2) {
-  float x[4], far = 0.0f;
+template <int N>
+__device__ __forceinline__ void capped(float (&s)[N], float to_cap, float cap2) {
+  float far = 0.0f;
 #pragma unroll
-  for (int e = 0; e < 4; e++) {
-    x[e] = s[e] * to_cap;
-    far = fmaxf(far, fabsf(x[e]));
-  }
-  if (__any_sync(0xffffffffu, far > 1.0f)) {
+  for (int j = 0; j < N; j++) far = fmaxf(far, fabsf(s[j]));
+  const F2 t = f2_both(to_cap), c = f2_both(cap2);
+  if (__any_sync(0xffffffffu, far * to_cap > 1.0f)) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) s[e] = cap2 * (fabsf(x[e]) > 1.0f ? tanh_exp(x[e]) : tanh_poly(x[e]));
+    for (int j = 0; j < N; j += 2) {
+      const F2 x = f2_mul(f2_pack(s[j], s[j + 1]), t);
+      const float2 xs = f2_unpack(x), y = f2_unpack(tanh_poly(x));
+      s[j] = cap2 * tanh_far(xs.x, y.x);
+      s[j + 1] = cap2 * tanh_far(xs.y, y.y);
+    }
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; e++) s[e] = cap2 * tanh_poly(x[e]);
+    for (int j = 0; j < N; j += 2) {
+      const float2 y = f2_unpack(f2_mul(tanh_poly(f2_mul(f2_pack(s[j], s[j + 1]), t)), c));
+      s[j] = y.x;
+      s[j + 1] = y.y;
+    }
   }
+}
+
+// The larger of three.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 template <typename T>

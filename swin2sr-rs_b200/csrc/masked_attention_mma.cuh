@@ -104,10 +104,13 @@ struct MmaCfg {
   static constexpr int KEYS = kMmaKeys / KW;     // keys of a tile that one warp takes
   static constexpr int TILE = kMmaKeys * DP * 2; // bytes of a K or V tile
   static constexpr int POS = S2S_MAX_AXES * kMmaKeys * 4;
-  static constexpr int RING = kMmaStages * (2 * TILE + POS);
+  static constexpr int STAGE = 2 * TILE + POS;
+  static constexpr int RING = kMmaStages * STAGE;
   static constexpr int LD = DP + 4;              // floats of a joined output row
   static constexpr int JOIN = 4 * 16 * LD * 4;   // the four warps' outputs, over the ring
   static constexpr int BODY = RING > JOIN ? RING : JOIN;
+  // resident CTAs that the registers are cut to: the more, the more loads are in flight
+  static constexpr int CTAS = DP == 32 ? 4 : DP == 64 ? 3 : 2;
   static constexpr int SMEM = BODY + 4 * 16 * 8 + ROWS * 12;  // + maxima and sums, + flags
 };
 
@@ -119,267 +122,51 @@ __device__ __forceinline__ uint32_t tile_at(int r, int c) {
   return (uint32_t)(r * DP * 2 + ((c ^ x) << 4));
 }
 
+// Outputs of a head from the warps that have their rows to themselves.
+template <typename T, int DN>
+__device__ __forceinline__ void write_rows(const AttnArgs& A, const Doc& D, int hk, const float (&o)[DN][4],
+                                           const float (&m)[2], const float (&l)[2], const int (&row_q)[2],
+                                           const int (&row_h)[2], const int (&row_seen)[2],
+                                           const bool (&live)[2], int kend, int lane) {
+  const int t4 = lane & 3;
+#pragma unroll
+  for (int e = 0; e < 2; e++) {
+    const bool none = m[e] == -INFINITY;
+    const float inv = none ? 0.0f : 1.0f / l[e];
+    const int h = hk * A.group + row_h[e];
+    bool bad = false;
+    T* op = static_cast<T*>(A.out.data) + (int64_t)row_q[e] * A.out.token + (int64_t)h * A.out.head;
+#pragma unroll
+    for (int n = 0; n < DN; n++) {
+      const float x = none ? 0.0f : o[n][2 * e] * inv, y = none ? 0.0f : o[n][2 * e + 1] * inv;
+      bad = bad || !(fabsf(x) < INFINITY) || !(fabsf(y) < INFINITY);
+      if (live[e] && n * 8 < A.head_dim) *reinterpret_cast<uint32_t*>(op + n * 8 + 2 * t4) = pack2<T>(x, y);
+    }
+    if (live[e] && t4 == 0 && A.lse)
+      A.lse[(int64_t)h * A.q_tokens + row_q[e]] = none ? -INFINITY : (m[e] + log2f(l[e])) * kLn2;
+    // keys that the row does not see were multiplied by zero weights: a NaN or infinity among
+    // their values shows here, and the row is done again without them
+    const unsigned redo = __ballot_sync(0xffffffffu, bad && live[e] && row_seen[e] < kend);
+    __syncwarp();
+    for (int q = 0; q < 8; q++)
+      if (redo >> (4 * q) & 15u) {
+        const int i = __shfl_sync(0xffffffffu, row_q[e], 4 * q) - D.q0;
+        attend_row<T>(A, D, i, __shfl_sync(0xffffffffu, h, 4 * q), lane);
+      }
+  }
+}
+
+// Outputs of a head whose keys lie with several warps, and CTAs of a cluster: everything they
+// have goes through shared memory (over the ring, which is idle by then).
 template <typename T, int DP, int RW>
-__global__ void __launch_bounds__(kMmaThreads) k_attention_mma(const __grid_constant__ AttnArgs A) {
+__device__ __forceinline__ void join_rows(const AttnArgs& A, const Doc& D, int hk, uint8_t* smem,
+                                          const float (&o)[DP / 8][4], const float (&m)[2],
+                                          const float (&l)[2], long long r0, long long nrows, int kend,
+                                          int S, int split) {
   using C = MmaCfg<DP, RW>;
-  constexpr int KW = C::KW, NT = C::KEYS / 8, DN = DP / 8, DK = DP / 16;
-  extern __shared__ __align__(128) uint8_t smem[];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rw = warp % RW, kw = warp / RW, g = lane >> 2, t4 = lane & 3;
-  const int S = A.splits;
-  const int split = S > 1 ? (int)cluster_rank() : 0;
-  const unsigned item = blockIdx.x / S;
-  const int slot = item / A.kv_heads, hk = item % A.kv_heads;
-  pdl_trigger();
-  pdl_wait();
-
-  int tile;
-  const int doc = find_document(A, slot, C::ROWS, A.group, lane, &tile);
-  if (doc < 0) return;  // the same for all of a cluster
-  const Doc D = document(A, doc);
-  const long long r0 = (long long)tile * C::ROWS;  // rows of the document: query * group + head
-  const long long nrows = (long long)D.nq * A.group - r0;
-  if (nrows <= 0) return;
-  const int i_first = (int)(r0 / A.group);
-  const int i_last = min(D.nq - 1, (int)((r0 + C::ROWS - 1) / A.group));
-  const int kend = seen(A, D, i_last);           // keys that any row of the tile sees
-  const int ntiles = (kend + kMmaKeys - 1) / kMmaKeys;
-  const int tb = (int)((long long)ntiles * split / S), te = (int)((long long)ntiles * (split + 1) / S);
+  constexpr int KW = C::KW, DN = DP / 8;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int hd = A.head_dim;
-
-  // this thread's two rows
-  const T* qp[2];
-  int row_seen[2], row_q[2], row_h[2];
-  bool live[2];
-#pragma unroll
-  for (int e = 0; e < 2; e++) {
-    const long long r = r0 + rw * 16 + g + 8 * e;
-    live[e] = r - r0 < nrows;
-    const int i = live[e] ? (int)(r / A.group) : i_first;
-    row_q[e] = D.q0 + i;
-    row_h[e] = hk * A.group + (live[e] ? (int)(r - (long long)i * A.group) : 0);
-    row_seen[e] = live[e] ? seen(A, D, i) : 0;
-    qp[e] = static_cast<const T*>(A.q.data) + (int64_t)row_q[e] * A.q.token +
-            (int64_t)row_h[e] * A.q.head;
-  }
-  const int open = seen(A, D, i_first);  // every row sees the keys before this one
-
-  // bias: per axis the rows' slopes times log2 e and positions, from the tile's first query
-  float slope[2][S2S_MAX_AXES], qpos[2][S2S_MAX_AXES];
-  int ref[S2S_MAX_AXES];
-  if (A.axes) {
-#pragma unroll
-    for (int a = 0; a < S2S_MAX_AXES; a++)
-      if (a < A.axes) {
-        const int* qa = A.qpos + (int64_t)a * A.q_tokens;
-        ref[a] = qa[D.q0 + i_first];
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          slope[e][a] = fabsf(A.slopes[a * A.q_heads + row_h[e]]) * kLog2e;
-          qpos[e][a] = (float)(int)((unsigned)qa[row_q[e]] - (unsigned)ref[a]);
-        }
-      }
-  }
-
-  // K and V tiles into the ring
-  constexpr int CH = DP / 8, STEP = kMmaThreads / CH;  // chunks of a row, rows a pass
-  const int lrow = tid / CH, lch = tid % CH;
-  const bool lok = lch * 8 < hd;
-  const T* kbase = static_cast<const T*>(A.k.data) + (int64_t)D.k0 * A.k.token +
-                   (int64_t)hk * A.k.head + (lok ? lch * 8 : 0);
-  const T* vbase = static_cast<const T*>(A.v.data) + (int64_t)D.k0 * A.v.token +
-                   (int64_t)hk * A.v.head + (lok ? lch * 8 : 0);
-  auto fetch = [&](int t) {
-    const int st = (t - tb) % kMmaStages;
-    const uint32_t kd = smem_u32(smem) + st * (2 * C::TILE + C::POS), vd = kd + C::TILE;
-#pragma unroll
-    for (int r = lrow; r < kMmaKeys; r += STEP) {
-      const int j = t * kMmaKeys + r;
-      const bool ok = lok && j < kend;
-      const int64_t row = ok ? j : 0;
-      cp_async16(kd + tile_at<DP>(r, lch), kbase + row * A.k.token, ok);
-      cp_async16(vd + tile_at<DP>(r, lch), vbase + row * A.v.token, ok);
-    }
-    if (A.axes)
-      for (int u = tid; u < A.axes * kMmaKeys; u += kMmaThreads) {
-        const int a = u / kMmaKeys, j = t * kMmaKeys + u % kMmaKeys;
-        const bool ok = j < kend;
-        cp_async4(vd + C::TILE + u * 4, A.kpos + (int64_t)a * A.kv_tokens + D.k0 + (ok ? j : 0), ok);
-      }
-  };
-#pragma unroll
-  for (int s = 0; s < kMmaStages - 1; s++) {
-    if (tb + s < te) fetch(tb + s);
-    cp_async_commit();
-  }
-
-  // Q fragments straight from global memory
-  uint32_t qf[DK][4];
-#pragma unroll
-  for (int kk = 0; kk < DK; kk++)
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const int d = kk * 16 + 2 * t4 + (e >> 1) * 8;
-      qf[kk][e] = live[e & 1] && d < hd ? *reinterpret_cast<const uint32_t*>(qp[e & 1] + d) : 0u;
-    }
-
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-  float o[DN][4];
-#pragma unroll
-  for (int n = 0; n < DN; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
-  const float to_cap = A.cap > 0.0f ? A.scale / A.cap : 0.0f;
-  const float cap2 = A.cap * kLog2e, scale2 = A.scale * kLog2e;
-
-  for (int t = tb; t < te; t++) {
-    cp_async_wait<kMmaStages - 2>();
-    __syncthreads();
-    if (t + kMmaStages - 1 < te) fetch(t + kMmaStages - 1);
-    cp_async_commit();
-    const uint32_t ks = smem_u32(smem) + ((t - tb) % kMmaStages) * (2 * C::TILE + C::POS);
-    const uint32_t vs = ks + C::TILE;
-    const int j0 = t * kMmaKeys + kw * C::KEYS;
-    if (KW > 1 && j0 >= kend) continue;  // no key of this warp is seen
-
-    float s[NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-#pragma unroll
-    for (int kk = 0; kk < DK; kk++) {
-      if (kk * 16 >= hd) break;
-#pragma unroll
-      for (int n = 0; n < NT; n += 2) {
-        uint32_t b0, b1, b2, b3;
-        const int r = kw * C::KEYS + n * 8 + (lane & 7) + ((lane >> 4) << 3);
-        ldsm_x4(ks + tile_at<DP>(r, kk * 2 + ((lane >> 3) & 1)), b0, b1, b2, b3);
-        mma_tile<T>(s[n], qf[kk], b0, b1);
-        mma_tile<T>(s[n + 1], qf[kk], b2, b3);
-      }
-    }
-    // scores in units of log 2
-    if (A.cap > 0.0f) {
-#pragma unroll
-      for (int n = 0; n < NT; n++) capped(s[n], to_cap, cap2);
-    } else {
-#pragma unroll
-      for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) s[n][e] *= scale2;
-    }
-    if (A.axes) {
-      const int* kp = reinterpret_cast<const int*>(
-          smem + ((t - tb) % kMmaStages) * (2 * C::TILE + C::POS) + 2 * C::TILE);
-#pragma unroll
-      for (int a = 0; a < S2S_MAX_AXES; a++)
-        if (a < A.axes)
-#pragma unroll
-          for (int n = 0; n < NT; n++) {
-            const int2 k2 = *reinterpret_cast<const int2*>(kp + a * kMmaKeys + kw * C::KEYS + n * 8 + 2 * t4);
-            const float x0 = (float)(int)((unsigned)k2.x - (unsigned)ref[a]);
-            const float x1 = (float)(int)((unsigned)k2.y - (unsigned)ref[a]);
-            s[n][0] -= slope[0][a] * fabsf(qpos[0][a] - x0);
-            s[n][1] -= slope[0][a] * fabsf(qpos[0][a] - x1);
-            s[n][2] -= slope[1][a] * fabsf(qpos[1][a] - x0);
-            s[n][3] -= slope[1][a] * fabsf(qpos[1][a] - x1);
-          }
-    }
-    if (j0 + C::KEYS > open) {
-#pragma unroll
-      for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-          if (j0 + n * 8 + 2 * t4 + (e & 1) >= row_seen[e >> 1]) s[n][e] = -INFINITY;
-    }
-    // running maximum and sum
-    float keep[2], base[2];
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-      float top = -INFINITY;
-#pragma unroll
-      for (int n = 0; n < NT; n++) top = fmaxf(top, fmaxf(s[n][2 * e], s[n][2 * e + 1]));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      top = fmaxf(top, m[e]);
-      base[e] = top == -INFINITY ? 0.0f : top;  // a row that has seen nothing yet
-      keep[e] = ex2(m[e] - base[e]);
-      m[e] = top;
-      l[e] *= keep[e];
-    }
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        s[n][e] = ex2(s[n][e] - base[e >> 1]);
-        l[e >> 1] += s[n][e];
-      }
-    if (__any_sync(0xffffffffu, keep[0] != 1.0f || keep[1] != 1.0f)) {
-#pragma unroll
-      for (int n = 0; n < DN; n++) {
-        o[n][0] *= keep[0];
-        o[n][1] *= keep[0];
-        o[n][2] *= keep[1];
-        o[n][3] *= keep[1];
-      }
-    }
-    // O += P V; the weights are rounded to the type of v, the sum l is not
-#pragma unroll
-    for (int kk = 0; kk < NT / 2; kk++) {
-      const uint32_t a[4] = {pack2<T>(s[2 * kk][0], s[2 * kk][1]), pack2<T>(s[2 * kk][2], s[2 * kk][3]),
-                             pack2<T>(s[2 * kk + 1][0], s[2 * kk + 1][1]),
-                             pack2<T>(s[2 * kk + 1][2], s[2 * kk + 1][3])};
-#pragma unroll
-      for (int n = 0; n < DN; n += 2) {
-        if (n * 8 >= hd) break;
-        uint32_t b0, b1, b2, b3;
-        const int r = kw * C::KEYS + kk * 16 + (lane & 7) + (((lane >> 3) & 1) << 3);
-        ldsm_x4_t(vs + tile_at<DP>(r, n + (lane >> 4)), b0, b1, b2, b3);
-        mma_tile<T>(o[n], a, b0, b1);
-        mma_tile<T>(o[n + 1], a, b2, b3);
-      }
-    }
-  }
-  cp_async_wait<0>();
-#pragma unroll
-  for (int e = 0; e < 2; e++) {
-    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-  }
-
-  if (KW == 1 && S == 1) {
-    // the warp has its rows to itself
-    unsigned redo = 0;
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-      const float inv = m[e] == -INFINITY ? 0.0f : 1.0f / l[e];
-      bool bad = false;
-      T* op = static_cast<T*>(A.out.data) + (int64_t)row_q[e] * A.out.token + (int64_t)row_h[e] * A.out.head;
-#pragma unroll
-      for (int n = 0; n < DN; n++) {
-        const float x = m[e] == -INFINITY ? 0.0f : o[n][2 * e] * inv;
-        const float y = m[e] == -INFINITY ? 0.0f : o[n][2 * e + 1] * inv;
-        bad = bad || !(fabsf(x) < INFINITY) || !(fabsf(y) < INFINITY);
-        if (live[e] && n * 8 < hd) *reinterpret_cast<uint32_t*>(op + n * 8 + 2 * t4) = pack2<T>(x, y);
-      }
-      if (live[e] && t4 == 0 && A.lse)
-        A.lse[(int64_t)row_h[e] * A.q_tokens + row_q[e]] =
-            m[e] == -INFINITY ? -INFINITY : (m[e] + log2f(l[e])) * kLn2;
-      // keys that the row does not see were multiplied by zero weights: a NaN or infinity
-      // among their values shows here, and the row is done again without them
-      redo |= __ballot_sync(0xffffffffu, bad && live[e] && row_seen[e] < kend) ? 1u << e : 0u;
-      if (redo >> e & 1) {
-        const unsigned who = __ballot_sync(0xffffffffu, bad && live[e] && row_seen[e] < kend);
-        __syncwarp();
-        for (int q = 0; q < 8; q++)
-          if (who >> (4 * q) & 15u) {
-            const int src = 4 * q;
-            const int i = __shfl_sync(0xffffffffu, row_q[e], src) - D.q0;
-            attend_row<T>(A, D, i, __shfl_sync(0xffffffffu, row_h[e], src), lane);
-          }
-      }
-    }
-    return;
-  }
-
-  // Join: the warps' outputs, maxima and sums in shared memory (over the ring)
   float* part = reinterpret_cast<float*>(smem);                 // [4][16][LD]
   float2* ml = reinterpret_cast<float2*>(smem + C::BODY);       // [4][16]
   float2* mlc = ml + 64;                                        // [ROWS] of the CTA
@@ -472,6 +259,284 @@ __global__ void __launch_bounds__(kMmaThreads) k_attention_mma(const __grid_cons
 }
 
 template <typename T, int DP, int RW>
+__global__ void __launch_bounds__(kMmaThreads, MmaCfg<DP, RW>::CTAS)
+    k_attention_mma(const __grid_constant__ AttnArgs A) {
+  using C = MmaCfg<DP, RW>;
+  constexpr int KW = C::KW, NT = C::KEYS / 8, DN = DP / 8, DK = DP / 16;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rw = warp % RW, kw = warp / RW, g = lane >> 2, t4 = lane & 3;
+  const int S = A.splits;
+  const int split = S > 1 ? (int)cluster_rank() : 0;
+  const unsigned item = blockIdx.x / S, hgroups = (A.kv_heads + A.cta_heads - 1) / A.cta_heads;
+  const int hk0 = (int)(item % hgroups) * A.cta_heads;
+  const int hk1 = min(A.kv_heads, hk0 + A.cta_heads);
+  const int hd = A.head_dim;
+  const float to_cap = A.cap > 0.0f ? A.scale / A.cap : 0.0f;
+  const float cap2 = A.cap * kLog2e, scale2 = A.scale * kLog2e;
+  pdl_trigger();
+  pdl_wait();
+
+  for (int sl = 0; sl < A.cta_slots; sl++) {
+    const long long slot = (long long)(item / hgroups) * A.cta_slots + sl;
+    if (slot >= A.slots) break;
+    int tile;
+    Doc D;
+    if (!find_document(A, (int)slot, A.slots, C::ROWS, A.group, lane, &D, &tile)) continue;
+    const long long r0 = (long long)tile * C::ROWS;  // rows of the document: query * group + head
+    const long long nrows = (long long)D.nq * A.group - r0;
+    if (nrows <= 0) continue;
+    const int i_first = (int)(r0 / A.group);
+    const int i_last = min(D.nq - 1, (int)((r0 + C::ROWS - 1) / A.group));
+    const int kend = seen(A, D, i_last);   // keys that any row of the tile sees
+    const int open = seen(A, D, i_first);  // keys that every row sees
+    const int ntiles = (kend + kMmaKeys - 1) / kMmaKeys;
+    const int tb = (int)((long long)ntiles * split / S), te = (int)((long long)ntiles * (split + 1) / S);
+
+    // this thread's two rows
+    int row_seen[2], row_q[2], row_h[2];
+    bool live[2];
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const long long r = r0 + rw * 16 + g + 8 * e;
+      live[e] = r - r0 < nrows;
+      const int i = live[e] ? (int)(r / A.group) : i_first;
+      row_q[e] = D.q0 + i;
+      row_h[e] = live[e] ? (int)(r - (long long)i * A.group) : 0;  // within the key head
+      row_seen[e] = live[e] ? seen(A, D, i) : 0;
+    }
+
+    // bias: positions count from the tile's first query, so that near ones are exact
+    float qpos[2][S2S_MAX_AXES];
+    int ref[S2S_MAX_AXES];
+    if (A.axes) {
+#pragma unroll
+      for (int a = 0; a < S2S_MAX_AXES; a++)
+        if (a < A.axes) {
+          const int* qa = A.qpos + (int64_t)a * A.q_tokens;
+          ref[a] = qa[D.q0 + i_first];
+#pragma unroll
+          for (int e = 0; e < 2; e++) qpos[e][a] = (float)(int)((unsigned)qa[row_q[e]] - (unsigned)ref[a]);
+        }
+    }
+
+    // K and V tiles of head after head into the ring; the key positions of a tile, as fp32,
+    // through registers a tile later
+    constexpr int CH = DP / 8, STEP = kMmaThreads / CH;  // chunks of a row, rows a pass
+    const int lrow = tid / CH, lch = tid % CH;
+    const bool lok = lch * 8 < hd;
+    int ft = tb, fh = hk0, fstage = 0;  // the next tile to fetch
+    int kraw[2];
+    auto fetch = [&]() {
+      if (fh < hk1 && tb < te) {
+        const uint32_t kd = smem_u32(smem) + fstage * C::STAGE, vd = kd + C::TILE;
+        const T* kbase = static_cast<const T*>(A.k.data) + (int64_t)D.k0 * A.k.token +
+                         (int64_t)fh * A.k.head + (lok ? lch * 8 : 0);
+        const T* vbase = static_cast<const T*>(A.v.data) + (int64_t)D.k0 * A.v.token +
+                         (int64_t)fh * A.v.head + (lok ? lch * 8 : 0);
+#pragma unroll
+        for (int r = lrow; r < kMmaKeys; r += STEP) {
+          const int j = ft * kMmaKeys + r;
+          const bool ok = lok && j < kend;
+          const int64_t row = ok ? j : 0;
+          cp_async16(kd + tile_at<DP>(r, lch), kbase + row * A.k.token, ok);
+          cp_async16(vd + tile_at<DP>(r, lch), vbase + row * A.v.token, ok);
+        }
+        if (A.axes)
+#pragma unroll
+          for (int x = 0; x < 2; x++) {
+            const int u = tid + x * kMmaThreads, a = u / kMmaKeys, j = ft * kMmaKeys + u % kMmaKeys;
+            if (a < A.axes) kraw[x] = A.kpos[(int64_t)a * A.kv_tokens + D.k0 + min(j, kend - 1)];
+          }
+      }
+      cp_async_commit();
+    };
+    auto fetched = [&]() {  // the positions of the tile last fetched
+      if (fh < hk1 && tb < te) {
+        if (A.axes) {
+          float* kp = reinterpret_cast<float*>(smem + fstage * C::STAGE + 2 * C::TILE);
+#pragma unroll
+          for (int x = 0; x < 2; x++) {
+            const int u = tid + x * kMmaThreads, a = u / kMmaKeys;
+            if (a < A.axes) {
+              const int rf = a == 0 ? ref[0] : a == 1 ? ref[1] : ref[2];
+              kp[u] = (float)(int)((unsigned)kraw[x] - (unsigned)rf);
+            }
+          }
+        }
+        if (++ft == te) {
+          ft = tb;
+          fh++;
+        }
+        fstage = fstage + 1 == kMmaStages ? 0 : fstage + 1;
+      }
+    };
+    // Q fragments of a head straight from global memory
+    uint32_t qf[DK][4], qnext[DK][4];
+    auto load_q = [&](int hk) {
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const T* qp = static_cast<const T*>(A.q.data) + (int64_t)row_q[e] * A.q.token +
+                      (int64_t)(hk * A.group + row_h[e]) * A.q.head;
+#pragma unroll
+        for (int kk = 0; kk < DK; kk++)
+#pragma unroll
+          for (int x = 0; x < 2; x++) {
+            const int d = kk * 16 + 2 * t4 + x * 8;
+            qnext[kk][e + 2 * x] = live[e] && d < hd ? *reinterpret_cast<const uint32_t*>(qp + d) : 0u;
+          }
+      }
+    };
+    __syncthreads();  // the ring is free
+    load_q(hk0);
+#pragma unroll
+    for (int s = 0; s < kMmaStages - 1; s++) {
+      fetch();
+      fetched();
+    }
+
+    int stage = 0;
+    for (int hk = hk0; hk < hk1; hk++) {
+#pragma unroll
+      for (int kk = 0; kk < DK; kk++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) qf[kk][e] = qnext[kk][e];
+      if constexpr (KW == 1)
+        if (hk + 1 < hk1) load_q(hk + 1);
+      float slope[2][S2S_MAX_AXES];
+#pragma unroll
+      for (int a = 0; a < S2S_MAX_AXES; a++)
+        if (a < A.axes)
+#pragma unroll
+          for (int e = 0; e < 2; e++)
+            slope[e][a] = fabsf(A.slopes[a * A.q_heads + hk * A.group + row_h[e]]) * kLog2e;
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+      float o[DN][4];
+#pragma unroll
+      for (int n = 0; n < DN; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+
+      for (int t = tb; t < te; t++, stage = stage + 1 == kMmaStages ? 0 : stage + 1) {
+        cp_async_wait<kMmaStages - 2>();
+        __syncthreads();
+        fetch();
+        const uint8_t* sp = smem + stage * C::STAGE;
+        const uint32_t ks = smem_u32(sp), vs = ks + C::TILE;
+        const int j0 = t * kMmaKeys + kw * C::KEYS;
+        if (KW == 1 || j0 < kend) {  // some key of this warp is seen
+          float s[NT][4];
+#pragma unroll
+          for (int n = 0; n < NT; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+#pragma unroll
+          for (int kk = 0; kk < DK; kk++) {
+            if (kk * 16 >= hd) break;
+#pragma unroll
+            for (int n = 0; n < NT; n += 2) {
+              uint32_t b0, b1, b2, b3;
+              const int r = kw * C::KEYS + n * 8 + (lane & 7) + ((lane >> 4) << 3);
+              ldsm_x4(ks + tile_at<DP>(r, kk * 2 + ((lane >> 3) & 1)), b0, b1, b2, b3);
+              mma_tile<T>(s[n], qf[kk], b0, b1);
+              mma_tile<T>(s[n + 1], qf[kk], b2, b3);
+            }
+          }
+          // scores in units of log 2
+          if (A.cap > 0.0f) {
+            capped(reinterpret_cast<float (&)[NT * 4]>(s), to_cap, cap2);
+          } else {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+              for (int e = 0; e < 4; e++) s[n][e] *= scale2;
+          }
+          if (A.axes) {
+            const float* kp = reinterpret_cast<const float*>(sp + 2 * C::TILE) + kw * C::KEYS + 2 * t4;
+#pragma unroll
+            for (int a = 0; a < S2S_MAX_AXES; a++)
+              if (a < A.axes) {
+                // |slope| |q - k| as |slope q - slope k|
+                const F2 s0 = f2_both(-slope[0][a]), s1 = f2_both(-slope[1][a]);
+                const F2 q0 = f2_both(slope[0][a] * qpos[0][a]), q1 = f2_both(slope[1][a] * qpos[1][a]);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                  const F2 k2 = *reinterpret_cast<const F2*>(kp + a * kMmaKeys + n * 8);
+                  const float2 d0 = f2_unpack(f2_fma(k2, s0, q0)), d1 = f2_unpack(f2_fma(k2, s1, q1));
+                  s[n][0] -= fabsf(d0.x);
+                  s[n][1] -= fabsf(d0.y);
+                  s[n][2] -= fabsf(d1.x);
+                  s[n][3] -= fabsf(d1.y);
+                }
+              }
+          }
+          if (j0 + C::KEYS > open) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+              for (int e = 0; e < 4; e++)
+                if (j0 + n * 8 + 2 * t4 + (e & 1) >= row_seen[e >> 1]) s[n][e] = -INFINITY;
+          }
+          // running maximum and sum
+          float keep[2], base[2];
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            float top = m[e];
+#pragma unroll
+            for (int n = 0; n < NT; n++) top = max3(top, s[n][2 * e], s[n][2 * e + 1]);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            base[e] = top == -INFINITY ? 0.0f : top;  // a row that has seen nothing yet
+            keep[e] = ex2(m[e] - base[e]);
+            m[e] = top;
+            l[e] *= keep[e];
+          }
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              s[n][e] = ex2(s[n][e] - base[e >> 1]);
+              l[e >> 1] += s[n][e];
+            }
+          if (__any_sync(0xffffffffu, keep[0] != 1.0f || keep[1] != 1.0f)) {
+#pragma unroll
+            for (int n = 0; n < DN; n++) {
+              o[n][0] *= keep[0];
+              o[n][1] *= keep[0];
+              o[n][2] *= keep[1];
+              o[n][3] *= keep[1];
+            }
+          }
+          // O += P V; the weights are rounded to the type of v, the sum l is not
+#pragma unroll
+          for (int kk = 0; kk < NT / 2; kk++) {
+            const uint32_t a[4] = {
+                pack2<T>(s[2 * kk][0], s[2 * kk][1]), pack2<T>(s[2 * kk][2], s[2 * kk][3]),
+                pack2<T>(s[2 * kk + 1][0], s[2 * kk + 1][1]), pack2<T>(s[2 * kk + 1][2], s[2 * kk + 1][3])};
+#pragma unroll
+            for (int n = 0; n < DN; n += 2) {
+              if (n * 8 >= hd) break;
+              uint32_t b0, b1, b2, b3;
+              const int r = kw * C::KEYS + kk * 16 + (lane & 7) + (((lane >> 3) & 1) << 3);
+              ldsm_x4_t(vs + tile_at<DP>(r, n + (lane >> 4)), b0, b1, b2, b3);
+              mma_tile<T>(o[n], a, b0, b1);
+              mma_tile<T>(o[n + 1], a, b2, b3);
+            }
+          }
+        }
+        fetched();
+      }
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+      }
+      if (KW == 1 && S == 1)
+        write_rows<T, DN>(A, D, hk, o, m, l, row_q, row_h, row_seen, live, kend, lane);
+      else  // one head (cta_heads is 1)
+        join_rows<T, DP, RW>(A, D, hk, smem, o, m, l, r0, nrows, kend, S, split);
+    }
+    cp_async_wait<0>();
+  }
+}
+
+template <typename T, int DP, int RW>
 cudaError_t launch_attention_mma(AttnArgs& A, cudaStream_t st) {
   using C = MmaCfg<DP, RW>;
   auto kernel = k_attention_mma<T, DP, RW>;
@@ -479,15 +544,28 @@ cudaError_t launch_attention_mma(AttnArgs& A, cudaStream_t st) {
   int ctas = 0;
   cudaError_t err = resident_ctas(setup, kernel, kMmaThreads, C::SMEM, &ctas);
   if (err != cudaSuccess) return err;
-  const long long slots = (long long)A.q_tokens * A.group / C::ROWS + A.documents;
-  const long long items = slots * A.kv_heads;
-  // Few tiles with many keys: the keys of a tile are split over a cluster, until the CTAs
-  // fill the device or have two key tiles each (by the mean length: the host does not know
-  // the offsets).
+  const long long rows = (long long)A.q_tokens * A.group;
+  const long long slots = rows / C::ROWS + A.documents;
+  // The host knows mean lengths only: documents shorter than a tile have two slots each, of
+  // which one is empty, and share a CTA.
+  A.cta_slots = rows <= (long long)A.documents * C::ROWS ? 2 : 1;
+  A.slots = (int)slots;
+  const long long groups = (slots + A.cta_slots - 1) / A.cta_slots;
+  // The keys of a tile are split over a cluster while each part has two tiles or more by the
+  // mean length, until there are eight times the CTAs that fit on the device: documents of
+  // very different lengths then even out.
   const long long keys = A.kv_tokens / A.documents;
   int splits = 1;
-  while (splits < kMaxSplits && items * splits * 2 <= ctas && keys >= 4LL * kMmaKeys * splits) splits *= 2;
+  while (splits < kMaxSplits && groups * A.kv_heads * splits <= 4LL * ctas &&
+         keys >= 4LL * kMmaKeys * splits)
+    splits *= 2;
   A.splits = splits;
+  // many tiles: a CTA takes several heads of a tile, the next head's loads under way while it
+  // computes, as long as three rounds of CTAs are left
+  A.cta_heads = 1;
+  if (C::KW == 1 && splits == 1)
+    A.cta_heads = (int)std::max(1LL, std::min((long long)A.kv_heads, groups * A.kv_heads / (3LL * ctas)));
+  const long long items = groups * ((A.kv_heads + A.cta_heads - 1) / A.cta_heads);
   const long long grid = items * splits;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg;
@@ -502,6 +580,10 @@ cudaError_t launch_attention_mma(AttnArgs& A, cudaStream_t st) {
     attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[n++].val.programmaticStreamSerializationAllowed = 1;
   }
+  if (splits > 8) {  // beyond the portable size
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (err != cudaSuccess) return err;
+  }
   if (splits > 1) {
     attr[n].id = cudaLaunchAttributeClusterDimension;
     attr[n].val.clusterDim.x = splits;
@@ -515,10 +597,13 @@ cudaError_t launch_attention_mma(AttnArgs& A, cudaStream_t st) {
 
 template <typename T, int DP>
 cudaError_t launch_attention_mma(AttnArgs& A, cudaStream_t st) {
-  const long long rows = (long long)A.q_tokens * A.group / A.documents;
-  return rows <= 16   ? launch_attention_mma<T, DP, 1>(A, st)
-         : rows <= 32 ? launch_attention_mma<T, DP, 2>(A, st)
-                      : launch_attention_mma<T, DP, 4>(A, st);
+  // The fewest row warps that hold the mean document's rows; fewer still where the tiles, split
+  // as far as they go, would not fill the device (K and V are then read again, from L2).
+  const long long rows = (long long)A.q_tokens * A.group, mean = rows / A.documents;
+  auto ctas = [&](int n) { return (rows / n + A.documents) * A.kv_heads * kMaxSplits; };
+  if (mean <= 16 || ctas(32) < 148) return launch_attention_mma<T, DP, 1>(A, st);
+  if (mean <= 32 || ctas(64) < 148) return launch_attention_mma<T, DP, 2>(A, st);
+  return launch_attention_mma<T, DP, 4>(A, st);
 }
 
 template <typename T>

@@ -150,15 +150,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   pdl_wait();
 
   // The slots from the back: in causal order the last tiles have the most keys.
-  const int slots = gridDim.x / A.q_heads;
-  const int slot = slots - 1 - (int)(blockIdx.x / A.q_heads), h = blockIdx.x % A.q_heads;
+  const int slot = A.slots - 1 - (int)(blockIdx.x / A.q_heads), h = blockIdx.x % A.q_heads;
   const int hk = h / A.group;
   int tile = 0;
-  const int doc = find_document(A, slot, 2 * kTcTile, 1, lane, &tile);
-  Doc D = {0, 0, 0, 0, 0};
-  if (doc >= 0) D = document(A, doc);
+  Doc D;
   // the CTA's first query; slots behind the document's last tile have none
-  const bool any = doc >= 0 && (long long)tile * (2 * kTcTile) < D.nq;
+  const bool any = find_document(A, slot, A.slots, 2 * kTcTile, 1, lane, &D, &tile) &&
+                   (long long)tile * (2 * kTcTile) < D.nq;
   const int i0 = any ? tile * (2 * kTcTile) : D.nq;
   int rows[2], kend[2], n[2];
 #pragma unroll
@@ -334,11 +332,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // scores in units of log 2
         if (A.cap > 0.0f) {
 #pragma unroll
-          for (int j = 0; j < 128; j += 4) {
-            float x[4] = {at(j), at(j + 1), at(j + 2), at(j + 3)};
+          for (int c = 0; c < 4; c++) {
+            float x[32];
+#pragma unroll
+            for (int e = 0; e < 32; e++) x[e] = __uint_as_float(s[c][e]);
             capped(x, to_cap, cap2);
 #pragma unroll
-            for (int e = 0; e < 4; e++) set(j + e, x[e]);
+            for (int e = 0; e < 32; e++) s[c][e] = __float_as_uint(x[e]);
           }
         } else {
 #pragma unroll
@@ -465,7 +465,7 @@ inline bool make_map_heads(CUtensorMap* map, const Rows& x, bool bf16, int64_t t
 }
 
 template <typename T, int NP, bool PLAIN>
-cudaError_t launch_attention_tc(const AttnArgs& A, cudaStream_t st) {
+cudaError_t launch_attention_tc(AttnArgs& A, cudaStream_t st) {
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   using C = TcCfg<NP>;
   auto kernel = k_attention_tc<T, NP, PLAIN>;
@@ -481,11 +481,12 @@ cudaError_t launch_attention_tc(const AttnArgs& A, cudaStream_t st) {
   const long long slots = (long long)A.q_tokens / (2 * kTcTile) + A.documents;
   const long long grid = slots * A.q_heads;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+  A.slots = (int)slots;
   return launch_pdl(kernel, dim3((unsigned)grid), dim3(kTcThreads), C::SMEM, st, A, q, k, v);
 }
 
 template <typename T>
-cudaError_t launch_attention_tc(const AttnArgs& A, cudaStream_t st) {
+cudaError_t launch_attention_tc(AttnArgs& A, cudaStream_t st) {
   const bool plain = A.cap == 0.0f && A.axes == 0;
   if (A.head_dim <= 64)
     return plain ? launch_attention_tc<T, 1, true>(A, st) : launch_attention_tc<T, 1, false>(A, st);
