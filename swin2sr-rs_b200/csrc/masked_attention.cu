@@ -166,6 +166,15 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar,
+                                            int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
 template <typename T>
 __device__ __forceinline__ float4 load4(const T* p) {
   const uint2 u = *reinterpret_cast<const uint2*>(p);
@@ -177,7 +186,7 @@ __device__ __forceinline__ float4 load4(const T* p) {
 // 4l .. 4l + 3 of the head. For rows that a tile cannot do: it multiplies the values of
 // keys that a row does not see by zero weights, and zero times NaN or infinity is NaN.
 template <typename T>
-__device__ __noinline__ void attend_row(const AttnArgs& A, const Doc& D, int i, int h, int lane) {
+__device__ __noinline__ void attend_row(const AttnArgs& A, const Doc D, int i, int h, int lane) {
   const int qrow = D.q0 + i, hk = h / A.group, d = lane * 4;
   const bool mine = d < A.head_dim;
   const T* k = static_cast<const T*>(A.k.data) + (int64_t)hk * A.k.head + d;
@@ -225,6 +234,25 @@ __device__ __noinline__ void attend_row(const AttnArgs& A, const Doc& D, int i, 
   }
   if (A.lse && lane == 0)
     A.lse[(int64_t)h * A.q_tokens + qrow] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+// Rows of heads as a [tokens][heads][head_dim] tensor, in boxes of `rows` tokens, one head and
+// `cols` values (32 or 64; zeros beyond head_dim and beyond the tokens), swizzled over the box's
+// rows of 64 or 128 bytes.
+inline bool make_map_heads(CUtensorMap* map, const Rows& x, bool bf16, int64_t tokens, int heads,
+                           int head_dim, int rows, int cols) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)heads, (cuuint64_t)tokens};
+  // a stride that is never used still has to be a valid one
+  cuuint64_t strides[2] = {(cuuint64_t)(heads > 1 ? x.head : head_dim) * 2,
+                           (cuuint64_t)(tokens > 1 ? x.token : head_dim) * 2};
+  cuuint32_t box[3] = {(cuuint32_t)cols, 1, (cuuint32_t)rows};
+  cuuint32_t es[3] = {1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, x.data,
+            dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace

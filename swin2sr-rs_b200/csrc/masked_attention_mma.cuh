@@ -3,7 +3,7 @@
 //
 // A CTA of four warps takes 16 * RW rows of one document and key head - a row is a query and
 // one of the query heads that share the key head, so K and V are read once for all of them -
-// and walks the keys in tiles of 64 through a ring of three cp.async stages. RW warps lie
+// and walks the keys in tiles of 64 through a ring of three stages that TMA fills. RW warps lie
 // along the rows, 4 / RW along the keys of a tile: one query of eight heads is one row tile,
 // whose keys the four warps share. Every warp keeps a running maximum, sum and output of its
 // own; they are joined once at the end, first within the CTA, then over the CTAs of a cluster
@@ -48,25 +48,6 @@ __device__ __forceinline__ void mma_tile<__nv_bfloat16>(float (&c)[4], const uin
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// 16 bytes global -> shared, zeros where `ok` is false (the source is not read then).
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst),
-               "l"(reinterpret_cast<uint64_t>(src)), "r"(ok ? 16 : 0)
-               : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst),
-               "l"(reinterpret_cast<uint64_t>(src)), "r"(ok ? 4 : 0)
-               : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() {
-  asm volatile("cp.async.commit_group;" ::: "memory");
-}
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // ------------------------------------------------------------------------- clusters
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -102,24 +83,27 @@ struct MmaCfg {
   static constexpr int KW = 4 / RW;              // warps along the keys
   static constexpr int ROWS = 16 * RW;
   static constexpr int KEYS = kMmaKeys / KW;     // keys of a tile that one warp takes
-  static constexpr int TILE = kMmaKeys * DP * 2; // bytes of a K or V tile
-  static constexpr int POS = S2S_MAX_AXES * kMmaKeys * 4;
-  static constexpr int STAGE = 2 * TILE + POS;
-  static constexpr int RING = kMmaStages * STAGE;
+  static constexpr int PV = DP < 64 ? DP : 64;   // values of a panel: a TMA box's row
+  static constexpr int PANEL = kMmaKeys * PV * 2;
+  static constexpr int TILE = kMmaKeys * DP * 2; // bytes of a K or V tile, panel after panel
+  static constexpr int RING = kMmaStages * 2 * TILE;
   static constexpr int LD = DP + 4;              // floats of a joined output row
   static constexpr int JOIN = 4 * 16 * LD * 4;   // the four warps' outputs, over the ring
   static constexpr int BODY = RING > JOIN ? RING : JOIN;
+  static constexpr int POS = S2S_MAX_AXES * kMmaKeys * 4;  // key positions of a stage
+  static constexpr int BARS = BODY + kMmaStages * POS;
+  static constexpr int ENDS = BARS + kMmaStages * 8 + 8;   // maxima and sums, flags
+  static constexpr int SMEM = ENDS + 4 * 16 * 8 + ROWS * 12 + 1024;  // + alignment
   // resident CTAs that the registers are cut to: the more, the more loads are in flight
   static constexpr int CTAS = DP == 32 ? 4 : DP == 64 ? 3 : 2;
-  static constexpr int SMEM = BODY + 4 * 16 * 8 + ROWS * 12;  // + maxima and sums, + flags
 };
 
-// Byte offset of 16-byte chunk `c` of row `r` in a [rows][DP] tile: the chunks of a row are
-// permuted so that eight rows' equal chunks lie in different banks.
+// Where lane `lane` finds, in a tile, chunk `b` (16 bytes) of row `r`; chunk b + 2k of the same
+// panel is at this offset ^ (32 k), as the swizzle permutes the chunks of a row by exclusive or.
 template <int DP>
-__device__ __forceinline__ uint32_t tile_at(int r, int c) {
-  const int x = DP == 32 ? (r >> 1) & 3 : r & 7;
-  return (uint32_t)(r * DP * 2 + ((c ^ x) << 4));
+__device__ __forceinline__ uint32_t tile_at(int r, int b) {
+  return DP == 32 ? (uint32_t)(r * 64 + ((b ^ ((r >> 1) & 3)) << 4))
+                  : (uint32_t)(r * 128 + ((b ^ (r & 7)) << 4));
 }
 
 // Outputs of a head from the warps that have their rows to themselves.
@@ -168,7 +152,7 @@ __device__ __forceinline__ void join_rows(const AttnArgs& A, const Doc& D, int h
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int hd = A.head_dim;
   float* part = reinterpret_cast<float*>(smem);                 // [4][16][LD]
-  float2* ml = reinterpret_cast<float2*>(smem + C::BODY);       // [4][16]
+  float2* ml = reinterpret_cast<float2*>(smem + C::ENDS);       // [4][16]
   float2* mlc = ml + 64;                                        // [ROWS] of the CTA
   int* flag = reinterpret_cast<int*>(mlc + C::ROWS);            // [ROWS]
   __syncthreads();
@@ -260,10 +244,14 @@ __device__ __forceinline__ void join_rows(const AttnArgs& A, const Doc& D, int h
 
 template <typename T, int DP, int RW>
 __global__ void __launch_bounds__(kMmaThreads, MmaCfg<DP, RW>::CTAS)
-    k_attention_mma(const __grid_constant__ AttnArgs A) {
+    k_attention_mma(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap mapK,
+                    const __grid_constant__ CUtensorMap mapV) {
   using C = MmaCfg<DP, RW>;
-  constexpr int KW = C::KW, NT = C::KEYS / 8, DN = DP / 8, DK = DP / 16;
-  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int KW = C::KW, NT = C::KEYS / 8, DN = DP / 8, DK = DP / 16, PK = C::PV / 16;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  float* spos = reinterpret_cast<float*>(smem + C::BODY);  // [stage][axis][key]
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BARS);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rw = warp % RW, kw = warp / RW, g = lane >> 2, t4 = lane & 3;
   const int S = A.splits;
@@ -274,8 +262,22 @@ __global__ void __launch_bounds__(kMmaThreads, MmaCfg<DP, RW>::CTAS)
   const int hd = A.head_dim;
   const float to_cap = A.cap > 0.0f ? A.scale / A.cap : 0.0f;
   const float cap2 = A.cap * kLog2e, scale2 = A.scale * kLog2e;
+  const float unit = A.cap > 0.0f || A.axes ? 1.0f : scale2;  // what scores still lack at the exponential
+  // this lane's place in the 16 x 16 blocks of K and V that ldmatrix takes
+  const uint32_t kat = tile_at<DP>(kw * C::KEYS + (lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1);
+  const uint32_t vat = tile_at<DP>(kw * C::KEYS + (lane & 7) + (((lane >> 3) & 1) << 3), lane >> 4);
+  if (tid == 0) {
+    for (int s = 0; s < kMmaStages; s++) mbar_init(&full[s], 1);
+    fence_barrier_init();
+    tma_prefetch_desc(&mapK);
+    tma_prefetch_desc(&mapV);
+  }
   pdl_trigger();
   pdl_wait();
+  // tiles fetched and computed so far; a wait that gave up is not followed by others, but the
+  // CTA's barriers are met all the same
+  uint32_t fetches = 0, steps = 0;
+  bool ok = true;
 
   for (int sl = 0; sl < A.cta_slots; sl++) {
     const long long slot = (long long)(item / hgroups) * A.cta_slots + sl;
@@ -322,53 +324,44 @@ __global__ void __launch_bounds__(kMmaThreads, MmaCfg<DP, RW>::CTAS)
 
     // K and V tiles of head after head into the ring; the key positions of a tile, as fp32,
     // through registers a tile later
-    constexpr int CH = DP / 8, STEP = kMmaThreads / CH;  // chunks of a row, rows a pass
-    const int lrow = tid / CH, lch = tid % CH;
-    const bool lok = lch * 8 < hd;
-    int ft = tb, fh = hk0, fstage = 0;  // the next tile to fetch
+    int ft = tb, fh = hk0;  // the next tile to fetch
     int kraw[2];
     auto fetch = [&]() {
-      if (fh < hk1 && tb < te) {
-        const uint32_t kd = smem_u32(smem) + fstage * C::STAGE, vd = kd + C::TILE;
-        const T* kbase = static_cast<const T*>(A.k.data) + (int64_t)D.k0 * A.k.token +
-                         (int64_t)fh * A.k.head + (lok ? lch * 8 : 0);
-        const T* vbase = static_cast<const T*>(A.v.data) + (int64_t)D.k0 * A.v.token +
-                         (int64_t)fh * A.v.head + (lok ? lch * 8 : 0);
+      if (fh >= hk1 || tb >= te) return;
+      const uint32_t st = fetches % kMmaStages;
+      if (tid == 0) {
+        uint8_t* dst = smem + st * 2 * C::TILE;
+        mbar_arrive_expect_tx(&full[st], 2 * C::TILE);
 #pragma unroll
-        for (int r = lrow; r < kMmaKeys; r += STEP) {
-          const int j = ft * kMmaKeys + r;
-          const bool ok = lok && j < kend;
-          const int64_t row = ok ? j : 0;
-          cp_async16(kd + tile_at<DP>(r, lch), kbase + row * A.k.token, ok);
-          cp_async16(vd + tile_at<DP>(r, lch), vbase + row * A.v.token, ok);
+        for (int p = 0; p < DP / C::PV; p++) {
+          tma_load_3d(dst + p * C::PANEL, &mapK, &full[st], p * C::PV, fh, D.k0 + ft * kMmaKeys);
+          tma_load_3d(dst + C::TILE + p * C::PANEL, &mapV, &full[st], p * C::PV, fh, D.k0 + ft * kMmaKeys);
         }
-        if (A.axes)
-#pragma unroll
-          for (int x = 0; x < 2; x++) {
-            const int u = tid + x * kMmaThreads, a = u / kMmaKeys, j = ft * kMmaKeys + u % kMmaKeys;
-            if (a < A.axes) kraw[x] = A.kpos[(int64_t)a * A.kv_tokens + D.k0 + min(j, kend - 1)];
-          }
       }
-      cp_async_commit();
+      if (A.axes)
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+          const int u = tid + x * kMmaThreads, a = u / kMmaKeys, j = ft * kMmaKeys + u % kMmaKeys;
+          if (a < A.axes) kraw[x] = A.kpos[(int64_t)a * A.kv_tokens + D.k0 + min(j, kend - 1)];
+        }
     };
     auto fetched = [&]() {  // the positions of the tile last fetched
-      if (fh < hk1 && tb < te) {
-        if (A.axes) {
-          float* kp = reinterpret_cast<float*>(smem + fstage * C::STAGE + 2 * C::TILE);
+      if (fh >= hk1 || tb >= te) return;
+      if (A.axes) {
+        float* kp = spos + (fetches % kMmaStages) * (S2S_MAX_AXES * kMmaKeys);
 #pragma unroll
-          for (int x = 0; x < 2; x++) {
-            const int u = tid + x * kMmaThreads, a = u / kMmaKeys;
-            if (a < A.axes) {
-              const int rf = a == 0 ? ref[0] : a == 1 ? ref[1] : ref[2];
-              kp[u] = (float)(int)((unsigned)kraw[x] - (unsigned)rf);
-            }
+        for (int x = 0; x < 2; x++) {
+          const int u = tid + x * kMmaThreads, a = u / kMmaKeys;
+          if (a < A.axes) {
+            const int rf = a == 0 ? ref[0] : a == 1 ? ref[1] : ref[2];
+            kp[u] = (float)(int)((unsigned)kraw[x] - (unsigned)rf);
           }
         }
-        if (++ft == te) {
-          ft = tb;
-          fh++;
-        }
-        fstage = fstage + 1 == kMmaStages ? 0 : fstage + 1;
+      }
+      fetches++;
+      if (++ft == te) {
+        ft = tb;
+        fh++;
       }
     };
     // Q fragments of a head straight from global memory
@@ -387,7 +380,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaCfg<DP, RW>::CTAS)
           }
       }
     };
-    __syncthreads();  // the ring is free
+    __syncthreads();  // the barriers are set up, the ring is free
     load_q(hk0);
 #pragma unroll
     for (int s = 0; s < kMmaStages - 1; s++) {
@@ -395,7 +388,6 @@ __global__ void __launch_bounds__(kMmaThreads, MmaCfg<DP, RW>::CTAS)
       fetched();
     }
 
-    int stage = 0;
     for (int hk = hk0; hk < hk1; hk++) {
 #pragma unroll
       for (int kk = 0; kk < DK; kk++)
@@ -415,40 +407,48 @@ __global__ void __launch_bounds__(kMmaThreads, MmaCfg<DP, RW>::CTAS)
 #pragma unroll
       for (int n = 0; n < DN; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
 
-      for (int t = tb; t < te; t++, stage = stage + 1 == kMmaStages ? 0 : stage + 1) {
-        cp_async_wait<kMmaStages - 2>();
-        __syncthreads();
+      for (int t = tb; t < te; t++, steps++) {
+        const uint32_t stage = steps % kMmaStages;
+        if (ok) ok = mbar_wait(&full[stage], (steps / kMmaStages) & 1, DEV_TIMEOUT_FULL);
+        const int tail = kend - t * kMmaKeys;  // keys of the tile that some row sees
+        if (tail < kMmaKeys) {
+          // behind them lie other documents' rows, or none: zero weights must not meet what is
+          // there, nor may the copies into the stage pass these writes
+          for (int u = tid; u < (kMmaKeys - tail) * (DP / 8); u += kMmaThreads) {
+            const int p = u / ((kMmaKeys - tail) * (C::PV / 8)), c = u % ((kMmaKeys - tail) * (C::PV / 8));
+            *reinterpret_cast<uint4*>(smem + stage * 2 * C::TILE + C::TILE + p * C::PANEL +
+                                      tail * C::PV * 2 + c * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
+        __syncthreads();  // everyone has left the stage that is filled now
         fetch();
-        const uint8_t* sp = smem + stage * C::STAGE;
-        const uint32_t ks = smem_u32(sp), vs = ks + C::TILE;
+        const uint32_t ks = smem_u32(smem + stage * 2 * C::TILE), vs = ks + C::TILE;
         const int j0 = t * kMmaKeys + kw * C::KEYS;
         if (KW == 1 || j0 < kend) {  // some key of this warp is seen
           float s[NT][4];
 #pragma unroll
           for (int n = 0; n < NT; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
 #pragma unroll
-          for (int kk = 0; kk < DK; kk++) {
-            if (kk * 16 >= hd) break;
+          for (int kk = 0; kk < DK; kk++)
 #pragma unroll
             for (int n = 0; n < NT; n += 2) {
               uint32_t b0, b1, b2, b3;
-              const int r = kw * C::KEYS + n * 8 + (lane & 7) + ((lane >> 4) << 3);
-              ldsm_x4(ks + tile_at<DP>(r, kk * 2 + ((lane >> 3) & 1)), b0, b1, b2, b3);
+              ldsm_x4(ks + (kk / PK) * C::PANEL + n * 8 * C::PV * 2 + (kat ^ (kk % PK * 32)), b0, b1, b2, b3);
               mma_tile<T>(s[n], qf[kk], b0, b1);
               mma_tile<T>(s[n + 1], qf[kk], b2, b3);
             }
-          }
           // scores in units of log 2
           if (A.cap > 0.0f) {
             capped(reinterpret_cast<float (&)[NT * 4]>(s), to_cap, cap2);
-          } else {
+          } else if (A.axes) {
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
               for (int e = 0; e < 4; e++) s[n][e] *= scale2;
           }
           if (A.axes) {
-            const float* kp = reinterpret_cast<const float*>(sp + 2 * C::TILE) + kw * C::KEYS + 2 * t4;
+            const float* kp = spos + stage * (S2S_MAX_AXES * kMmaKeys) + kw * C::KEYS + 2 * t4;
 #pragma unroll
             for (int a = 0; a < S2S_MAX_AXES; a++)
               if (a < A.axes) {
@@ -477,23 +477,32 @@ __global__ void __launch_bounds__(kMmaThreads, MmaCfg<DP, RW>::CTAS)
           float keep[2], base[2];
 #pragma unroll
           for (int e = 0; e < 2; e++) {
-            float top = m[e];
+            float top = -INFINITY;
 #pragma unroll
             for (int n = 0; n < NT; n++) top = max3(top, s[n][2 * e], s[n][2 * e + 1]);
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            top = fmaxf(top * unit, m[e]);
             base[e] = top == -INFINITY ? 0.0f : top;  // a row that has seen nothing yet
             keep[e] = ex2(m[e] - base[e]);
             m[e] = top;
-            l[e] *= keep[e];
           }
+          const F2 u2 = f2_both(unit), b0 = f2_both(-base[0]), b1 = f2_both(-base[1]);
+          F2 sum0 = 0, sum1 = 0;  // two zeros each
 #pragma unroll
-          for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              s[n][e] = ex2(s[n][e] - base[e >> 1]);
-              l[e >> 1] += s[n][e];
-            }
+          for (int n = 0; n < NT; n++) {
+            const float2 x = f2_unpack(f2_fma(f2_pack(s[n][0], s[n][1]), u2, b0));
+            const float2 y = f2_unpack(f2_fma(f2_pack(s[n][2], s[n][3]), u2, b1));
+            s[n][0] = ex2(x.x);
+            s[n][1] = ex2(x.y);
+            s[n][2] = ex2(y.x);
+            s[n][3] = ex2(y.y);
+            sum0 = f2_add(sum0, f2_pack(s[n][0], s[n][1]));
+            sum1 = f2_add(sum1, f2_pack(s[n][2], s[n][3]));
+          }
+          const float2 t0 = f2_unpack(sum0), t1 = f2_unpack(sum1);
+          l[0] = fmaf(l[0], keep[0], t0.x + t0.y);
+          l[1] = fmaf(l[1], keep[1], t1.x + t1.y);
           if (__any_sync(0xffffffffu, keep[0] != 1.0f || keep[1] != 1.0f)) {
 #pragma unroll
             for (int n = 0; n < DN; n++) {
@@ -511,10 +520,9 @@ __global__ void __launch_bounds__(kMmaThreads, MmaCfg<DP, RW>::CTAS)
                 pack2<T>(s[2 * kk + 1][0], s[2 * kk + 1][1]), pack2<T>(s[2 * kk + 1][2], s[2 * kk + 1][3])};
 #pragma unroll
             for (int n = 0; n < DN; n += 2) {
-              if (n * 8 >= hd) break;
               uint32_t b0, b1, b2, b3;
-              const int r = kw * C::KEYS + kk * 16 + (lane & 7) + (((lane >> 3) & 1) << 3);
-              ldsm_x4_t(vs + tile_at<DP>(r, n + (lane >> 4)), b0, b1, b2, b3);
+              ldsm_x4_t(vs + (n / (2 * PK)) * C::PANEL + kk * 16 * C::PV * 2 + (vat ^ (n % (2 * PK) * 16)), b0, b1,
+                        b2, b3);
               mma_tile<T>(o[n], a, b0, b1);
               mma_tile<T>(o[n + 1], a, b2, b3);
             }
@@ -532,7 +540,6 @@ __global__ void __launch_bounds__(kMmaThreads, MmaCfg<DP, RW>::CTAS)
       else  // one head (cta_heads is 1)
         join_rows<T, DP, RW>(A, D, hk, smem, o, m, l, r0, nrows, kend, S, split);
     }
-    cp_async_wait<0>();
   }
 }
 
@@ -592,7 +599,15 @@ cudaError_t launch_attention_mma(AttnArgs& A, cudaStream_t st) {
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  return cudaLaunchKernelEx(&cfg, kernel, A);
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  CUtensorMap k, v;
+  memset(&k, 0, sizeof k);
+  memset(&v, 0, sizeof v);
+  if (A.kv_tokens > 0 &&
+      (!make_map_heads(&k, A.k, BF16, A.kv_tokens, A.kv_heads, A.head_dim, kMmaKeys, C::PV) ||
+       !make_map_heads(&v, A.v, BF16, A.kv_tokens, A.kv_heads, A.head_dim, kMmaKeys, C::PV)))
+    return cudaErrorInvalidValue;
+  return cudaLaunchKernelEx(&cfg, kernel, A, k, v);
 }
 
 template <typename T, int DP>

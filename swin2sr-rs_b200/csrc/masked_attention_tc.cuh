@@ -33,15 +33,6 @@ struct TcCfg {
   static constexpr int SMEM = BARS + NBARS * 8 + 16 + 1024;  // + alignment
 };
 
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar,
-                                            int c0, int c1, int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
-}
-
 // A [rows][64] panel in the 128-byte swizzle read along its rows as the contraction (V: keys
 // contract, values are the N extent): 64-value panels `panel` bytes apart, groups of eight
 // keys 1024 bytes apart.
@@ -447,23 +438,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
-// Rows of heads as a [tokens][heads][head_dim] tensor, in boxes of `rows` tokens, one head and
-// 64 values (zeros beyond head_dim and beyond the tokens).
-inline bool make_map_heads(CUtensorMap* map, const Rows& x, bool bf16, int64_t tokens, int heads,
-                           int head_dim, int rows) {
-  EncodeTiledFn fn = encode_fn();
-  if (!fn) return false;
-  cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)heads, (cuuint64_t)tokens};
-  // a stride that is never used still has to be a valid one
-  cuuint64_t strides[2] = {(cuuint64_t)(heads > 1 ? x.head : head_dim) * 2,
-                           (cuuint64_t)(tokens > 1 ? x.token : head_dim) * 2};
-  cuuint32_t box[3] = {64, 1, (cuuint32_t)rows};
-  cuuint32_t es[3] = {1, 1, 1};
-  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, x.data,
-            dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <typename T, int NP, bool PLAIN>
 cudaError_t launch_attention_tc(AttnArgs& A, cudaStream_t st) {
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
@@ -474,9 +448,9 @@ cudaError_t launch_attention_tc(AttnArgs& A, cudaStream_t st) {
   const cudaError_t err = resident_ctas(setup, kernel, kTcThreads, C::SMEM, &ctas);
   if (err != cudaSuccess) return err;
   CUtensorMap q, k, v;
-  if (!make_map_heads(&q, A.q, BF16, A.q_tokens, A.q_heads, A.head_dim, kTcTile) ||
-      !make_map_heads(&k, A.k, BF16, A.kv_tokens, A.kv_heads, A.head_dim, kTcTile) ||
-      !make_map_heads(&v, A.v, BF16, A.kv_tokens, A.kv_heads, A.head_dim, kTcTile))
+  if (!make_map_heads(&q, A.q, BF16, A.q_tokens, A.q_heads, A.head_dim, kTcTile, 64) ||
+      !make_map_heads(&k, A.k, BF16, A.kv_tokens, A.kv_heads, A.head_dim, kTcTile, 64) ||
+      !make_map_heads(&v, A.v, BF16, A.kv_tokens, A.kv_heads, A.head_dim, kTcTile, 64))
     return cudaErrorInvalidValue;
   const long long slots = (long long)A.q_tokens / (2 * kTcTile) + A.documents;
   const long long grid = slots * A.q_heads;
