@@ -8,7 +8,9 @@
 //   o_i = sum_{j < seen(i)} exp(z_j - m) v_j / sum_{j < seen(i)} exp(z_j - m)
 // All masks together leave each query a run of its document's first keys:
 //   seen(i) = nk, or with causal order min(nk, max(prefix, i + 1 + nk - nq)).
-// Scores, maxima, sums and outputs are fp32 until the one rounding of o.
+// Scores, maxima, sums and outputs are fp32 until the one rounding of o. The tile kernels hold
+// the scores as the products give them, caps and biases divided by `scale`; scale log2 e comes
+// in with the multiply-add in front of the exponential, which is one of base 2.
 #include "heads.cuh"
 
 namespace s2s {
@@ -29,7 +31,7 @@ struct AttnArgs {
   int q_heads, kv_heads, group, head_dim;
   int splits;      // CTAs of a cluster that share a tile's keys
   int slots;       // of row tiles (find_document)
-  int cta_slots;   // slots that a CTA takes, one after the other
+  unsigned long long guess;  // documents per slot, 32.32 fixed point
   int cta_heads;   // key heads that a CTA takes, one after the other
   float scale, cap;
 };
@@ -66,18 +68,17 @@ __device__ __forceinline__ Doc document(const AttnArgs& A, int d) {
 // without a look at the others. The document of a slot, by a whole warp, and the slot's tile
 // in it; false where there is none. Documents of about one length are found at the first
 // guess, in one round of loads; others by a search of 32 places a round.
-__device__ __forceinline__ bool find_document(const AttnArgs& A, int slot, int slots, int rows,
-                                              int mult, int lane, Doc* D, int* tile) {
-  auto first = [&](int d) -> long long {
-    const long long q = A.qoff ? (long long)min(max(A.qoff[d], 0), A.q_tokens)
-                               : (long long)d * (A.q_tokens / A.documents);
-    return q * mult / rows + d;
+__device__ __forceinline__ bool find_document(const AttnArgs& A, int slot, int rows, int mult, int lane,
+                                              Doc* D, int* tile) {
+  auto first = [&](int d) -> int {
+    const int q = A.qoff ? min(max(A.qoff[d], 0), A.q_tokens) : d * (A.q_tokens / A.documents);
+    return (int)((unsigned)(q * mult) / (unsigned)rows) + d;  // q_tokens * group is below 2^31
   };
-  int d = (int)min((long long)A.documents - 1, (long long)slot * A.documents / slots);
+  const int d = min(A.documents - 1, (int)((slot * A.guess) >> 32));
   *D = document(A, d);
-  const long long at = first(d), next = d + 1 < A.documents ? first(d + 1) : (long long)slot + 1;
+  const int at = first(d), next = d + 1 < A.documents ? first(d + 1) : slot + 1;
   if (at <= slot && slot < next) {
-    *tile = (int)(slot - at);
+    *tile = slot - at;
     return true;
   }
   int lo = 0, n = A.documents;  // the last d of [lo, lo + n) with first(d) <= slot
@@ -89,9 +90,14 @@ __device__ __forceinline__ bool find_document(const AttnArgs& A, int slot, int s
     n = min(step, n - c);
   }
   *D = document(A, lo);
-  const long long t = slot - first(lo);
-  *tile = (int)t;
-  return t >= 0;
+  *tile = slot - first(lo);
+  return *tile >= 0;
+}
+
+// The slots of a call with tiles of `rows` rows.
+inline void set_slots(AttnArgs& A, int rows, int mult) {
+  A.slots = (int)((long long)A.q_tokens * mult / rows + A.documents);
+  A.guess = (((unsigned long long)A.documents << 32) + A.slots - 1) / A.slots;
 }
 
 // Keys that query i of the document sees.
@@ -115,7 +121,7 @@ __device__ __forceinline__ float distance_bias(const AttnArgs& A, int h, int qro
 using F2 = unsigned long long;  // two fp32 lanes of the packed operations
 __device__ __forceinline__ F2 f2_both(float x) { return f2_pack(x, x); }
 
-// Scores s -> cap2 * tanh(s * to_cap). Up to 1, tanh x = x P(x^2) with P the polynomial of
+// Scores s -> cap * tanh(s * to_cap). Up to 1, tanh x = x P(x^2) with P the polynomial of
 // degree 6 of least relative error on [0, 1] (5e-8, by the exchange algorithm), two scores an
 // instruction; beyond, 1 - 2 / (1 + e^{2x}). The second form costs two more operations of the
 // special function unit, which softmax is bound by, so a warp takes it only where it has such
@@ -136,18 +142,18 @@ __device__ __forceinline__ float tanh_far(float x, float near) {
   return fabsf(x) > 1.0f ? copysignf(fmaf(-2.0f, r, 1.0f), x) : near;
 }
 template <int N>
-__device__ __forceinline__ void capped(float (&s)[N], float to_cap, float cap2) {
+__device__ __forceinline__ void capped(float (&s)[N], float to_cap, float cap) {
   float far = 0.0f;
 #pragma unroll
   for (int j = 0; j < N; j++) far = fmaxf(far, fabsf(s[j]));
-  const F2 t = f2_both(to_cap), c = f2_both(cap2);
+  const F2 t = f2_both(to_cap), c = f2_both(cap);
   if (__any_sync(0xffffffffu, far * to_cap > 1.0f)) {
 #pragma unroll
     for (int j = 0; j < N; j += 2) {
       const F2 x = f2_mul(f2_pack(s[j], s[j + 1]), t);
       const float2 xs = f2_unpack(x), y = f2_unpack(tanh_poly(x));
-      s[j] = cap2 * tanh_far(xs.x, y.x);
-      s[j + 1] = cap2 * tanh_far(xs.y, y.y);
+      s[j] = cap * tanh_far(xs.x, y.x);
+      s[j + 1] = cap * tanh_far(xs.y, y.y);
     }
   } else {
 #pragma unroll
@@ -292,8 +298,8 @@ int s2s_masked_attention(const s2s_attention* a, void* stream) {
         (a->q_tokens % a->documents || a->kv_tokens % a->documents))
       fail(S2S_ERR_INVALID, me + "without offsets the documents must divide the tokens");
     if (a->d_prefix && !a->causal) fail(S2S_ERR_INVALID, me + "a prefix needs causal order");
-    if (!(a->scale > 0.0f) || !std::isfinite(a->scale))
-      fail(S2S_ERR_INVALID, me + "scale must be positive and finite");
+    if (!(a->scale >= 1e-12f && a->scale <= 1e12f))
+      fail(S2S_ERR_INVALID, me + "scale must be between 1e-12 and 1e12");
     if (!(a->cap >= 0.0f) || !std::isfinite(a->cap))
       fail(S2S_ERR_INVALID, me + "cap must be 0 or positive and finite");
     if (a->axes < 0 || a->axes > S2S_MAX_AXES)
@@ -306,6 +312,9 @@ int s2s_masked_attention(const s2s_attention* a, void* stream) {
       fail(S2S_ERR_INVALID, me + "k and v, and q and out, must have the same heads, q's a "
                                  "multiple of k's");
     if (a->q.heads > 65535) fail(S2S_ERR_INVALID, me + "at most 65535 heads");
+    if ((int64_t)a->q_tokens * (a->q.heads / a->k.heads) > 0x7fffff00)
+      fail(S2S_ERR_INVALID, me + "q_tokens * (q heads / k heads) must stay below 2^31");
+    if (a->documents > 1 << 30) fail(S2S_ERR_INVALID, me + "at most 2^30 documents");
     for (const void* p : {(const void*)a->d_q_offsets, (const void*)a->d_kv_offsets,
                           (const void*)a->d_prefix, (const void*)a->d_slopes,
                           (const void*)a->d_q_pos, (const void*)a->d_kv_pos,

@@ -16,8 +16,6 @@
 namespace s2s {
 namespace {
 
-constexpr int kMmaThreads = 128;
-constexpr int kMmaKeys = 64;    // keys of a tile
 constexpr int kMmaStages = 3;
 
 template <typename T>
@@ -78,24 +76,26 @@ __device__ __forceinline__ float4 cluster_load4(uint32_t addr, uint32_t rank) {
   return v;
 }
 
-template <int DP, int RW>
+template <int DP, int RW, int WARPS>
 struct MmaCfg {
-  static constexpr int KW = 4 / RW;              // warps along the keys
+  static constexpr int THREADS = 32 * WARPS;
+  static constexpr int TKEYS = 16 * WARPS;       // keys of a tile
+  static constexpr int KW = WARPS / RW;          // warps along the keys
   static constexpr int ROWS = 16 * RW;
-  static constexpr int KEYS = kMmaKeys / KW;     // keys of a tile that one warp takes
+  static constexpr int KEYS = TKEYS / KW;        // keys of a tile that one warp takes
   static constexpr int PV = DP < 64 ? DP : 64;   // values of a panel: a TMA box's row
-  static constexpr int PANEL = kMmaKeys * PV * 2;
-  static constexpr int TILE = kMmaKeys * DP * 2; // bytes of a K or V tile, panel after panel
+  static constexpr int PANEL = TKEYS * PV * 2;
+  static constexpr int TILE = TKEYS * DP * 2;    // bytes of a K or V tile, panel after panel
   static constexpr int RING = kMmaStages * 2 * TILE;
   static constexpr int LD = DP + 4;              // floats of a joined output row
-  static constexpr int JOIN = 4 * 16 * LD * 4;   // the four warps' outputs, over the ring
+  static constexpr int JOIN = WARPS * 16 * LD * 4;  // the warps' outputs, over the ring
   static constexpr int BODY = RING > JOIN ? RING : JOIN;
-  static constexpr int POS = S2S_MAX_AXES * kMmaKeys * 4;  // key positions of a stage
+  static constexpr int POS = S2S_MAX_AXES * TKEYS * 4;  // key positions of a stage
   static constexpr int BARS = BODY + kMmaStages * POS;
   static constexpr int ENDS = BARS + kMmaStages * 8 + 8;   // maxima and sums, flags
-  static constexpr int SMEM = ENDS + 4 * 16 * 8 + ROWS * 12 + 1024;  // + alignment
+  static constexpr int SMEM = ENDS + WARPS * 16 * 8 + ROWS * 12 + 1024;  // + alignment
   // resident CTAs that the registers are cut to: the more, the more loads are in flight
-  static constexpr int CTAS = DP == 32 ? 4 : DP == 64 ? 3 : 2;
+  static constexpr int CTAS = (DP == 32 ? 4 : DP == 64 ? 3 : 2) * 4 / WARPS;
 };
 
 // Where lane `lane` finds, in a tile, chunk `b` (16 bytes) of row `r`; chunk b + 2k of the same
@@ -118,42 +118,43 @@ __device__ __forceinline__ void write_rows(const AttnArgs& A, const Doc& D, int 
     const bool none = m[e] == -INFINITY;
     const float inv = none ? 0.0f : 1.0f / l[e];
     const int h = hk * A.group + row_h[e];
-    bool bad = false;
-    T* op = static_cast<T*>(A.out.data) + (int64_t)row_q[e] * A.out.token + (int64_t)h * A.out.head;
+    float check = 0.0f;  // NaN where an output is NaN or infinite
+    T* op = static_cast<T*>(A.out.data) + (int64_t)row_q[e] * A.out.token + (int64_t)h * A.out.head + 2 * t4;
 #pragma unroll
     for (int n = 0; n < DN; n++) {
-      const float x = none ? 0.0f : o[n][2 * e] * inv, y = none ? 0.0f : o[n][2 * e + 1] * inv;
-      bad = bad || !(fabsf(x) < INFINITY) || !(fabsf(y) < INFINITY);
-      if (live[e] && n * 8 < A.head_dim) *reinterpret_cast<uint32_t*>(op + n * 8 + 2 * t4) = pack2<T>(x, y);
+      const float x = o[n][2 * e] * inv, y = o[n][2 * e + 1] * inv;
+      check = fmaf(x, 0.0f, fmaf(y, 0.0f, check));
+      if (live[e] && n * 8 < A.head_dim) *reinterpret_cast<uint32_t*>(op + n * 8) = pack2<T>(x, y);
     }
     if (live[e] && t4 == 0 && A.lse)
       A.lse[(int64_t)h * A.q_tokens + row_q[e]] = none ? -INFINITY : (m[e] + log2f(l[e])) * kLn2;
     // keys that the row does not see were multiplied by zero weights: a NaN or infinity among
     // their values shows here, and the row is done again without them
-    const unsigned redo = __ballot_sync(0xffffffffu, bad && live[e] && row_seen[e] < kend);
+    unsigned redo = __ballot_sync(0xffffffffu, check != 0.0f && live[e] && row_seen[e] < kend);
     __syncwarp();
-    for (int q = 0; q < 8; q++)
-      if (redo >> (4 * q) & 15u) {
-        const int i = __shfl_sync(0xffffffffu, row_q[e], 4 * q) - D.q0;
-        attend_row<T>(A, D, i, __shfl_sync(0xffffffffu, h, 4 * q), lane);
-      }
+    while (redo) {
+      const int src = __ffs(redo) - 1;
+      redo &= ~(15u << (src & ~3));
+      const int i = __shfl_sync(0xffffffffu, row_q[e], src) - D.q0;
+      attend_row<T>(A, D, i, __shfl_sync(0xffffffffu, h, src), lane);
+    }
   }
 }
 
 // Outputs of a head whose keys lie with several warps, and CTAs of a cluster: everything they
 // have goes through shared memory (over the ring, which is idle by then).
-template <typename T, int DP, int RW>
+template <typename T, int DP, int RW, int WARPS>
 __device__ __forceinline__ void join_rows(const AttnArgs& A, const Doc& D, int hk, uint8_t* smem,
                                           const float (&o)[DP / 8][4], const float (&m)[2],
-                                          const float (&l)[2], long long r0, long long nrows, int kend,
-                                          int S, int split) {
-  using C = MmaCfg<DP, RW>;
+                                          const float (&l)[2], int r0, int nrows, int kend, int S,
+                                          int split) {
+  using C = MmaCfg<DP, RW, WARPS>;
   constexpr int KW = C::KW, DN = DP / 8;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int hd = A.head_dim;
   float* part = reinterpret_cast<float*>(smem);                 // [4][16][LD]
   float2* ml = reinterpret_cast<float2*>(smem + C::ENDS);       // [4][16]
-  float2* mlc = ml + 64;                                        // [ROWS] of the CTA
+  float2* mlc = ml + WARPS * 16;                                        // [ROWS] of the CTA
   int* flag = reinterpret_cast<int*>(mlc + C::ROWS);            // [ROWS]
   __syncthreads();
 #pragma unroll
@@ -163,11 +164,11 @@ __device__ __forceinline__ void join_rows(const AttnArgs& A, const Doc& D, int h
     for (int n = 0; n < DN; n++) *reinterpret_cast<float2*>(p + n * 8) = make_float2(o[n][2 * e], o[n][2 * e + 1]);
     if (t4 == 0) ml[warp * 16 + g + 8 * e] = make_float2(m[e], l[e]);
   }
-  if (tid < C::ROWS) flag[tid] = 0;
+  if (tid < C::ROWS) flag[tid] = 0;  // at most 64 rows
   __syncthreads();
   // the key warps of a row into the first of them
   constexpr int Q4 = DP / 4;
-  for (int u = tid; u < C::ROWS * Q4; u += kMmaThreads) {
+  for (int u = tid; u < C::ROWS * Q4; u += C::THREADS) {
     const int r = u / Q4, c = (u % Q4) * 4, w = r / 16, rr = r % 16;
     float top = -INFINITY;
 #pragma unroll
@@ -193,7 +194,7 @@ __device__ __forceinline__ void join_rows(const AttnArgs& A, const Doc& D, int h
   else __syncthreads();
   // the CTAs of the cluster: each finishes every S-th row
   const int mine = (C::ROWS - split + S - 1) / S;
-  for (int u = tid; u < mine * Q4; u += kMmaThreads) {
+  for (int u = tid; u < mine * Q4; u += C::THREADS) {
     const int r = split + (u / Q4) * S, c = (u % Q4) * 4;
     if (r >= nrows) continue;
     float4 sum;
@@ -219,7 +220,7 @@ __device__ __forceinline__ void join_rows(const AttnArgs& A, const Doc& D, int h
       top = mlc[r].x;
       total = mlc[r].y;
     }
-    const int i = (int)((r0 + r) / A.group), h = hk * A.group + (int)(r0 + r - (long long)i * A.group);
+    const int i = (r0 + r) / A.group, h = hk * A.group + r0 + r - i * A.group;
     const bool none = top == -INFINITY;
     const float inv = none ? 0.0f : 1.0f / total;
     const float4 x = none ? make_float4(0, 0, 0, 0)
@@ -234,19 +235,19 @@ __device__ __forceinline__ void join_rows(const AttnArgs& A, const Doc& D, int h
       flag[r] = 1;
   }
   __syncthreads();
-  for (int r = warp; r < C::ROWS; r += 4)
+  for (int r = warp; r < C::ROWS; r += WARPS)
     if (flag[r]) {
-      const int i = (int)((r0 + r) / A.group);
-      attend_row<T>(A, D, i, hk * A.group + (int)(r0 + r - (long long)i * A.group), lane);
+      const int i = (r0 + r) / A.group;
+      attend_row<T>(A, D, i, hk * A.group + r0 + r - i * A.group, lane);
     }
   if (S > 1) cluster_sync();  // nobody leaves while its shared memory is read
 }
 
-template <typename T, int DP, int RW>
-__global__ void __launch_bounds__(kMmaThreads, MmaCfg<DP, RW>::CTAS)
+template <typename T, int DP, int RW, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS>::CTAS)
     k_attention_mma(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap mapK,
                     const __grid_constant__ CUtensorMap mapV) {
-  using C = MmaCfg<DP, RW>;
+  using C = MmaCfg<DP, RW, WARPS>;
   constexpr int KW = C::KW, NT = C::KEYS / 8, DN = DP / 8, DK = DP / 16, PK = C::PV / 16;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -261,8 +262,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaCfg<DP, RW>::CTAS)
   const int hk1 = min(A.kv_heads, hk0 + A.cta_heads);
   const int hd = A.head_dim;
   const float to_cap = A.cap > 0.0f ? A.scale / A.cap : 0.0f;
-  const float cap2 = A.cap * kLog2e, scale2 = A.scale * kLog2e;
-  const float unit = A.cap > 0.0f || A.axes ? 1.0f : scale2;  // what scores still lack at the exponential
+  const float raw_cap = A.cap / A.scale, unit = A.scale * kLog2e;
   // this lane's place in the 16 x 16 blocks of K and V that ldmatrix takes
   const uint32_t kat = tile_at<DP>(kw * C::KEYS + (lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1);
   const uint32_t vat = tile_at<DP>(kw * C::KEYS + (lane & 7) + (((lane >> 3) & 1) << 3), lane >> 4);
@@ -274,311 +274,298 @@ __global__ void __launch_bounds__(kMmaThreads, MmaCfg<DP, RW>::CTAS)
   }
   pdl_trigger();
   pdl_wait();
-  // tiles fetched and computed so far; a wait that gave up is not followed by others, but the
-  // CTA's barriers are met all the same
-  uint32_t fetches = 0, steps = 0;
+  // the stages that are filled and computed next, the phase of the latter; a wait that gave up is
+  // not followed by others, but the CTA's barriers are met all the same
+  int fstage = 0, stage = 0;
+  uint32_t phase = 0;
   bool ok = true;
 
-  for (int sl = 0; sl < A.cta_slots; sl++) {
-    const long long slot = (long long)(item / hgroups) * A.cta_slots + sl;
-    if (slot >= A.slots) break;
-    int tile;
-    Doc D;
-    if (!find_document(A, (int)slot, A.slots, C::ROWS, A.group, lane, &D, &tile)) continue;
-    const long long r0 = (long long)tile * C::ROWS;  // rows of the document: query * group + head
-    const long long nrows = (long long)D.nq * A.group - r0;
-    if (nrows <= 0) continue;
-    const int i_first = (int)(r0 / A.group);
-    const int i_last = min(D.nq - 1, (int)((r0 + C::ROWS - 1) / A.group));
-    const int kend = seen(A, D, i_last);   // keys that any row of the tile sees
-    const int open = seen(A, D, i_first);  // keys that every row sees
-    const int ntiles = (kend + kMmaKeys - 1) / kMmaKeys;
-    const int tb = (int)((long long)ntiles * split / S), te = (int)((long long)ntiles * (split + 1) / S);
+  int tile;
+  Doc D;
+  if (!find_document(A, (int)(item / hgroups), C::ROWS, A.group, lane, &D, &tile)) return;
+  if ((long long)tile * C::ROWS >= (long long)D.nq * A.group) return;  // the same for all of a cluster
+  const int r0 = tile * C::ROWS;  // rows of the document: query * group + head
+  const int nrows = D.nq * A.group - r0;
+  const int i_first = r0 / A.group;
+  const int i_last = min(D.nq - 1, (r0 + C::ROWS - 1) / A.group);
+  const int kend = seen(A, D, i_last);   // keys that any row of the tile sees
+  const int open = seen(A, D, i_first);  // keys that every row sees
+  const int ntiles = (kend + C::TKEYS - 1) / C::TKEYS;
+  const int tb = (int)((long long)ntiles * split / S), te = (int)((long long)ntiles * (split + 1) / S);
 
-    // this thread's two rows
-    int row_seen[2], row_q[2], row_h[2];
-    bool live[2];
+  // this thread's two rows
+  int row_seen[2], row_q[2], row_h[2];
+  bool live[2];
+#pragma unroll
+  for (int e = 0; e < 2; e++) {
+    const int r = r0 + rw * 16 + g + 8 * e;
+    live[e] = r - r0 < nrows;
+    const int i = live[e] ? r / A.group : i_first;
+    row_q[e] = D.q0 + i;
+    row_h[e] = live[e] ? r - i * A.group : 0;  // within the key head
+    row_seen[e] = live[e] ? seen(A, D, i) : 0;
+  }
+
+  // bias: positions count from the tile's first query, so that near ones are exact
+  float qpos[2][S2S_MAX_AXES];
+  int ref[S2S_MAX_AXES];
+  if (A.axes) {
+#pragma unroll
+    for (int a = 0; a < S2S_MAX_AXES; a++)
+      if (a < A.axes) {
+        const int* qa = A.qpos + (int64_t)a * A.q_tokens;
+        ref[a] = qa[D.q0 + i_first];
+#pragma unroll
+        for (int e = 0; e < 2; e++) qpos[e][a] = (float)(int)((unsigned)qa[row_q[e]] - (unsigned)ref[a]);
+      }
+  }
+
+  // K and V tiles of head after head into the ring; the key positions of a tile, as fp32,
+  // through registers a tile later
+  int ft = tb, fh = hk0;  // the next tile to fetch
+  int kraw[2];
+  auto fetch = [&]() {
+    if (fh >= hk1 || tb >= te) return;
+    if (tid == 0) {
+      uint8_t* dst = smem + fstage * 2 * C::TILE;
+      mbar_arrive_expect_tx(&full[fstage], 2 * C::TILE);
+#pragma unroll
+      for (int p = 0; p < DP / C::PV; p++) {
+        tma_load_3d(dst + p * C::PANEL, &mapK, &full[fstage], p * C::PV, fh, D.k0 + ft * C::TKEYS);
+        tma_load_3d(dst + C::TILE + p * C::PANEL, &mapV, &full[fstage], p * C::PV, fh, D.k0 + ft * C::TKEYS);
+      }
+    }
+    if (A.axes)
+#pragma unroll
+      for (int x = 0; x < 2; x++) {
+        const int u = tid + x * C::THREADS, a = u / C::TKEYS, j = ft * C::TKEYS + u % C::TKEYS;
+        if (a < A.axes) kraw[x] = A.kpos[(int64_t)a * A.kv_tokens + D.k0 + min(j, kend - 1)];
+      }
+  };
+  auto fetched = [&]() {  // the positions of the tile last fetched
+    if (fh >= hk1 || tb >= te) return;
+    if (A.axes) {
+      float* kp = spos + fstage * (S2S_MAX_AXES * C::TKEYS);
+#pragma unroll
+      for (int x = 0; x < 2; x++) {
+        const int u = tid + x * C::THREADS, a = u / C::TKEYS;
+        if (a < A.axes) {
+          const int rf = a == 0 ? ref[0] : a == 1 ? ref[1] : ref[2];
+          kp[u] = (float)(int)((unsigned)kraw[x] - (unsigned)rf);
+        }
+      }
+    }
+    fstage = fstage + 1 == kMmaStages ? 0 : fstage + 1;
+    if (++ft == te) {
+      ft = tb;
+      fh++;
+    }
+  };
+  // Q fragments of a head straight from global memory
+  uint32_t qf[DK][4], qnext[DK][4];
+  auto load_q = [&](int hk) {
 #pragma unroll
     for (int e = 0; e < 2; e++) {
-      const long long r = r0 + rw * 16 + g + 8 * e;
-      live[e] = r - r0 < nrows;
-      const int i = live[e] ? (int)(r / A.group) : i_first;
-      row_q[e] = D.q0 + i;
-      row_h[e] = live[e] ? (int)(r - (long long)i * A.group) : 0;  // within the key head
-      row_seen[e] = live[e] ? seen(A, D, i) : 0;
-    }
-
-    // bias: positions count from the tile's first query, so that near ones are exact
-    float qpos[2][S2S_MAX_AXES];
-    int ref[S2S_MAX_AXES];
-    if (A.axes) {
-#pragma unroll
-      for (int a = 0; a < S2S_MAX_AXES; a++)
-        if (a < A.axes) {
-          const int* qa = A.qpos + (int64_t)a * A.q_tokens;
-          ref[a] = qa[D.q0 + i_first];
-#pragma unroll
-          for (int e = 0; e < 2; e++) qpos[e][a] = (float)(int)((unsigned)qa[row_q[e]] - (unsigned)ref[a]);
-        }
-    }
-
-    // K and V tiles of head after head into the ring; the key positions of a tile, as fp32,
-    // through registers a tile later
-    int ft = tb, fh = hk0;  // the next tile to fetch
-    int kraw[2];
-    auto fetch = [&]() {
-      if (fh >= hk1 || tb >= te) return;
-      const uint32_t st = fetches % kMmaStages;
-      if (tid == 0) {
-        uint8_t* dst = smem + st * 2 * C::TILE;
-        mbar_arrive_expect_tx(&full[st], 2 * C::TILE);
-#pragma unroll
-        for (int p = 0; p < DP / C::PV; p++) {
-          tma_load_3d(dst + p * C::PANEL, &mapK, &full[st], p * C::PV, fh, D.k0 + ft * kMmaKeys);
-          tma_load_3d(dst + C::TILE + p * C::PANEL, &mapV, &full[st], p * C::PV, fh, D.k0 + ft * kMmaKeys);
-        }
-      }
-      if (A.axes)
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-          const int u = tid + x * kMmaThreads, a = u / kMmaKeys, j = ft * kMmaKeys + u % kMmaKeys;
-          if (a < A.axes) kraw[x] = A.kpos[(int64_t)a * A.kv_tokens + D.k0 + min(j, kend - 1)];
-        }
-    };
-    auto fetched = [&]() {  // the positions of the tile last fetched
-      if (fh >= hk1 || tb >= te) return;
-      if (A.axes) {
-        float* kp = spos + (fetches % kMmaStages) * (S2S_MAX_AXES * kMmaKeys);
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-          const int u = tid + x * kMmaThreads, a = u / kMmaKeys;
-          if (a < A.axes) {
-            const int rf = a == 0 ? ref[0] : a == 1 ? ref[1] : ref[2];
-            kp[u] = (float)(int)((unsigned)kraw[x] - (unsigned)rf);
-          }
-        }
-      }
-      fetches++;
-      if (++ft == te) {
-        ft = tb;
-        fh++;
-      }
-    };
-    // Q fragments of a head straight from global memory
-    uint32_t qf[DK][4], qnext[DK][4];
-    auto load_q = [&](int hk) {
-#pragma unroll
-      for (int e = 0; e < 2; e++) {
-        const T* qp = static_cast<const T*>(A.q.data) + (int64_t)row_q[e] * A.q.token +
-                      (int64_t)(hk * A.group + row_h[e]) * A.q.head;
-#pragma unroll
-        for (int kk = 0; kk < DK; kk++)
-#pragma unroll
-          for (int x = 0; x < 2; x++) {
-            const int d = kk * 16 + 2 * t4 + x * 8;
-            qnext[kk][e + 2 * x] = live[e] && d < hd ? *reinterpret_cast<const uint32_t*>(qp + d) : 0u;
-          }
-      }
-    };
-    __syncthreads();  // the barriers are set up, the ring is free
-    load_q(hk0);
-#pragma unroll
-    for (int s = 0; s < kMmaStages - 1; s++) {
-      fetch();
-      fetched();
-    }
-
-    for (int hk = hk0; hk < hk1; hk++) {
+      const T* qp = static_cast<const T*>(A.q.data) + (int64_t)row_q[e] * A.q.token +
+                    (int64_t)(hk * A.group + row_h[e]) * A.q.head;
 #pragma unroll
       for (int kk = 0; kk < DK; kk++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) qf[kk][e] = qnext[kk][e];
-      if constexpr (KW == 1)
-        if (hk + 1 < hk1) load_q(hk + 1);
-      float slope[2][S2S_MAX_AXES];
-#pragma unroll
-      for (int a = 0; a < S2S_MAX_AXES; a++)
-        if (a < A.axes)
-#pragma unroll
-          for (int e = 0; e < 2; e++)
-            slope[e][a] = fabsf(A.slopes[a * A.q_heads + hk * A.group + row_h[e]]) * kLog2e;
-      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-      float o[DN][4];
-#pragma unroll
-      for (int n = 0; n < DN; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
-
-      for (int t = tb; t < te; t++, steps++) {
-        const uint32_t stage = steps % kMmaStages;
-        if (ok) ok = mbar_wait(&full[stage], (steps / kMmaStages) & 1, DEV_TIMEOUT_FULL);
-        const int tail = kend - t * kMmaKeys;  // keys of the tile that some row sees
-        if (tail < kMmaKeys) {
-          // behind them lie other documents' rows, or none: zero weights must not meet what is
-          // there, nor may the copies into the stage pass these writes
-          for (int u = tid; u < (kMmaKeys - tail) * (DP / 8); u += kMmaThreads) {
-            const int p = u / ((kMmaKeys - tail) * (C::PV / 8)), c = u % ((kMmaKeys - tail) * (C::PV / 8));
-            *reinterpret_cast<uint4*>(smem + stage * 2 * C::TILE + C::TILE + p * C::PANEL +
-                                      tail * C::PV * 2 + c * 16) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
+        for (int x = 0; x < 2; x++) {
+          const int d = kk * 16 + 2 * t4 + x * 8;
+          qnext[kk][e + 2 * x] = live[e] && d < hd ? *reinterpret_cast<const uint32_t*>(qp + d) : 0u;
         }
-        __syncthreads();  // everyone has left the stage that is filled now
-        fetch();
-        const uint32_t ks = smem_u32(smem + stage * 2 * C::TILE), vs = ks + C::TILE;
-        const int j0 = t * kMmaKeys + kw * C::KEYS;
-        if (KW == 1 || j0 < kend) {  // some key of this warp is seen
-          float s[NT][4];
-#pragma unroll
-          for (int n = 0; n < NT; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-#pragma unroll
-          for (int kk = 0; kk < DK; kk++)
-#pragma unroll
-            for (int n = 0; n < NT; n += 2) {
-              uint32_t b0, b1, b2, b3;
-              ldsm_x4(ks + (kk / PK) * C::PANEL + n * 8 * C::PV * 2 + (kat ^ (kk % PK * 32)), b0, b1, b2, b3);
-              mma_tile<T>(s[n], qf[kk], b0, b1);
-              mma_tile<T>(s[n + 1], qf[kk], b2, b3);
-            }
-          // scores in units of log 2
-          if (A.cap > 0.0f) {
-            capped(reinterpret_cast<float (&)[NT * 4]>(s), to_cap, cap2);
-          } else if (A.axes) {
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-              for (int e = 0; e < 4; e++) s[n][e] *= scale2;
-          }
-          if (A.axes) {
-            const float* kp = spos + stage * (S2S_MAX_AXES * kMmaKeys) + kw * C::KEYS + 2 * t4;
-#pragma unroll
-            for (int a = 0; a < S2S_MAX_AXES; a++)
-              if (a < A.axes) {
-                // |slope| |q - k| as |slope q - slope k|
-                const F2 s0 = f2_both(-slope[0][a]), s1 = f2_both(-slope[1][a]);
-                const F2 q0 = f2_both(slope[0][a] * qpos[0][a]), q1 = f2_both(slope[1][a] * qpos[1][a]);
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-                  const F2 k2 = *reinterpret_cast<const F2*>(kp + a * kMmaKeys + n * 8);
-                  const float2 d0 = f2_unpack(f2_fma(k2, s0, q0)), d1 = f2_unpack(f2_fma(k2, s1, q1));
-                  s[n][0] -= fabsf(d0.x);
-                  s[n][1] -= fabsf(d0.y);
-                  s[n][2] -= fabsf(d1.x);
-                  s[n][3] -= fabsf(d1.y);
-                }
-              }
-          }
-          if (j0 + C::KEYS > open) {
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-              for (int e = 0; e < 4; e++)
-                if (j0 + n * 8 + 2 * t4 + (e & 1) >= row_seen[e >> 1]) s[n][e] = -INFINITY;
-          }
-          // running maximum and sum
-          float keep[2], base[2];
-#pragma unroll
-          for (int e = 0; e < 2; e++) {
-            float top = -INFINITY;
-#pragma unroll
-            for (int n = 0; n < NT; n++) top = max3(top, s[n][2 * e], s[n][2 * e + 1]);
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            top = fmaxf(top * unit, m[e]);
-            base[e] = top == -INFINITY ? 0.0f : top;  // a row that has seen nothing yet
-            keep[e] = ex2(m[e] - base[e]);
-            m[e] = top;
-          }
-          const F2 u2 = f2_both(unit), b0 = f2_both(-base[0]), b1 = f2_both(-base[1]);
-          F2 sum0 = 0, sum1 = 0;  // two zeros each
-#pragma unroll
-          for (int n = 0; n < NT; n++) {
-            const float2 x = f2_unpack(f2_fma(f2_pack(s[n][0], s[n][1]), u2, b0));
-            const float2 y = f2_unpack(f2_fma(f2_pack(s[n][2], s[n][3]), u2, b1));
-            s[n][0] = ex2(x.x);
-            s[n][1] = ex2(x.y);
-            s[n][2] = ex2(y.x);
-            s[n][3] = ex2(y.y);
-            sum0 = f2_add(sum0, f2_pack(s[n][0], s[n][1]));
-            sum1 = f2_add(sum1, f2_pack(s[n][2], s[n][3]));
-          }
-          const float2 t0 = f2_unpack(sum0), t1 = f2_unpack(sum1);
-          l[0] = fmaf(l[0], keep[0], t0.x + t0.y);
-          l[1] = fmaf(l[1], keep[1], t1.x + t1.y);
-          if (__any_sync(0xffffffffu, keep[0] != 1.0f || keep[1] != 1.0f)) {
-#pragma unroll
-            for (int n = 0; n < DN; n++) {
-              o[n][0] *= keep[0];
-              o[n][1] *= keep[0];
-              o[n][2] *= keep[1];
-              o[n][3] *= keep[1];
-            }
-          }
-          // O += P V; the weights are rounded to the type of v, the sum l is not
-#pragma unroll
-          for (int kk = 0; kk < NT / 2; kk++) {
-            const uint32_t a[4] = {
-                pack2<T>(s[2 * kk][0], s[2 * kk][1]), pack2<T>(s[2 * kk][2], s[2 * kk][3]),
-                pack2<T>(s[2 * kk + 1][0], s[2 * kk + 1][1]), pack2<T>(s[2 * kk + 1][2], s[2 * kk + 1][3])};
-#pragma unroll
-            for (int n = 0; n < DN; n += 2) {
-              uint32_t b0, b1, b2, b3;
-              ldsm_x4_t(vs + (n / (2 * PK)) * C::PANEL + kk * 16 * C::PV * 2 + (vat ^ (n % (2 * PK) * 16)), b0, b1,
-                        b2, b3);
-              mma_tile<T>(o[n], a, b0, b1);
-              mma_tile<T>(o[n + 1], a, b2, b3);
-            }
-          }
-        }
-        fetched();
-      }
-#pragma unroll
-      for (int e = 0; e < 2; e++) {
-        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-      }
-      if (KW == 1 && S == 1)
-        write_rows<T, DN>(A, D, hk, o, m, l, row_q, row_h, row_seen, live, kend, lane);
-      else  // one head (cta_heads is 1)
-        join_rows<T, DP, RW>(A, D, hk, smem, o, m, l, r0, nrows, kend, S, split);
     }
+  };
+  __syncthreads();  // the barriers are set up, the ring is free
+  load_q(hk0);
+#pragma unroll
+  for (int s = 0; s < kMmaStages - 1; s++) {
+    fetch();
+    fetched();
+  }
+
+  for (int hk = hk0; hk < hk1; hk++) {
+#pragma unroll
+    for (int kk = 0; kk < DK; kk++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) qf[kk][e] = qnext[kk][e];
+    if constexpr (KW == 1)
+      if (hk + 1 < hk1) load_q(hk + 1);
+    float slope[2][S2S_MAX_AXES];
+#pragma unroll
+    for (int a = 0; a < S2S_MAX_AXES; a++)
+      if (a < A.axes)
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+          slope[e][a] = fabsf(A.slopes[a * A.q_heads + hk * A.group + row_h[e]]) / A.scale;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    float o[DN][4];
+#pragma unroll
+    for (int n = 0; n < DN; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+
+    for (int t = tb; t < te; t++) {
+      if (ok) ok = mbar_wait(&full[stage], phase, DEV_TIMEOUT_FULL);
+      const int tail = kend - t * C::TKEYS;  // keys of the tile that some row sees
+      if (tail < C::TKEYS) {
+        // behind them lie other documents' rows, or none: zero weights must not meet what is
+        // there, nor may the copies into the stage pass these writes
+        for (int u = tid; u < (C::TKEYS - tail) * (DP / 8); u += C::THREADS) {
+          const int p = u / ((C::TKEYS - tail) * (C::PV / 8)), c = u % ((C::TKEYS - tail) * (C::PV / 8));
+          *reinterpret_cast<uint4*>(smem + stage * 2 * C::TILE + C::TILE + p * C::PANEL +
+                                    tail * C::PV * 2 + c * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+      }
+      __syncthreads();  // everyone has left the stage that is filled now
+      fetch();
+      const uint32_t ks = smem_u32(smem + stage * 2 * C::TILE), vs = ks + C::TILE;
+      const int j0 = t * C::TKEYS + kw * C::KEYS;
+      if (KW == 1 || j0 < kend) {  // some key of this warp is seen
+        float s[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < DK; kk++)
+#pragma unroll
+          for (int n = 0; n < NT; n += 2) {
+            uint32_t b0, b1, b2, b3;
+            ldsm_x4(ks + (kk / PK) * C::PANEL + n * 8 * C::PV * 2 + (kat ^ (kk % PK * 32)), b0, b1, b2, b3);
+            mma_tile<T>(s[n], qf[kk], b0, b1);
+            mma_tile<T>(s[n + 1], qf[kk], b2, b3);
+          }
+        if (A.cap > 0.0f) capped(reinterpret_cast<float (&)[NT * 4]>(s), to_cap, raw_cap);
+        if (A.axes) {
+          const float* kp = spos + stage * (S2S_MAX_AXES * C::TKEYS) + kw * C::KEYS + 2 * t4;
+#pragma unroll
+          for (int a = 0; a < S2S_MAX_AXES; a++)
+            if (a < A.axes) {
+              // |slope| |q - k| as |slope q - slope k|
+              const F2 s0 = f2_both(-slope[0][a]), s1 = f2_both(-slope[1][a]);
+              const F2 q0 = f2_both(slope[0][a] * qpos[0][a]), q1 = f2_both(slope[1][a] * qpos[1][a]);
+#pragma unroll
+              for (int n = 0; n < NT; n++) {
+                const F2 k2 = *reinterpret_cast<const F2*>(kp + a * C::TKEYS + n * 8);
+                const float2 d0 = f2_unpack(f2_fma(k2, s0, q0)), d1 = f2_unpack(f2_fma(k2, s1, q1));
+                s[n][0] -= fabsf(d0.x);
+                s[n][1] -= fabsf(d0.y);
+                s[n][2] -= fabsf(d1.x);
+                s[n][3] -= fabsf(d1.y);
+              }
+            }
+        }
+        if (j0 + C::KEYS > open) {
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              if (j0 + n * 8 + 2 * t4 + (e & 1) >= row_seen[e >> 1]) s[n][e] = -INFINITY;
+        }
+        // running maximum and sum
+        float keep[2], base[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int n = 0; n < NT; n++) top = max3(top, s[n][2 * e], s[n][2 * e + 1]);
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          top = fmaxf(top * unit, m[e]);
+          base[e] = top == -INFINITY ? 0.0f : top;  // a row that has seen nothing yet
+          keep[e] = ex2(m[e] - base[e]);
+          m[e] = top;
+        }
+        const F2 u2 = f2_both(unit), b0 = f2_both(-base[0]), b1 = f2_both(-base[1]);
+        F2 sum0 = 0, sum1 = 0;  // two zeros each
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          const float2 x = f2_unpack(f2_fma(f2_pack(s[n][0], s[n][1]), u2, b0));
+          const float2 y = f2_unpack(f2_fma(f2_pack(s[n][2], s[n][3]), u2, b1));
+          s[n][0] = ex2(x.x);
+          s[n][1] = ex2(x.y);
+          s[n][2] = ex2(y.x);
+          s[n][3] = ex2(y.y);
+          sum0 = f2_add(sum0, f2_pack(s[n][0], s[n][1]));
+          sum1 = f2_add(sum1, f2_pack(s[n][2], s[n][3]));
+        }
+        const float2 t0 = f2_unpack(sum0), t1 = f2_unpack(sum1);
+        l[0] = fmaf(l[0], keep[0], t0.x + t0.y);
+        l[1] = fmaf(l[1], keep[1], t1.x + t1.y);
+        if (__any_sync(0xffffffffu, keep[0] != 1.0f || keep[1] != 1.0f)) {
+#pragma unroll
+          for (int n = 0; n < DN; n++) {
+            o[n][0] *= keep[0];
+            o[n][1] *= keep[0];
+            o[n][2] *= keep[1];
+            o[n][3] *= keep[1];
+          }
+        }
+        // O += P V; the weights are rounded to the type of v, the sum l is not
+#pragma unroll
+        for (int kk = 0; kk < NT / 2; kk++) {
+          const uint32_t a[4] = {
+              pack2<T>(s[2 * kk][0], s[2 * kk][1]), pack2<T>(s[2 * kk][2], s[2 * kk][3]),
+              pack2<T>(s[2 * kk + 1][0], s[2 * kk + 1][1]), pack2<T>(s[2 * kk + 1][2], s[2 * kk + 1][3])};
+#pragma unroll
+          for (int n = 0; n < DN; n += 2) {
+            uint32_t b0, b1, b2, b3;
+            ldsm_x4_t(vs + (n / (2 * PK)) * C::PANEL + kk * 16 * C::PV * 2 + (vat ^ (n % (2 * PK) * 16)), b0, b1,
+                      b2, b3);
+            mma_tile<T>(o[n], a, b0, b1);
+            mma_tile<T>(o[n + 1], a, b2, b3);
+          }
+        }
+      }
+      fetched();
+      if (++stage == kMmaStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+    }
+    if (KW == 1 && S == 1)
+      write_rows<T, DN>(A, D, hk, o, m, l, row_q, row_h, row_seen, live, kend, lane);
+    else  // one head (cta_heads is 1)
+      join_rows<T, DP, RW, WARPS>(A, D, hk, smem, o, m, l, r0, nrows, kend, S, split);
   }
 }
 
-template <typename T, int DP, int RW>
+template <typename T, int DP, int RW, int WARPS>
 cudaError_t launch_attention_mma(AttnArgs& A, cudaStream_t st) {
-  using C = MmaCfg<DP, RW>;
-  auto kernel = k_attention_mma<T, DP, RW>;
+  using C = MmaCfg<DP, RW, WARPS>;
+  auto kernel = k_attention_mma<T, DP, RW, WARPS>;
   static LaunchSetup setup;
   int ctas = 0;
-  cudaError_t err = resident_ctas(setup, kernel, kMmaThreads, C::SMEM, &ctas);
+  cudaError_t err = resident_ctas(setup, kernel, C::THREADS, C::SMEM, &ctas);
   if (err != cudaSuccess) return err;
-  const long long rows = (long long)A.q_tokens * A.group;
-  const long long slots = rows / C::ROWS + A.documents;
-  // The host knows mean lengths only: documents shorter than a tile have two slots each, of
-  // which one is empty, and share a CTA.
-  A.cta_slots = rows <= (long long)A.documents * C::ROWS ? 2 : 1;
-  A.slots = (int)slots;
-  const long long groups = (slots + A.cta_slots - 1) / A.cta_slots;
-  // The keys of a tile are split over a cluster while each part has two tiles or more by the
-  // mean length, until there are eight times the CTAs that fit on the device: documents of
-  // very different lengths then even out.
-  const long long keys = A.kv_tokens / A.documents;
+  set_slots(A, C::ROWS, A.group);
+  const long long tiles = (long long)A.slots * A.kv_heads;
+  // The keys of a tile are split over a cluster until there are twice the CTAs that fit on the
+  // device, which evens out documents of different lengths, with eight tiles of keys or more
+  // for each (by the mean length: the host does not know the offsets); or with one, while that
+  // is all that half fills the device.
+  const long long ktiles = (A.kv_tokens / A.documents + C::TKEYS - 1) / C::TKEYS;
   int splits = 1;
-  while (splits < kMaxSplits && groups * A.kv_heads * splits <= 4LL * ctas &&
-         keys >= 4LL * kMmaKeys * splits)
+  while (splits < kMaxSplits && (tiles * splits < ctas / 2 ? ktiles >= 2 * splits
+                                                           : tiles * splits < 2LL * ctas && ktiles >= 16 * splits))
     splits *= 2;
   A.splits = splits;
   // many tiles: a CTA takes several heads of a tile, the next head's loads under way while it
   // computes, as long as three rounds of CTAs are left
   A.cta_heads = 1;
   if (C::KW == 1 && splits == 1)
-    A.cta_heads = (int)std::max(1LL, std::min((long long)A.kv_heads, groups * A.kv_heads / (3LL * ctas)));
-  const long long items = groups * ((A.kv_heads + A.cta_heads - 1) / A.cta_heads);
+    A.cta_heads = (int)std::max(1LL, std::min((long long)A.kv_heads, tiles / (3LL * ctas)));
+  const long long items = (long long)A.slots * ((A.kv_heads + A.cta_heads - 1) / A.cta_heads);
   const long long grid = items * splits;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof cfg);
   cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(kMmaThreads);
+  cfg.blockDim = dim3(C::THREADS);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -604,8 +591,8 @@ cudaError_t launch_attention_mma(AttnArgs& A, cudaStream_t st) {
   memset(&k, 0, sizeof k);
   memset(&v, 0, sizeof v);
   if (A.kv_tokens > 0 &&
-      (!make_map_heads(&k, A.k, BF16, A.kv_tokens, A.kv_heads, A.head_dim, kMmaKeys, C::PV) ||
-       !make_map_heads(&v, A.v, BF16, A.kv_tokens, A.kv_heads, A.head_dim, kMmaKeys, C::PV)))
+      (!make_map_heads(&k, A.k, BF16, A.kv_tokens, A.kv_heads, A.head_dim, C::TKEYS, C::PV) ||
+       !make_map_heads(&v, A.v, BF16, A.kv_tokens, A.kv_heads, A.head_dim, C::TKEYS, C::PV)))
     return cudaErrorInvalidValue;
   return cudaLaunchKernelEx(&cfg, kernel, A, k, v);
 }
@@ -613,12 +600,15 @@ cudaError_t launch_attention_mma(AttnArgs& A, cudaStream_t st) {
 template <typename T, int DP>
 cudaError_t launch_attention_mma(AttnArgs& A, cudaStream_t st) {
   // The fewest row warps that hold the mean document's rows; fewer still where the tiles, split
-  // as far as they go, would not fill the device (K and V are then read again, from L2).
+  // as far as they go, would not fill the device (K and V are then read again, from L2). Where
+  // even so there is at most one CTA for an SM, it has eight warps and tiles of 128 keys.
   const long long rows = (long long)A.q_tokens * A.group, mean = rows / A.documents;
   auto ctas = [&](int n) { return (rows / n + A.documents) * A.kv_heads * kMaxSplits; };
-  if (mean <= 16 || ctas(32) < 148) return launch_attention_mma<T, DP, 1>(A, st);
-  if (mean <= 32 || ctas(64) < 148) return launch_attention_mma<T, DP, 2>(A, st);
-  return launch_attention_mma<T, DP, 4>(A, st);
+  const bool wide = ctas(16) <= 148 && A.kv_tokens / A.documents >= 1024;
+  if (mean <= 16 || ctas(32) < 148)
+    return wide ? launch_attention_mma<T, DP, 1, 8>(A, st) : launch_attention_mma<T, DP, 1, 4>(A, st);
+  if (mean <= 32 || ctas(64) < 148) return launch_attention_mma<T, DP, 2, 4>(A, st);
+  return launch_attention_mma<T, DP, 4, 4>(A, st);
 }
 
 template <typename T>

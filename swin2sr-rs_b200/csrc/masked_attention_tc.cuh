@@ -1,8 +1,8 @@
 // The attention of masked_attention.cu on tcgen05, for documents with many queries.
 //
 // A CTA takes 256 query rows of one document and head as two tiles of 128, which share every
-// K and V tile of 128 keys that TMA brings in. Ten warps: two groups of four for the softmax
-// of the two tiles, one that loads, one that issues the MMAs:
+// K and V tile of 128 keys that TMA brings in. Two groups of four warps do the softmax
+// of the two tiles; of a third group one warp loads and one issues the MMAs:
 //   S_w = Q_w K_i^T      both operands from shared memory, S_w in TMEM (128 columns)
 //   softmax group w      reads S_w, a row per thread, and writes the weights P_w as 16-bit
 //                        values over the first half of S_w's columns
@@ -19,7 +19,7 @@ namespace s2s {
 namespace {
 
 constexpr int kTcTile = 128;     // rows and keys of a tile
-constexpr int kTcThreads = 320;
+constexpr int kTcThreads = 384;
 constexpr int kTcPanel = kTcTile * 128;  // bytes of 128 rows of 64 values
 
 template <int NP>  // panels of 64 values: head_dim <= 64 * NP
@@ -86,6 +86,33 @@ __device__ __forceinline__ void loaded(uint32_t (&r)[32]) {
                       "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
 
+// 2^x of two values on the multiply-add pipe: x = n + f with n the nearest whole number (by
+// adding 1.5 2^23, after which n is in the low bits), 2^f by the polynomial of degree 4 of least
+// relative error on [-1/2, 1/2] (2.6e-6; the weights are rounded to 2^-9 or 2^-12 next), n into
+// the exponent. Below 2^-125 it stays there.
+__device__ __forceinline__ F2 ex2_poly(F2 x) {
+  const float2 xs = f2_unpack(x);
+  const F2 c = f2_pack(fmaxf(xs.x, -125.0f), fmaxf(xs.y, -125.0f));
+  const F2 t = f2_add(c, f2_both(12582912.0f));
+  const F2 f = f2_add(c, f2_fma(t, f2_both(-1.0f), f2_both(12582912.0f)));
+  F2 p = f2_fma(f2_both(0.009570102207362652f), f, f2_both(0.05591785907745361f));
+  p = f2_fma(p, f, f2_both(0.240247443318367f));
+  p = f2_fma(p, f, f2_both(0.6931217908859253f));
+  p = f2_fma(p, f, f2_both(0.9999992847442627f));
+  const float2 n = f2_unpack(t), y = f2_unpack(p);
+  return f2_pack(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(n.x) << 23)),
+                 __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(n.y) << 23)));
+}
+
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 __device__ __forceinline__ void group_sync(int id) {
   asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
 }
@@ -146,7 +173,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   int tile = 0;
   Doc D;
   // the CTA's first query; slots behind the document's last tile have none
-  const bool any = find_document(A, slot, A.slots, 2 * kTcTile, 1, lane, &D, &tile) &&
+  const bool any = find_document(A, slot, 2 * kTcTile, 1, lane, &D, &tile) &&
                    (long long)tile * (2 * kTcTile) < D.nq;
   const int i0 = any ? tile * (2 * kTcTile) : D.nq;
   int rows[2], kend[2], n[2];
@@ -159,8 +186,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int N = max(n[0], n[1]), kmax = max(kend[0], kend[1]);
   const int ksteps = (A.head_dim + 15) / 16;
 
-  if (warp == 8) {
-    if (lane == 0) {
+  // registers: 384 threads begin with 168 each; the softmax groups take what the third gives
+  // (2 * 128 * 200 + 128 * 96 = 63488 of 64512)
+  if (warp >= 8) {
+    fewer_registers<96>();
+    if (warp == 8 && lane == 0) {
       // ------------------------------------------------------------------ loads
       auto load = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int head, int row) {
         mbar_arrive_expect_tx(bar, C::QB);
@@ -183,82 +213,84 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int k = max(0, it - C::STAGES); k < it; k++)
         mbar_wait(&kv_full[k % C::STAGES], (k / C::STAGES) & 1, DEV_TIMEOUT_FULL);
     }
-  } else if (warp == 9) {
-    // --------------------------------------------------------------------- MMAs
-    const uint32_t id_s = idesc_16(128, 128, BF16, false);
-    const uint32_t id_o = idesc_16(128, ksteps * 16, BF16, true);
-    bool ok = true;
-    auto arrived = [&](int it) {
-      ok = ok && mbar_wait(&kv_full[it % C::STAGES], (it / C::STAGES) & 1, DEV_TIMEOUT_FULL);
-      tc_fence_after();
-    };
-    auto scores = [&](int w, int i) {
-      if (lane == 0) {
-        const uint32_t q = smem_u32(sQ + w * C::QB), k = smem_u32(ring + ((2 * i) % C::STAGES) * C::QB);
+    if (warp == 9) {
+      // --------------------------------------------------------------------- MMAs
+      const uint32_t id_s = idesc_16(128, 128, BF16, false);
+      const uint32_t id_o = idesc_16(128, ksteps * 16, BF16, true);
+      bool ok = true;
+      auto arrived = [&](int it) {
+        ok = ok && mbar_wait(&kv_full[it % C::STAGES], (it / C::STAGES) & 1, DEV_TIMEOUT_FULL);
+        tc_fence_after();
+      };
+      auto scores = [&](int w, int i) {
+        if (lane == 0) {
+          const uint32_t q = smem_u32(sQ + w * C::QB), k = smem_u32(ring + ((2 * i) % C::STAGES) * C::QB);
 #pragma unroll
-        for (int c = 0; c < 4 * NP; c++) {
-          if (c >= ksteps) break;
-          const uint32_t at = (c >> 2) * kTcPanel + (c & 3) * 32;
-          tc_mma_f16(tmem + w * 128, sw128_desc(q + at), sw128_desc(k + at), id_s, c != 0);
-        }
-        tc_commit(&s_full[w]);
-      }
-      __syncwarp();
-    };
-    if (N > 0) {
-      arrived(0);
-      for (int w = 0; w < 2 && ok; w++)
-        if (n[w] > 0) {
-          ok = mbar_wait(&q_full[w], 0, DEV_TIMEOUT_FULL);
-          tc_fence_after();
-          if (ok) scores(w, 0);
-        }
-      if (ok && lane == 0) tc_commit(&kv_empty[0]);
-    }
-    for (int i = 0; i < N && ok; i++) {
-      const int vs = (2 * i + 1) % C::STAGES;
-      arrived(2 * i + 1);
-      if (!ok) break;
-      // keys that no row sees, and rows of other documents behind them, have zero weights:
-      // what lies there must not reach the product
-      const int valid = min(kTcTile, kmax - i * kTcTile), vsteps = (valid + 15) / 16;
-      if (valid & 15) {
-        for (int p = 0; p < NP; p++)
-          for (int c = lane; c < (vsteps * 16 - valid) * 8; c += 32)
-            *reinterpret_cast<uint4*>(ring + vs * C::QB + p * kTcPanel + valid * 128 + c * 16) =
-                make_uint4(0, 0, 0, 0);
-        fence_proxy_async_smem();
-        __syncwarp();
-      }
-      for (int w = 0; w < 2 && ok; w++) {
-        if (i < n[w]) {
-          ok = mbar_wait(&p_full[w], i & 1, DEV_TIMEOUT_ACC);
-          tc_fence_after();
-          if (!ok) break;
-          if (lane == 0) {
-            const uint32_t v = smem_u32(ring + vs * C::QB);
-#pragma unroll
-            for (int c = 0; c < 8; c++) {
-              if (c >= vsteps) break;
-              tc_mma_f16_ta(tmem + 256 + w * 128, tmem + w * 128 + c * 8, sw128_mn_desc(v + c * 2048, kTcPanel),
-                            id_o, (i | c) != 0);
-            }
-            if (i == n[w] - 1) tc_commit(&o_full[w]);
+          for (int c = 0; c < 4 * NP; c++) {
+            if (c >= ksteps) break;
+            const uint32_t at = (c >> 2) * kTcPanel + (c & 3) * 32;
+            tc_mma_f16(tmem + w * 128, sw128_desc(q + at), sw128_desc(k + at), id_s, c != 0);
           }
+          tc_commit(&s_full[w]);
+        }
+        __syncwarp();
+      };
+      if (N > 0) {
+        arrived(0);
+        for (int w = 0; w < 2 && ok; w++)
+          if (n[w] > 0) {
+            ok = mbar_wait(&q_full[w], 0, DEV_TIMEOUT_FULL);
+            tc_fence_after();
+            if (ok) scores(w, 0);
+          }
+        if (ok && lane == 0) tc_commit(&kv_empty[0]);
+      }
+      for (int i = 0; i < N && ok; i++) {
+        const int vs = (2 * i + 1) % C::STAGES;
+        arrived(2 * i + 1);
+        if (!ok) break;
+        // keys that no row sees, and rows of other documents behind them, have zero weights:
+        // what lies there must not reach the product
+        const int valid = min(kTcTile, kmax - i * kTcTile), vsteps = (valid + 15) / 16;
+        if (valid & 15) {
+          for (int p = 0; p < NP; p++)
+            for (int c = lane; c < (vsteps * 16 - valid) * 8; c += 32)
+              *reinterpret_cast<uint4*>(ring + vs * C::QB + p * kTcPanel + valid * 128 + c * 16) =
+                  make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();
           __syncwarp();
         }
-        if (w == 1 && lane == 0) tc_commit(&kv_empty[vs]);
-        if (i + 1 < N && w == 0) arrived(2 * i + 2);
-        if (ok && i + 1 < n[w]) scores(w, i + 1);
+        for (int w = 0; w < 2 && ok; w++) {
+          if (i < n[w]) {
+            ok = mbar_wait(&p_full[w], i & 1, DEV_TIMEOUT_ACC);
+            tc_fence_after();
+            if (!ok) break;
+            if (lane == 0) {
+              const uint32_t v = smem_u32(ring + vs * C::QB);
+#pragma unroll
+              for (int c = 0; c < 8; c++) {
+                if (c >= vsteps) break;
+                tc_mma_f16_ta(tmem + 256 + w * 128, tmem + w * 128 + c * 8, sw128_mn_desc(v + c * 2048, kTcPanel),
+                              id_o, (i | c) != 0);
+              }
+              if (i == n[w] - 1) tc_commit(&o_full[w]);
+            }
+            __syncwarp();
+          }
+          if (w == 1 && lane == 0) tc_commit(&kv_empty[vs]);
+          if (i + 1 < N && w == 0) arrived(2 * i + 2);
+          if (ok && i + 1 < n[w]) scores(w, i + 1);
+        }
+        if (ok && i + 1 < N && lane == 0) tc_commit(&kv_empty[(2 * i + 2) % C::STAGES]);
       }
-      if (ok && i + 1 < N && lane == 0) tc_commit(&kv_empty[(2 * i + 2) % C::STAGES]);
-    }
-    // TMEM is freed when every MMA has retired
-    if (lane == 0) {
-      tc_commit(fin);
-      mbar_wait(fin, 0, DEV_TIMEOUT_ACC);
+      // TMEM is freed when every MMA has retired
+      if (lane == 0) {
+        tc_commit(fin);
+        mbar_wait(fin, 0, DEV_TIMEOUT_ACC);
+      }
     }
   } else {
+    more_registers<200>();
     // ------------------------------------------------------------------ softmax
     const int w = warp >> 2, r = tid & 127;
     const int rows_w = w ? rows[1] : rows[0], n_w = w ? n[1] : n[0];
@@ -268,7 +300,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int open = rows_w > 0 ? seen(A, D, i0 + w * kTcTile) : 0;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t ts = lanes + w * 128, to = lanes + 256 + w * 128;
-    const float scale2 = A.scale * kLog2e, cap2 = A.cap * kLog2e;
+    const float unit = A.scale * kLog2e, raw_cap = A.cap / A.scale;
     const float to_cap = A.cap > 0.0f ? A.scale / A.cap : 0.0f;
     bool ok = true;
     float m = -INFINITY, l = 0.0f;
@@ -290,7 +322,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (a < A.axes) {
           const int* qa = A.qpos + (int64_t)a * A.q_tokens + D.q0;
           ref[a] = qa[i0];
-          slope[a] = fabsf(A.slopes[a * A.q_heads + h]) * kLog2e;
+          slope[a] = fabsf(A.slopes[a * A.q_heads + h]) / A.scale;
           qf[a] = slope[a] * (float)(int)((unsigned)qa[live ? i : i0] - (unsigned)ref[a]);
         }
       key_positions(0);
@@ -320,31 +352,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       auto set = [&](int j, float x) { s[j >> 5][j & 31] = __float_as_uint(x); };
 
       if (!PLAIN) {
-        // scores in units of log 2
         if (A.cap > 0.0f) {
 #pragma unroll
-          for (int c = 0; c < 4; c++) {
-            float x[32];
-#pragma unroll
-            for (int e = 0; e < 32; e++) x[e] = __uint_as_float(s[c][e]);
-            capped(x, to_cap, cap2);
-#pragma unroll
-            for (int e = 0; e < 32; e++) s[c][e] = __float_as_uint(x[e]);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 128; j++) set(j, at(j) * scale2);
+          for (int c = 0; c < 4; c++) capped(reinterpret_cast<float (&)[32]>(s[c]), to_cap, raw_cap);
         }
 #pragma unroll
         for (int a = 0; a < S2S_MAX_AXES; a++)
           if (a < A.axes) {
+            const F2 q2 = f2_both(-qf[a]);
 #pragma unroll
             for (int j = 0; j < 128; j += 4) {
-              const float4 k = *reinterpret_cast<const float4*>(kp + a * kTcTile + j);
-              set(j, at(j) - fabsf(qf[a] - k.x));
-              set(j + 1, at(j + 1) - fabsf(qf[a] - k.y));
-              set(j + 2, at(j + 2) - fabsf(qf[a] - k.z));
-              set(j + 3, at(j + 3) - fabsf(qf[a] - k.w));
+              const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(kp + a * kTcTile + j);
+              const float2 x = f2_unpack(f2_add(k.x, q2)), y = f2_unpack(f2_add(k.y, q2));
+              set(j, at(j) - fabsf(x.x));
+              set(j + 1, at(j + 1) - fabsf(x.y));
+              set(j + 2, at(j + 2) - fabsf(y.x));
+              set(j + 3, at(j + 3) - fabsf(y.y));
             }
           }
       }
@@ -356,10 +379,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int j = 0; j < 128; j++) top[j & 3] = fmaxf(top[j & 3], at(j));
-      float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-      const float unit = PLAIN ? scale2 : 1.0f;
-      high *= unit;
+      for (int j = 0; j < 128; j += 2) top[(j >> 1) & 3] = max3(top[(j >> 1) & 3], at(j), at(j + 1));
+      const float high = fmaxf(max3(top[0], top[1], top[2]), top[3]) * unit;
       if (t == 0) {
         m = high;
       } else if (__any_sync(0xffffffffu, high > m + 8.0f)) {
@@ -374,22 +395,28 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           tmem_st16(to + c, o);
         }
       }
-      const float base = m == -INFINITY ? 0.0f : m;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      const F2 base2 = f2_both(m == -INFINITY ? 0.0f : -m), unit2 = f2_both(unit);
+      F2 sum[2] = {0, 0};  // two zeros each
 #pragma unroll
       for (int c = 0; c < 2; c++) {
         uint32_t p[32];
 #pragma unroll
         for (int j = 0; j < 32; j++) {
-          const float x = ex2(fmaf(at(64 * c + 2 * j), unit, -base));
-          const float y = ex2(fmaf(at(64 * c + 2 * j + 1), unit, -base));
-          sum[(2 * j) & 3] += x;
-          sum[(2 * j + 1) & 3] += y;
-          p[j] = pack2<T>(x, y);
+          F2 x = f2_fma(f2_pack(at(64 * c + 2 * j), at(64 * c + 2 * j + 1)), unit2, base2);
+          if (j % 4 == 3) {
+            x = ex2_poly(x);
+          } else {
+            const float2 xs = f2_unpack(x);
+            x = f2_pack(ex2(xs.x), ex2(xs.y));
+          }
+          sum[j & 1] = f2_add(sum[j & 1], x);
+          const float2 y = f2_unpack(x);
+          p[j] = pack2<T>(y.x, y.y);
         }
         tmem_st32(ts + c * 32, p);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      const float2 total = f2_unpack(f2_add(sum[0], sum[1]));
+      l += total.x + total.y;
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -401,7 +428,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     tc_fence_after();
     const bool none = m == -INFINITY;
     const float inv = none ? 0.0f : 1.0f / l;
-    bool bad = false;
+    float check = 0.0f;  // NaN where an output is NaN or infinite
     T* out = static_cast<T*>(A.out.data) + (int64_t)(D.q0 + i) * A.out.token + (int64_t)h * A.out.head;
     if (rows_w > 0)
       for (int c = 0; c < ksteps * 16; c += 16) {
@@ -410,9 +437,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         uint32_t v[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          const float x = none ? 0.0f : __uint_as_float(o[2 * e]) * inv;
-          const float y = none ? 0.0f : __uint_as_float(o[2 * e + 1]) * inv;
-          bad = bad || !(fabsf(x) < INFINITY) || !(fabsf(y) < INFINITY);
+          const float x = n_w > 0 ? __uint_as_float(o[2 * e]) * inv : 0.0f;
+          const float y = n_w > 0 ? __uint_as_float(o[2 * e + 1]) * inv : 0.0f;
+          check = fmaf(x, 0.0f, fmaf(y, 0.0f, check));
           v[e] = pack2<T>(x, y);
         }
         if (live) {
@@ -424,7 +451,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       A.lse[(int64_t)h * A.q_tokens + D.q0 + i] = none ? -INFINITY : (m + log2f(l)) * kLn2;
     // keys of the document that this row does not see had zero weights: a NaN or infinity
     // among their values shows here, and the row is done again without them
-    unsigned redo = __ballot_sync(0xffffffffu, bad && live && mine < kmax);
+    unsigned redo = __ballot_sync(0xffffffffu, check != 0.0f && live && mine < kmax);
     __syncwarp();
     while (redo) {
       const int src = __ffs(redo) - 1;
@@ -452,10 +479,9 @@ cudaError_t launch_attention_tc(AttnArgs& A, cudaStream_t st) {
       !make_map_heads(&k, A.k, BF16, A.kv_tokens, A.kv_heads, A.head_dim, kTcTile, 64) ||
       !make_map_heads(&v, A.v, BF16, A.kv_tokens, A.kv_heads, A.head_dim, kTcTile, 64))
     return cudaErrorInvalidValue;
-  const long long slots = (long long)A.q_tokens / (2 * kTcTile) + A.documents;
-  const long long grid = slots * A.q_heads;
+  set_slots(A, 2 * kTcTile, 1);
+  const long long grid = (long long)A.slots * A.q_heads;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-  A.slots = (int)slots;
   return launch_pdl(kernel, dim3((unsigned)grid), dim3(kTcThreads), C::SMEM, st, A, q, k, v);
 }
 
