@@ -1,50 +1,44 @@
 // The attention of masked_attention.cu on tcgen05, for documents with many queries.
 //
 // A CTA takes 256 query rows of one document and head as two tiles of 128, which share every
-// K and V tile of 128 keys that TMA brings in. Two groups of four warps do the softmax
-// of the two tiles; of a third group one warp loads and one issues the MMAs:
-//   S_w = Q_w K_i^T      both operands from shared memory, S_w in TMEM (128 columns)
-//   softmax group w      reads S_w, a row per thread, and writes the weights P_w as 16-bit
-//                        values over the first half of S_w's columns
-//   O_w += P_w V_i       P_w from TMEM, V_i as it lies in memory (keys by values: the MN-major
+// K and V tile that TMA brings in. Two groups of four warps do the softmax of the two tiles; of
+// a third group one warp loads and one issues the MMAs:
+//   S = Q_w K_i^T        both operands from shared memory, S in one of the score buffers in TMEM
+//   softmax group w      reads S, a row per thread, and writes the weights P as 16-bit values
+//                        over the first half of S's columns
+//   O_w += P V_i         P from TMEM, V_i as it lies in memory (keys by values: the MN-major
 //                        operand form), O_w in TMEM
-// While group 0 is at its softmax the tensor core does tile 1's two products and the other way
-// round. The output is scaled again only when a row's maximum grows by more than 2^8 beyond
-// the one its weights refer to (weights then stay below 2^8, in the range of both types, and
-// the sums are 32-bit), which after the first tiles is rare; the group does it itself, as
-// S_w(i) being complete means O_w += P_w V_{i-1} is too.
+// The score products run ahead of the softmax: three buffers of 128 keys for head_dim <= 64, four
+// of 64 keys beyond (TMEM holds 512 columns, of which the outputs take 128 or 256). With one
+// buffer a tile, each group's softmax (1900 cycles) waited for its own two products and they for
+// it, 3200-3400 cycles a round.
+//
+// The output is scaled again only when a row's maximum grows by more than 2^8 beyond the one its
+// weights refer to (weights then stay below 2^8, in the range of both types, and the sums are
+// 32-bit), which after the first tiles is rare; the group does it itself.
 #pragma once
 
 namespace s2s {
 namespace {
 
-constexpr int kTcTile = 128;     // rows and keys of a tile
+constexpr int kTcTile = 128;     // rows of a tile
 constexpr int kTcThreads = 384;
-constexpr int kTcPanel = kTcTile * 128;  // bytes of 128 rows of 64 values
 
 template <int NP>  // panels of 64 values: head_dim <= 64 * NP
 struct TcCfg {
-  static constexpr int QB = NP * kTcPanel;  // a Q, K or V tile
-  static constexpr int STAGES = NP == 1 ? 8 : 4;
-  static constexpr int RING = 2 * QB;
-  static constexpr int POS = RING + STAGES * QB;
-  static constexpr int BARS = POS + 2 * 2 * S2S_MAX_AXES * kTcTile * 4;
-  static constexpr int NBARS = 2 * STAGES + 9;
+  static constexpr int BN = NP == 1 ? 128 : 64;      // keys of a tile
+  static constexpr int NB = NP == 1 ? 3 : 4;         // score buffers
+  static constexpr int OUT = NB * BN;                // TMEM column of the outputs
+  static constexpr int QB = NP * kTcTile * 128;      // bytes of a Q tile
+  static constexpr int KB = NP * BN * 128;           // of a K or V tile
+  static constexpr int STAGES = 4;                   // of K, and of V
+  static constexpr int KRING = 2 * QB;
+  static constexpr int VRING = KRING + STAGES * KB;
+  static constexpr int POS = VRING + STAGES * KB;
+  static constexpr int BARS = POS + 2 * 2 * S2S_MAX_AXES * BN * 4;
+  static constexpr int NBARS = 4 * STAGES + 3 * NB + 4;
   static constexpr int SMEM = BARS + NBARS * 8 + 16 + 1024;  // + alignment
 };
-
-// A [rows][64] panel in the 128-byte swizzle read along its rows as the contraction (V: keys
-// contract, values are the N extent): 64-value panels `panel` bytes apart, groups of eight
-// keys 1024 bytes apart.
-__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t panel) {
-  uint64_t d = 0;
-  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
-  d |= (uint64_t)((panel >> 4) & 0x3FFFu) << 16;
-  d |= (uint64_t)(1024u >> 4) << 32;
-  d |= (uint64_t)1u << 46;
-  d |= (uint64_t)2u << 61;
-  return d;
-}
 
 // Instruction descriptor: fp16 or bf16 operands, fp32 sums; B K-major, or MN-major.
 __device__ __forceinline__ uint32_t idesc_16(int M, int N, bool bf16, bool b_mn) {
@@ -86,36 +80,45 @@ __device__ __forceinline__ void loaded(uint32_t (&r)[32]) {
                       "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
 
-// The MMA and its commit as one thread of a whole warp issues them (`one`: elect_one). All lanes
-// run the code around them, so that the descriptors stay in uniform registers: with the loop
-// inside `if (lane == 0)` each MMA took 130 cycles to issue, four times its execution.
+// What an MMA costs the issuing warp counts: it shares a scheduler with two softmax warps. All lanes
+// run the loop, steered by values that the compiler knows to be uniform, and an elected one issues;
+// descriptors are the 32-bit word that varies and a constant, predicates are constants but for the
+// first of an output product. An MMA then takes 22 cycles to issue; in a loop of one lane, or with
+// whole descriptors, 85 to 130, more than its execution.
 __device__ __forceinline__ uint32_t elect_one() {
   uint32_t one;
   asm volatile(
       "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(one));
   return one;
 }
-__device__ __forceinline__ void mma_ss(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                       uint32_t accumulate) {
+// High words: groups of eight rows 1024 bytes apart, descriptor version, 128-byte swizzle.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t saddr, uint32_t lead) {
+  return ((saddr >> 4) & 0x3FFFu) | (lead >> 4) << 16;
+}
+template <bool ACC>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one)
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "n"(ACC ? 1 : 0), "n"(kDescHigh)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t one, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                       uint32_t accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one)
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(kDescHigh)
       : "memory");
 }
-__device__ __forceinline__ void commit_to(uint32_t one, uint64_t* bar) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
   asm volatile(
-      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
-      "r"(one)
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, 1, 0;\n\t"
+      "mov.b64 b, {%2, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "n"(kDescHigh)
       : "memory");
 }
 
@@ -150,40 +153,62 @@ __device__ __forceinline__ void group_sync(int id) {
   asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
 }
 
+// The products of a CTA in the order they are issued: tile 0 and 1 in turn, for key tile after
+// key tile, the one with more of them alone at the end.
+struct TcStep {
+  int w, i;
+  __device__ __forceinline__ TcStep(int n0) : w(n0 > 0 ? 0 : 1), i(0) {}
+  __device__ __forceinline__ void next(int n0, int n1) {
+    if (w == 0 && i < n1) {
+      w = 1;
+    } else {
+      i++;
+      w = i < n0 ? 0 : 1;
+    }
+  }
+};
+
 // PLAIN: no cap, no bias.
 template <typename T, int NP, bool PLAIN>
 __global__ void __launch_bounds__(kTcThreads, 1)
     k_attention_tc(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap mapQ,
                    const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV) {
   using C = TcCfg<NP>;
+  constexpr int BN = C::BN, NB = C::NB, ST = C::STAGES;
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* sQ = smem;
-  uint8_t* ring = smem + C::RING;
+  uint8_t* kring = smem + C::KRING;
+  uint8_t* vring = smem + C::VRING;
   float* spos = reinterpret_cast<float*>(smem + C::POS);  // [group][buffer][axis][key]
-  uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem + C::BARS);
-  uint64_t* kv_empty = kv_full + C::STAGES;
-  uint64_t* q_full = kv_empty + C::STAGES;  // [2], as the rest: one of each tile
-  uint64_t* s_full = q_full + 2;
-  uint64_t* p_full = s_full + 2;
-  uint64_t* o_full = p_full + 2;
-  uint64_t* fin = o_full + 2;
-  uint32_t* holder = reinterpret_cast<uint32_t*>(fin + 1);
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + C::BARS);  // [stage]
+  uint64_t* k_empty = k_full + ST;
+  uint64_t* v_full = k_empty + ST;
+  uint64_t* v_empty = v_full + ST;
+  uint64_t* s_full = v_empty + ST;  // [score buffer]
+  uint64_t* p_full = s_full + NB;
+  uint64_t* o_done = p_full + NB;   // the output product that read the buffer's weights is complete
+  uint64_t* q_full = o_done + NB;   // [tile]
+  uint64_t* fin = q_full + 2;       // [scores, outputs]: every product has retired
+  uint32_t* holder = reinterpret_cast<uint32_t*>(fin + 2);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
-    for (int s = 0; s < C::STAGES; s++) {
-      mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], 1);
+    for (int s = 0; s < ST; s++) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
     }
-    for (int w = 0; w < 2; w++) {
-      mbar_init(&q_full[w], 1);
-      mbar_init(&s_full[w], 1);
-      mbar_init(&p_full[w], 4);
-      mbar_init(&o_full[w], 1);
+    for (int b = 0; b < NB; b++) {
+      mbar_init(&s_full[b], 1);
+      mbar_init(&p_full[b], 4);
+      mbar_init(&o_done[b], 1);
     }
-    mbar_init(fin, 1);
+    for (int w = 0; w < 2; w++) mbar_init(&q_full[w], 1);
+    mbar_init(&fin[0], 1);
+    mbar_init(&fin[1], 1);
     fence_barrier_init();
     tma_prefetch_desc(&mapQ);
     tma_prefetch_desc(&mapK);
@@ -214,9 +239,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   for (int w = 0; w < 2; w++) {
     rows[w] = max(0, min(kTcTile, D.nq - i0 - w * kTcTile));
     kend[w] = rows[w] > 0 ? seen(A, D, i0 + w * kTcTile + rows[w] - 1) : 0;
-    n[w] = (kend[w] + kTcTile - 1) / kTcTile;
+    n[w] = (kend[w] + BN - 1) / BN;
   }
-  const int N = max(n[0], n[1]), kmax = max(kend[0], kend[1]);
+  const int kmax = max(kend[0], kend[1]);
   const int ksteps = (A.head_dim + 15) / 16;
 
   // registers: 384 threads begin with 168 each; the softmax groups take what the third gives
@@ -225,97 +250,121 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     fewer_registers<96>();
     if (warp == 8 && lane == 0) {
       // ------------------------------------------------------------------ loads
-      auto load = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int head, int row) {
-        mbar_arrive_expect_tx(bar, C::QB);
+      auto load = [&](uint8_t* dst, int bytes, const CUtensorMap* map, uint64_t* bar, int head, int row) {
+        mbar_arrive_expect_tx(bar, bytes);
 #pragma unroll
-        for (int p = 0; p < NP; p++) tma_load_3d(dst + p * kTcPanel, map, bar, p * 64, head, row);
+        for (int p = 0; p < NP; p++) tma_load_3d(dst + p * (bytes / NP), map, bar, p * 64, head, row);
       };
-      for (int w = 0; w < 2; w++)
-        if (n[w] > 0) load(sQ + w * C::QB, &mapQ, &q_full[w], h, D.q0 + i0 + w * kTcTile);
+      const int N = max(n[0], n[1]);
       bool ok = true;
-      int it = 0;
-      for (; it < 2 * N; it++) {
-        const int s = it % C::STAGES;
-        if (it >= C::STAGES) ok = mbar_wait(&kv_empty[s], ((it / C::STAGES) - 1) & 1, DEV_TIMEOUT_EMPTY);
+      int i = 0;
+      for (; i < N && ok; i++) {
+        const int s = i % ST;
+        if (i >= ST) ok = mbar_wait(&k_empty[s], ((i / ST) - 1) & 1, DEV_TIMEOUT_EMPTY);
         if (!ok) break;
-        load(ring + s * C::QB, it & 1 ? &mapV : &mapK, &kv_full[s], hk, D.k0 + (it >> 1) * kTcTile);
+        load(kring + s * C::KB, C::KB, &mapK, &k_full[s], hk, D.k0 + i * BN);
+        if (i == 0)
+          for (int w = 0; w < 2; w++)
+            if (n[w] > 0) load(sQ + w * C::QB, C::QB, &mapQ, &q_full[w], h, D.q0 + i0 + w * kTcTile);
+        if (i >= ST) ok = mbar_wait(&v_empty[s], ((i / ST) - 1) & 1, DEV_TIMEOUT_EMPTY);
+        if (ok) load(vring + s * C::KB, C::KB, &mapV, &v_full[s], hk, D.k0 + i * BN);
       }
       // no copy is in flight when the CTA ends, also where a wait gave up
-      for (int w = 0; w < 2; w++)
-        if (n[w] > 0) mbar_wait(&q_full[w], 0, DEV_TIMEOUT_FULL);
-      for (int k = max(0, it - C::STAGES); k < it; k++)
-        mbar_wait(&kv_full[k % C::STAGES], (k / C::STAGES) & 1, DEV_TIMEOUT_FULL);
+      if (N > 0)
+        for (int w = 0; w < 2; w++)
+          if (n[w] > 0) mbar_wait(&q_full[w], 0, DEV_TIMEOUT_FULL);
+      for (int k = max(0, i - ST); k < i; k++) {
+        mbar_wait(&k_full[k % ST], (k / ST) & 1, DEV_TIMEOUT_FULL);
+        if (ok || k < i - 1) mbar_wait(&v_full[k % ST], (k / ST) & 1, DEV_TIMEOUT_FULL);
+      }
     }
+    // values that steer the products, from reductions, which give uniform registers
+    const int n0 = (int)__reduce_max_sync(0xffffffffu, (unsigned)n[0]);
+    const int n1 = (int)__reduce_max_sync(0xffffffffu, (unsigned)n[1]);
+    const int keys = (int)__reduce_max_sync(0xffffffffu, (unsigned)kmax);
+    const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
+    const int total = n0 + n1, last = max(n0, n1) - 1;
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, int phase, unsigned code) {
+      ok = __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, code));
+    };
     if (warp == 9) {
-      // --------------------------------------------------------------------- MMAs
-      const uint32_t id_s = idesc_16(128, 128, BF16, false);
-      const uint32_t id_o = idesc_16(128, ksteps * 16, BF16, true);
-      const uint32_t one = elect_one();
-      const uint64_t dq = sw128_desc(smem_u32(sQ)), dk = sw128_desc(smem_u32(ring));
-      const uint64_t dv = sw128_mn_desc(smem_u32(ring), kTcPanel);
-      bool ok = true;
-      auto arrived = [&](int it) {
-        ok = ok && mbar_wait(&kv_full[it % C::STAGES], (it / C::STAGES) & 1, DEV_TIMEOUT_FULL);
-        tc_fence_after();
-      };
-      auto scores = [&](int w, int i) {
-        const uint64_t q = dq + w * (C::QB >> 4), k = dk + ((2 * i) % C::STAGES) * (C::QB >> 4);
-#pragma unroll
-        for (int c = 0; c < 4 * NP; c++)
-          if (c < ksteps) {
-            const uint32_t at = ((c >> 2) * kTcPanel + (c & 3) * 32) >> 4;
-            mma_ss(one, tmem + w * 128, q + at, k + at, id_s, c != 0);
-          }
-        commit_to(one, &s_full[w]);
-      };
-      if (N > 0) {
-        arrived(0);
-        for (int w = 0; w < 2 && ok; w++)
-          if (n[w] > 0) {
-            ok = mbar_wait(&q_full[w], 0, DEV_TIMEOUT_FULL);
-            tc_fence_after();
-            if (ok) scores(w, 0);
-          }
-        if (ok) commit_to(one, &kv_empty[0]);
-      }
-      for (int i = 0; i < N && ok; i++) {
-        const int vs = (2 * i + 1) % C::STAGES;
-        arrived(2 * i + 1);
+      // ----------------------------------------------------------- score products
+      const uint32_t one = elect_one(), id = idesc_16(128, BN, BF16, false);
+      const uint32_t dq = desc_low(smem_u32(sQ), 16), dk = desc_low(smem_u32(kring), 16);
+      TcStep s(n0);
+      for (int p = 0, b = 0, ph = 1; p < total; p++, s.next(n0, n1)) {
+        const int st = s.i % ST;
+        if (p >= NB) wait(&o_done[b], ph, DEV_TIMEOUT_ACC);
+        if (ok && (s.w == 0 || s.i >= n0)) wait(&k_full[st], s.i / ST, DEV_TIMEOUT_FULL);
+        if (ok && s.i == 0) wait(&q_full[s.w], 0, DEV_TIMEOUT_FULL);
         if (!ok) break;
-        // keys that no row sees, and rows of other documents behind them, have zero weights:
-        // what lies there must not reach the product
-        const int valid = min(kTcTile, kmax - i * kTcTile), vsteps = (valid + 15) / 16;
-        if (valid & 15) {
-          for (int p = 0; p < NP; p++)
-            for (int c = lane; c < (vsteps * 16 - valid) * 8; c += 32)
-              *reinterpret_cast<uint4*>(ring + vs * C::QB + p * kTcPanel + valid * 128 + c * 16) =
-                  make_uint4(0, 0, 0, 0);
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
+        tc_fence_after();
+        const uint32_t q = dq + s.w * (C::QB >> 4), k = dk + st * (C::KB >> 4), d = tm + b * BN;
+        if (one) {
+          mma_ss<false>(d, q, k, id);
 #pragma unroll
-        for (int w = 0; w < 2; w++) {
-          if (ok && i < n[w]) {
-            ok = mbar_wait(&p_full[w], i & 1, DEV_TIMEOUT_ACC);
-            tc_fence_after();
-            if (ok) {
-              const uint64_t v = dv + vs * (C::QB >> 4);
-#pragma unroll
-              for (int c = 0; c < 8; c++)
-                if (c < vsteps)
-                  mma_ts(one, tmem + 256 + w * 128, tmem + w * 128 + c * 8, v + c * (2048 >> 4), id_o, (i | c) != 0);
-              if (i == n[w] - 1) commit_to(one, &o_full[w]);
-            }
-          }
-          if (w == 1 && ok) commit_to(one, &kv_empty[vs]);
-          if (w == 0 && i + 1 < N) arrived(2 * i + 2);
-          if (ok && i + 1 < n[w]) scores(w, i + 1);
+          for (int c = 1; c < 4 * NP; c++)
+            if (c < ksteps)
+              mma_ss<true>(d, q + (((c >> 2) * kTcTile * 128 + (c & 3) * 32) >> 4),
+                           k + (((c >> 2) * BN * 128 + (c & 3) * 32) >> 4), id);
+          tc_commit(&s_full[b]);
+          if (s.w == 1 || s.i >= n1) tc_commit(&k_empty[st]);  // the K tile's last use
         }
-        if (ok && i + 1 < N) commit_to(one, &kv_empty[(2 * i + 2) % C::STAGES]);
+        __syncwarp();
+        if (++b == NB) {
+          b = 0;
+          ph ^= 1;
+        }
       }
-      // TMEM is freed when every MMA has retired
-      commit_to(one, fin);
-      mbar_wait(fin, 0, DEV_TIMEOUT_ACC);
+      if (one) tc_commit(&fin[0]);
+      __syncwarp();
+      mbar_wait(&fin[0], 0, DEV_TIMEOUT_ACC);
+    } else if (warp == 10) {
+      // ---------------------------------------------------------- output products
+      // V is read along its rows as the contraction (keys contract, values are the N extent):
+      // panels of 64 values BN * 128 bytes apart
+      const uint32_t one = elect_one(), id = idesc_16(128, ksteps * 16, BF16, true);
+      const uint32_t dv = desc_low(smem_u32(vring), BN * 128);
+      TcStep s(n0);
+      for (int p = 0, b = 0, ph = 0; p < total; p++, s.next(n0, n1)) {
+        const int st = s.i % ST, tail = keys - last * BN, steps = (tail + 15) / 16;
+        if (s.w == 0 || s.i >= n0) {
+          wait(&v_full[st], s.i / ST, DEV_TIMEOUT_FULL);
+          if (s.i == last && tail % 16) {
+            // Keys that no row sees, and rows of other documents behind them, have zero weights:
+            // what lies there must not reach the product, which takes keys by 16.
+            for (int x = 0; x < NP; x++)
+              for (int c = tail * 8 + lane; c < steps * 16 * 8; c += 32)
+                *reinterpret_cast<uint4*>(vring + st * C::KB + x * BN * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+        }
+        if (ok) wait(&p_full[b], ph, DEV_TIMEOUT_ACC);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t v = dv + st * (C::KB >> 4), d = tm + C::OUT + s.w * 64 * NP, w = tm + b * BN;
+        if (one) {
+          mma_ts(d, w, v, id, s.i != 0);
+          if (s.i < last) {
+#pragma unroll
+            for (int c = 1; c < BN / 16; c++) mma_ts(d, w + c * 8, v + c * (2048 >> 4), id);
+          } else {
+            for (int c = 1; c < steps; c++) mma_ts(d, w + c * 8, v + c * (2048 >> 4), id);
+          }
+          tc_commit(&o_done[b]);
+          if (s.w == 1 || s.i >= n1) tc_commit(&v_empty[st]);  // the V tile's last use
+        }
+        __syncwarp();
+        if (++b == NB) {
+          b = 0;
+          ph ^= 1;
+        }
+      }
+      if (one) tc_commit(&fin[1]);
+      __syncwarp();
+      mbar_wait(&fin[1], 0, DEV_TIMEOUT_ACC);
     }
   } else {
     more_registers<200>();
@@ -327,7 +376,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int mine = live ? seen(A, D, i) : 0;
     const int open = rows_w > 0 ? seen(A, D, i0 + w * kTcTile) : 0;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t ts = lanes + w * 128, to = lanes + 256 + w * 128;
+    const uint32_t to = lanes + C::OUT + w * 64 * NP;
     const float unit = A.scale * kLog2e, raw_cap = A.cap / A.scale;
     const float to_cap = A.cap > 0.0f ? A.scale / A.cap : 0.0f;
     bool ok = true;
@@ -337,12 +386,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // in shared memory, for the keys of a tile, each loaded a tile ahead by one thread
     float qf[S2S_MAX_AXES], slope[S2S_MAX_AXES];
     int ref[S2S_MAX_AXES], kraw[S2S_MAX_AXES];
-    float* pos = spos + w * 2 * S2S_MAX_AXES * kTcTile;
+    float* pos = spos + w * 2 * S2S_MAX_AXES * BN;
     auto key_positions = [&](int t) {
-      const int j = t * kTcTile + r;
+      const int j = t * BN + r;
+      if (r < BN)
 #pragma unroll
-      for (int a = 0; a < S2S_MAX_AXES; a++)
-        if (a < A.axes) kraw[a] = j < D.nk ? A.kpos[(int64_t)a * A.kv_tokens + D.k0 + j] : ref[a];
+        for (int a = 0; a < S2S_MAX_AXES; a++)
+          if (a < A.axes) kraw[a] = j < D.nk ? A.kpos[(int64_t)a * A.kv_tokens + D.k0 + j] : ref[a];
     };
     if (!PLAIN && n_w > 0) {
 #pragma unroll
@@ -356,41 +406,57 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       key_positions(0);
     }
 
+    // The place of this group's tile t in the order of the products (TcStep): its buffer and phase.
+    // A group waits for its last output product only where it needs the outputs. That cannot be
+    // one phase off: a score product waited for the output product NB places before it, output
+    // products are in order, and behind this group's tile t there are fewer than NB of the other's
+    // before the group's next (at the end too: tile 1 has at most 128 / BN key tiles more).
+    auto place = [&](int t) { return min(t, n[0]) + min(t, n[1]) + (w & (t < n[0] ? 1 : 0)); };
+    auto output_done = [&](int t) {
+      const int q = place(t);
+      if (ok) ok = mbar_wait(&o_done[q % NB], (q / NB) & 1, DEV_TIMEOUT_ACC);
+      __syncwarp();
+      tc_fence_after();
+    };
+
     for (int t = 0; t < n_w; t++) {
-      const float* kp = pos + (t & 1) * S2S_MAX_AXES * kTcTile;
+      const int q = place(t), b = q % NB;
+      const uint32_t ts = lanes + b * BN;
+      const float* kp = pos + (t & 1) * S2S_MAX_AXES * BN;
       if (!PLAIN && A.axes) {
+        if (r < BN)
 #pragma unroll
-        for (int a = 0; a < S2S_MAX_AXES; a++)
-          if (a < A.axes)
-            const_cast<float*>(kp)[a * kTcTile + r] = slope[a] * (float)(int)((unsigned)kraw[a] - (unsigned)ref[a]);
+          for (int a = 0; a < S2S_MAX_AXES; a++)
+            if (a < A.axes)
+              const_cast<float*>(kp)[a * BN + r] = slope[a] * (float)(int)((unsigned)kraw[a] - (unsigned)ref[a]);
         group_sync(1 + w);
         if (t + 1 < n_w) key_positions(t + 1);
       }
       // after a wait that gave up the group goes on without waiting, so that its four warps
       // still meet at their barrier
-      if (ok) ok = mbar_wait(&s_full[w], t & 1, DEV_TIMEOUT_ACC);
+      if (ok) ok = mbar_wait(&s_full[b], (q / NB) & 1, DEV_TIMEOUT_ACC);
       tc_fence_after();
-      uint32_t s[4][32];
+      uint32_t s[BN / 32][32];
 #pragma unroll
-      for (int c = 0; c < 4; c++) tmem_ld32_nw(ts + c * 32, s[c]);
+      for (int c = 0; c < BN / 32; c++) tmem_ld32_nw(ts + c * 32, s[c]);
       tc_wait_ld();
 #pragma unroll
-      for (int c = 0; c < 4; c++) loaded(s[c]);
+      for (int c = 0; c < BN / 32; c++) loaded(s[c]);
       auto at = [&](int j) -> float { return __uint_as_float(s[j >> 5][j & 31]); };
       auto set = [&](int j, float x) { s[j >> 5][j & 31] = __float_as_uint(x); };
 
       if (!PLAIN) {
         if (A.cap > 0.0f) {
 #pragma unroll
-          for (int c = 0; c < 4; c++) capped(reinterpret_cast<float (&)[32]>(s[c]), to_cap, raw_cap);
+          for (int c = 0; c < BN / 32; c++) capped(reinterpret_cast<float (&)[32]>(s[c]), to_cap, raw_cap);
         }
 #pragma unroll
         for (int a = 0; a < S2S_MAX_AXES; a++)
           if (a < A.axes) {
             const F2 q2 = f2_both(-qf[a]);
 #pragma unroll
-            for (int j = 0; j < 128; j += 4) {
-              const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(kp + a * kTcTile + j);
+            for (int j = 0; j < BN; j += 4) {
+              const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(kp + a * BN + j);
               const float2 x = f2_unpack(f2_add(k.x, q2)), y = f2_unpack(f2_add(k.y, q2));
               set(j, at(j) - fabsf(x.x));
               set(j + 1, at(j + 1) - fabsf(x.y));
@@ -399,15 +465,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
           }
       }
-      if ((t + 1) * kTcTile > open) {
-        const int last = mine - t * kTcTile;
+      if ((t + 1) * BN > open) {
+        const int last = mine - t * BN;
 #pragma unroll
-        for (int j = 0; j < 128; j++)
+        for (int j = 0; j < BN; j++)
           if (j >= last) set(j, -INFINITY);
       }
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int j = 0; j < 128; j += 2) top[(j >> 1) & 3] = max3(top[(j >> 1) & 3], at(j), at(j + 1));
+      for (int j = 0; j < BN; j += 2) top[(j >> 1) & 3] = max3(top[(j >> 1) & 3], at(j), at(j + 1));
       const float high = fmaxf(max3(top[0], top[1], top[2]), top[3]) * unit;
       if (t == 0) {
         m = high;
@@ -415,6 +481,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const float next = fmaxf(m, high), keep = next == -INFINITY ? 1.0f : ex2(m - next);
         m = next;
         l *= keep;
+        // the output product before this tile's is complete, this one waits for the weights
+        output_done(t - 1);
         for (int c = 0; c < ksteps * 16; c += 16) {
           uint32_t o[16];
           tmem_ld16(to + c, o);
@@ -426,7 +494,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const F2 base2 = f2_both(m == -INFINITY ? 0.0f : -m), unit2 = f2_both(unit);
       F2 sum[2] = {0, 0};  // two zeros each
 #pragma unroll
-      for (int c = 0; c < 2; c++) {
+      for (int c = 0; c < BN / 64; c++) {
         uint32_t p[32];
 #pragma unroll
         for (int j = 0; j < 32; j++) {
@@ -448,12 +516,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[w]);
+      if (lane == 0) mbar_arrive(&p_full[b]);
     }
 
     // ------------------------------------------------------------------- output
-    if (n_w > 0 && ok) ok = mbar_wait(&o_full[w], 0, DEV_TIMEOUT_ACC);
-    tc_fence_after();
+    if (n_w > 0) output_done(n_w - 1);
     const bool none = m == -INFINITY;
     const float inv = none ? 0.0f : 1.0f / l;
     float check = 0.0f;  // NaN where an output is NaN or infinite
@@ -504,8 +571,8 @@ cudaError_t launch_attention_tc(AttnArgs& A, cudaStream_t st) {
   if (err != cudaSuccess) return err;
   CUtensorMap q, k, v;
   if (!make_map_heads(&q, A.q, BF16, A.q_tokens, A.q_heads, A.head_dim, kTcTile, 64) ||
-      !make_map_heads(&k, A.k, BF16, A.kv_tokens, A.kv_heads, A.head_dim, kTcTile, 64) ||
-      !make_map_heads(&v, A.v, BF16, A.kv_tokens, A.kv_heads, A.head_dim, kTcTile, 64))
+      !make_map_heads(&k, A.k, BF16, A.kv_tokens, A.kv_heads, A.head_dim, C::BN, 64) ||
+      !make_map_heads(&v, A.v, BF16, A.kv_tokens, A.kv_heads, A.head_dim, C::BN, 64))
     return cudaErrorInvalidValue;
   set_slots(A, 2 * kTcTile, 1);
   const long long grid = (long long)A.slots * A.q_heads;
