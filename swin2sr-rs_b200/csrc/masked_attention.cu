@@ -121,55 +121,76 @@ __device__ __forceinline__ float distance_bias(const AttnArgs& A, int h, int qro
 using F2 = unsigned long long;  // two fp32 lanes of the packed operations
 __device__ __forceinline__ F2 f2_both(float x) { return f2_pack(x, x); }
 
-// Scores s -> cap * tanh(s * to_cap). Up to 1, tanh x = x P(x^2) with P the polynomial of
-// degree 6 of least relative error on [0, 1] (5e-8, by the exchange algorithm), two scores an
-// instruction; beyond, 1 - 2 / (1 + e^{2x}). The second form costs two more operations of the
-// special function unit, which softmax is bound by, so a warp takes it only where it has such
-// a score.
-__device__ __forceinline__ F2 tanh_poly(F2 x) {
-  const F2 u = f2_mul(x, x);
-  F2 p = f2_fma(f2_both(0.0010410225950181484f), u, f2_both(-0.006203379016369581f));
-  p = f2_fma(p, u, f2_both(0.020289979875087738f));
-  p = f2_fma(p, u, f2_both(-0.05345702916383743f));
-  p = f2_fma(p, u, f2_both(0.13325203955173492f));
-  p = f2_fma(p, u, f2_both(-0.33332839608192444f));
-  p = f2_fma(p, u, f2_both(0.9999999403953552f));
-  return f2_mul(x, p);
+// The larger and the smaller of three.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float d;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Capped scores, divided by the scale: s -> raw_cap tanh(s to_cap), where raw_cap to_cap = 1. For
+// arguments up to 1, tanh x = x P(x^2) with P the polynomial of least relative error on [0, 1] of
+// degree 6 (5e-8, by the exchange algorithm), up to 0.35 of degree 3 (3.5e-8); beyond 1,
+// 1 - 2 / (1 + e^{2x}). A warp takes the shortest form that is enough for all its scores: caps are
+// there for the exception, and the special function unit is busy with the exponentials.
+template <int DEGREE>
+__device__ __forceinline__ F2 tanh_over_x(F2 u) {
+  F2 p;
+  if (DEGREE == 6) {
+    p = f2_fma(f2_both(0.0010410225950181484f), u, f2_both(-0.006203379016369581f));
+    p = f2_fma(p, u, f2_both(0.020289979875087738f));
+    p = f2_fma(p, u, f2_both(-0.05345702916383743f));
+    p = f2_fma(p, u, f2_both(0.13325203955173492f));
+    p = f2_fma(p, u, f2_both(-0.33332839608192444f));
+  } else {
+    p = f2_fma(f2_both(-0.04895823076367378f), u, f2_both(0.13295799493789673f));
+    p = f2_fma(p, u, f2_both(-0.33332422375679016f));
+  }
+  return f2_fma(p, u, f2_both(0.9999999403953552f));
 }
 __device__ __forceinline__ float tanh_far(float x, float near) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(fabsf(x) * (2.0f * kLog2e))));
   return fabsf(x) > 1.0f ? copysignf(fmaf(-2.0f, r, 1.0f), x) : near;
 }
+template <int DEGREE, int N>
+__device__ __forceinline__ void cap_by(float (&s)[N], float to_cap) {
+  const F2 t = f2_both(to_cap);
+#pragma unroll
+  for (int j = 0; j < N; j += 2) {
+    const F2 v = f2_pack(s[j], s[j + 1]), x = f2_mul(v, t);
+    const float2 y = f2_unpack(f2_mul(v, tanh_over_x<DEGREE>(f2_mul(x, x))));
+    s[j] = y.x;
+    s[j + 1] = y.y;
+  }
+}
 template <int N>
-__device__ __forceinline__ void capped(float (&s)[N], float to_cap, float cap) {
-  float far = 0.0f;
+__device__ __forceinline__ void capped(float (&s)[N], float to_cap, float raw_cap) {
+  float high = -INFINITY, low = INFINITY;
 #pragma unroll
-  for (int j = 0; j < N; j++) far = fmaxf(far, fabsf(s[j]));
-  const F2 t = f2_both(to_cap), c = f2_both(cap);
-  if (__any_sync(0xffffffffu, far * to_cap > 1.0f)) {
-#pragma unroll
-    for (int j = 0; j < N; j += 2) {
-      const F2 x = f2_mul(f2_pack(s[j], s[j + 1]), t);
-      const float2 xs = f2_unpack(x), y = f2_unpack(tanh_poly(x));
-      s[j] = cap * tanh_far(xs.x, y.x);
-      s[j + 1] = cap * tanh_far(xs.y, y.y);
-    }
+  for (int j = 0; j < N; j += 2) {
+    high = max3(high, s[j], s[j + 1]);
+    low = min3(low, s[j], s[j + 1]);
+  }
+  const float far = fmaxf(high, -low) * to_cap;
+  if (!__any_sync(0xffffffffu, far > 0.35f)) {
+    cap_by<3>(s, to_cap);
+  } else if (!__any_sync(0xffffffffu, far > 1.0f)) {
+    cap_by<6>(s, to_cap);
   } else {
 #pragma unroll
     for (int j = 0; j < N; j += 2) {
-      const float2 y = f2_unpack(f2_mul(tanh_poly(f2_mul(f2_pack(s[j], s[j + 1]), t)), c));
-      s[j] = y.x;
-      s[j + 1] = y.y;
+      const F2 x = f2_mul(f2_pack(s[j], s[j + 1]), f2_both(to_cap));
+      const float2 xs = f2_unpack(x), y = f2_unpack(f2_mul(x, tanh_over_x<6>(f2_mul(x, x))));
+      s[j] = raw_cap * tanh_far(xs.x, y.x);
+      s[j + 1] = raw_cap * tanh_far(xs.y, y.y);
     }
   }
-}
-
-// The larger of three.
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
 }
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar,

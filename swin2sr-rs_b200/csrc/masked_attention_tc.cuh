@@ -8,10 +8,10 @@
 //                        over the first half of S's columns
 //   O_w += P V_i         P from TMEM, V_i as it lies in memory (keys by values: the MN-major
 //                        operand form), O_w in TMEM
-// The score products run ahead of the softmax: three buffers of 128 keys for head_dim <= 64, four
-// of 64 keys beyond (TMEM holds 512 columns, of which the outputs take 128 or 256). With one
-// buffer a tile, each group's softmax (1900 cycles) waited for its own two products and they for
-// it, 3200-3400 cycles a round.
+// The score products run ahead of the softmax. TMEM holds 512 columns, of which the outputs take 128
+// or 256: for head_dim <= 64 three score buffers of 128 keys serve both tiles in turn, beyond it
+// each tile has two of 64 keys. With one buffer of 128 keys a tile, each group's softmax (1900
+// cycles) waited for its own two products and they for it, 3200-3400 cycles a round.
 //
 // The output is scaled again only when a row's maximum grows by more than 2^8 beyond the one its
 // weights refer to (weights then stay below 2^8, in the range of both types, and the sums are
@@ -28,6 +28,7 @@ template <int NP>  // panels of 64 values: head_dim <= 64 * NP
 struct TcCfg {
   static constexpr int BN = NP == 1 ? 128 : 64;      // keys of a tile
   static constexpr int NB = NP == 1 ? 3 : 4;         // score buffers
+  static constexpr int SW = NP;                      // warps that issue score products
   static constexpr int OUT = NB * BN;                // TMEM column of the outputs
   static constexpr int QB = NP * kTcTile * 128;      // bytes of a Q tile
   static constexpr int KB = NP * BN * 128;           // of a K or V tile
@@ -36,7 +37,7 @@ struct TcCfg {
   static constexpr int VRING = KRING + STAGES * KB;
   static constexpr int POS = VRING + STAGES * KB;
   static constexpr int BARS = POS + 2 * 2 * S2S_MAX_AXES * BN * 4;
-  static constexpr int NBARS = 4 * STAGES + 3 * NB + 4;
+  static constexpr int NBARS = 4 * STAGES + 3 * NB + 5;
   static constexpr int SMEM = BARS + NBARS * 8 + 16 + 1024;  // + alignment
 };
 
@@ -45,7 +46,8 @@ __device__ __forceinline__ uint32_t idesc_16(int M, int N, bool bf16, bool b_mn)
   return idesc_f16_f32(M, N) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u);
 }
 
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+// 32 lanes x 32 columns from registers into TMEM; tc_wait_st waits for the store.
+__device__ __forceinline__ void tmem_st32_nw(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
       "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
@@ -55,6 +57,30 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
       "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
       "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
       "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+// The fragments of mma.sync in TMEM: 16 lanes x 64 fp32 columns, thread 4 g + t holding of each 8
+// columns 2 t and 2 t + 1 of rows g and g + 8; and 16 lanes x 32 columns of 16-bit pairs, pair t of
+// each 4 columns of rows g and g + 8.
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st_frag(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+      "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -122,24 +148,6 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
       : "memory");
 }
 
-// 2^x of two values on the multiply-add pipe: x = n + f with n the nearest whole number (by
-// adding 1.5 2^23, after which n is in the low bits), 2^f by the polynomial of degree 4 of least
-// relative error on [-1/2, 1/2] (2.6e-6; the weights are rounded to 2^-9 or 2^-12 next), n into
-// the exponent. Below 2^-125 it stays there.
-__device__ __forceinline__ F2 ex2_poly(F2 x) {
-  const float2 xs = f2_unpack(x);
-  const F2 c = f2_pack(fmaxf(xs.x, -125.0f), fmaxf(xs.y, -125.0f));
-  const F2 t = f2_add(c, f2_both(12582912.0f));
-  const F2 f = f2_add(c, f2_fma(t, f2_both(-1.0f), f2_both(12582912.0f)));
-  F2 p = f2_fma(f2_both(0.009570102207362652f), f, f2_both(0.05591785907745361f));
-  p = f2_fma(p, f, f2_both(0.240247443318367f));
-  p = f2_fma(p, f, f2_both(0.6931217908859253f));
-  p = f2_fma(p, f, f2_both(0.9999992847442627f));
-  const float2 n = f2_unpack(t), y = f2_unpack(p);
-  return f2_pack(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(n.x) << 23)),
-                 __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(n.y) << 23)));
-}
-
 template <int N>
 __device__ __forceinline__ void more_registers() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -153,28 +161,38 @@ __device__ __forceinline__ void group_sync(int id) {
   asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
 }
 
-// The products of a CTA in the order they are issued: tile 0 and 1 in turn, for key tile after
-// key tile, the one with more of them alone at the end.
-struct TcStep {
-  int w, i;
-  __device__ __forceinline__ TcStep(int n0) : w(n0 > 0 ? 0 : 1), i(0) {}
-  __device__ __forceinline__ void next(int n0, int n1) {
-    if (w == 0 && i < n1) {
-      w = 1;
+// Where the products of key tile i and row tile w have their place: score buffer and the parity of
+// its use. Three buffers are taken in the order of the products, tile 0 and 1 in turn and at the
+// end the one that has more (n0, n1: their key tiles); of four each tile has two.
+//
+// Every wait is at most one phase from the one waited for. A score product into a buffer waits for
+// the output product that read it last. Output products are in order, also across the tiles; none
+// starts before its group's weights, which are made from these scores. So between two uses of a
+// buffer whoever waits for the first is through. At the end of tile 0, tile 1 has at most 128 / BN
+// key tiles more, fewer than buffers, so that an output product waited for there is not passed.
+template <int NB>
+struct TcPlace {
+  int buffer, parity;
+  __device__ __forceinline__ TcPlace(int w, int i, int n0, int n1) {
+    if (NB == 4) {
+      buffer = 2 * w + (i & 1);
+      parity = (i >> 1) & 1;
     } else {
-      i++;
-      w = i < n0 ? 0 : 1;
+      const int q = min(i, n0) + min(i, n1) + (i < n0 ? w : 0);
+      buffer = q % NB;
+      parity = (q / NB) & 1;
     }
   }
 };
 
-// PLAIN: no cap, no bias.
-template <typename T, int NP, bool PLAIN>
+// MODE 0: no cap, no bias; 1: a cap; 2: a bias, with or without a cap.
+template <typename T, int NP, int MODE>
 __global__ void __launch_bounds__(kTcThreads, 1)
     k_attention_tc(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap mapQ,
                    const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV) {
   using C = TcCfg<NP>;
   constexpr int BN = C::BN, NB = C::NB, ST = C::STAGES;
+  using Place = TcPlace<NB>;
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -190,14 +208,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint64_t* p_full = s_full + NB;
   uint64_t* o_done = p_full + NB;   // the output product that read the buffer's weights is complete
   uint64_t* q_full = o_done + NB;   // [tile]
-  uint64_t* fin = q_full + 2;       // [scores, outputs]: every product has retired
-  uint32_t* holder = reinterpret_cast<uint32_t*>(fin + 2);
+  uint64_t* fin = q_full + 2;       // [issuing warp]: every product has retired
+  uint32_t* holder = reinterpret_cast<uint32_t*>(fin + 3);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
     for (int s = 0; s < ST; s++) {
       mbar_init(&k_full[s], 1);
-      mbar_init(&k_empty[s], 1);
+      mbar_init(&k_empty[s], C::SW);
       mbar_init(&v_full[s], 1);
       mbar_init(&v_empty[s], 1);
     }
@@ -207,8 +225,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&o_done[b], 1);
     }
     for (int w = 0; w < 2; w++) mbar_init(&q_full[w], 1);
-    mbar_init(&fin[0], 1);
-    mbar_init(&fin[1], 1);
+    for (int k = 0; k < 3; k++) mbar_init(&fin[k], 1);
     fence_barrier_init();
     tma_prefetch_desc(&mapQ);
     tma_prefetch_desc(&mapK);
@@ -283,240 +300,364 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int n1 = (int)__reduce_max_sync(0xffffffffu, (unsigned)n[1]);
     const int keys = (int)__reduce_max_sync(0xffffffffu, (unsigned)kmax);
     const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
-    const int total = n0 + n1, last = max(n0, n1) - 1;
+    const int last = max(n0, n1) - 1;
+    // after a wait that gave up the products go on without waiting, over whatever is there
     bool ok = true;
     auto wait = [&](uint64_t* bar, int phase, unsigned code) {
-      ok = __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, code));
+      if (ok) ok = mbar_wait(bar, phase & 1, code);
     };
-    if (warp == 9) {
+    if (warp == 9 || (C::SW == 2 && warp == 11)) {
       // ----------------------------------------------------------- score products
+      // one warp for both tiles in turn, or one for each
+      const int mine = C::SW == 1 ? -1 : warp == 11 ? 1 : 0;
       const uint32_t one = elect_one(), id = idesc_16(128, BN, BF16, false);
       const uint32_t dq = desc_low(smem_u32(sQ), 16), dk = desc_low(smem_u32(kring), 16);
-      TcStep s(n0);
-      for (int p = 0, b = 0, ph = 1; p < total; p++, s.next(n0, n1)) {
-        const int st = s.i % ST;
-        if (p >= NB) wait(&o_done[b], ph, DEV_TIMEOUT_ACC);
-        if (ok && (s.w == 0 || s.i >= n0)) wait(&k_full[st], s.i / ST, DEV_TIMEOUT_FULL);
-        if (ok && s.i == 0) wait(&q_full[s.w], 0, DEV_TIMEOUT_FULL);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t q = dq + s.w * (C::QB >> 4), k = dk + st * (C::KB >> 4), d = tm + b * BN;
-        if (one) {
-          mma_ss<false>(d, q, k, id);
+      const int rounds = mine < 0 ? last + 1 : mine ? n1 : n0;
+      for (int i = 0, st = 0, ph = 0; i < rounds; i++) {
+        wait(&k_full[st], ph, DEV_TIMEOUT_FULL);
 #pragma unroll
-          for (int c = 1; c < 4 * NP; c++)
-            if (c < ksteps)
-              mma_ss<true>(d, q + (((c >> 2) * kTcTile * 128 + (c & 3) * 32) >> 4),
-                           k + (((c >> 2) * BN * 128 + (c & 3) * 32) >> 4), id);
-          tc_commit(&s_full[b]);
-          if (s.w == 1 || s.i >= n1) tc_commit(&k_empty[st]);  // the K tile's last use
+        for (int x = 0; x < 3 - C::SW; x++) {
+          const int w = mine < 0 ? x : mine;
+          if (i < (w ? n1 : n0)) {
+            const Place at(w, i, n0, n1);
+            if (i == 0) wait(&q_full[w], 0, DEV_TIMEOUT_FULL);
+            // the output product of the buffer's last use (at first there is none: the parity
+            // is then that of the phase before)
+            wait(&o_done[at.buffer], at.parity ^ 1, DEV_TIMEOUT_ACC);
+            __syncwarp();
+            tc_fence_after();
+            const uint32_t q = dq + w * (C::QB >> 4), k = dk + st * (C::KB >> 4), d = tm + at.buffer * BN;
+            if (one) {
+              mma_ss<false>(d, q, k, id);
+#pragma unroll
+              for (int c = 1; c < 4 * NP; c++)
+                if (c < ksteps)
+                  mma_ss<true>(d, q + (((c >> 2) * kTcTile * 128 + (c & 3) * 32) >> 4),
+                               k + (((c >> 2) * BN * 128 + (c & 3) * 32) >> 4), id);
+              tc_commit(&s_full[at.buffer]);
+            }
+            __syncwarp();
+          }
+        }
+        if (one) {
+          tc_commit(&k_empty[st]);
+          // for the other tile's warp, if that tile does not need this one
+          if (C::SW == 2 && i >= (mine ? n0 : n1)) tc_commit(&k_empty[st]);
         }
         __syncwarp();
-        if (++b == NB) {
-          b = 0;
+        if (++st == ST) {
+          st = 0;
           ph ^= 1;
         }
       }
-      if (one) tc_commit(&fin[0]);
+      if (one) tc_commit(&fin[mine == 1]);
       __syncwarp();
-      mbar_wait(&fin[0], 0, DEV_TIMEOUT_ACC);
+      mbar_wait(&fin[mine == 1], 0, DEV_TIMEOUT_ACC);
     } else if (warp == 10) {
       // ---------------------------------------------------------- output products
       // V is read along its rows as the contraction (keys contract, values are the N extent):
       // panels of 64 values BN * 128 bytes apart
       const uint32_t one = elect_one(), id = idesc_16(128, ksteps * 16, BF16, true);
       const uint32_t dv = desc_low(smem_u32(vring), BN * 128);
-      TcStep s(n0);
-      for (int p = 0, b = 0, ph = 0; p < total; p++, s.next(n0, n1)) {
-        const int st = s.i % ST, tail = keys - last * BN, steps = (tail + 15) / 16;
-        if (s.w == 0 || s.i >= n0) {
-          wait(&v_full[st], s.i / ST, DEV_TIMEOUT_FULL);
-          if (s.i == last && tail % 16) {
-            // Keys that no row sees, and rows of other documents behind them, have zero weights:
-            // what lies there must not reach the product, which takes keys by 16.
-            for (int x = 0; x < NP; x++)
-              for (int c = tail * 8 + lane; c < steps * 16 * 8; c += 32)
-                *reinterpret_cast<uint4*>(vring + st * C::KB + x * BN * 128 + c * 16) = make_uint4(0, 0, 0, 0);
-            fence_proxy_async_smem();
+      for (int i = 0, st = 0, ph = 0; i <= last; i++) {
+        const int tail = keys - last * BN, steps = (tail + 15) / 16;
+        wait(&v_full[st], ph, DEV_TIMEOUT_FULL);
+        if (i == last && tail % 16) {
+          // Keys that no row sees, and rows of other documents behind them, have zero weights:
+          // what lies there must not reach the product, which takes keys by 16.
+          for (int x = 0; x < NP; x++)
+            for (int c = tail * 8 + lane; c < steps * 16 * 8; c += 32)
+              *reinterpret_cast<uint4*>(vring + st * C::KB + x * BN * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();
+        }
+        const uint32_t v = dv + st * (C::KB >> 4);
+#pragma unroll
+        for (int w = 0; w < 2; w++)
+          if (i < (w ? n1 : n0)) {
+            const Place at(w, i, n0, n1);
+            wait(&p_full[at.buffer], at.parity, DEV_TIMEOUT_ACC);
+            __syncwarp();
+            tc_fence_after();
+            const uint32_t d = tm + C::OUT + w * 64 * NP, p = tm + at.buffer * BN;
+            if (one) {
+              mma_ts(d, p, v, id, i != 0);
+              if (i < last) {
+#pragma unroll
+                for (int c = 1; c < BN / 16; c++) mma_ts(d, p + c * 8, v + c * (2048 >> 4), id);
+              } else {
+                for (int c = 1; c < steps; c++) mma_ts(d, p + c * 8, v + c * (2048 >> 4), id);
+              }
+              tc_commit(&o_done[at.buffer]);
+            }
             __syncwarp();
           }
-        }
-        if (ok) wait(&p_full[b], ph, DEV_TIMEOUT_ACC);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t v = dv + st * (C::KB >> 4), d = tm + C::OUT + s.w * 64 * NP, w = tm + b * BN;
-        if (one) {
-          mma_ts(d, w, v, id, s.i != 0);
-          if (s.i < last) {
-#pragma unroll
-            for (int c = 1; c < BN / 16; c++) mma_ts(d, w + c * 8, v + c * (2048 >> 4), id);
-          } else {
-            for (int c = 1; c < steps; c++) mma_ts(d, w + c * 8, v + c * (2048 >> 4), id);
-          }
-          tc_commit(&o_done[b]);
-          if (s.w == 1 || s.i >= n1) tc_commit(&v_empty[st]);  // the V tile's last use
-        }
+        if (one) tc_commit(&v_empty[st]);
         __syncwarp();
-        if (++b == NB) {
-          b = 0;
+        if (++st == ST) {
+          st = 0;
           ph ^= 1;
         }
       }
-      if (one) tc_commit(&fin[1]);
+      if (one) tc_commit(&fin[2]);
       __syncwarp();
-      mbar_wait(&fin[1], 0, DEV_TIMEOUT_ACC);
+      mbar_wait(&fin[2], 0, DEV_TIMEOUT_ACC);
     }
   } else {
     more_registers<200>();
     // ------------------------------------------------------------------ softmax
     const int w = warp >> 2, r = tid & 127;
     const int rows_w = w ? rows[1] : rows[0], n_w = w ? n[1] : n[0];
-    const int i = i0 + w * kTcTile + r;       // this thread's query
+    const int first = i0 + w * kTcTile;       // the tile's first query
+    const int i = first + r;                  // this thread's query
     const bool live = r < rows_w;
     const int mine = live ? seen(A, D, i) : 0;
-    const int open = rows_w > 0 ? seen(A, D, i0 + w * kTcTile) : 0;
+    const int open = rows_w > 0 ? seen(A, D, first) : 0;  // keys that every row sees
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t to = lanes + C::OUT + w * 64 * NP;
     const float unit = A.scale * kLog2e, raw_cap = A.cap / A.scale;
     const float to_cap = A.cap > 0.0f ? A.scale / A.cap : 0.0f;
+    const F2 unit2 = f2_both(unit);
+    // after a wait that gave up the group goes on without waiting, so that its four warps still
+    // meet at their barrier
     bool ok = true;
     float m = -INFINITY, l = 0.0f;
-
-    // bias: slope times position for this row's query (from the CTA's first query on) and,
-    // in shared memory, for the keys of a tile, each loaded a tile ahead by one thread
-    float qf[S2S_MAX_AXES], slope[S2S_MAX_AXES];
-    int ref[S2S_MAX_AXES], kraw[S2S_MAX_AXES];
-    float* pos = spos + w * 2 * S2S_MAX_AXES * BN;
-    auto key_positions = [&](int t) {
-      const int j = t * BN + r;
-      if (r < BN)
-#pragma unroll
-        for (int a = 0; a < S2S_MAX_AXES; a++)
-          if (a < A.axes) kraw[a] = j < D.nk ? A.kpos[(int64_t)a * A.kv_tokens + D.k0 + j] : ref[a];
-    };
-    if (!PLAIN && n_w > 0) {
-#pragma unroll
-      for (int a = 0; a < S2S_MAX_AXES; a++)
-        if (a < A.axes) {
-          const int* qa = A.qpos + (int64_t)a * A.q_tokens + D.q0;
-          ref[a] = qa[i0];
-          slope[a] = fabsf(A.slopes[a * A.q_heads + h]) / A.scale;
-          qf[a] = slope[a] * (float)(int)((unsigned)qa[live ? i : i0] - (unsigned)ref[a]);
-        }
-      key_positions(0);
-    }
-
-    // The place of this group's tile t in the order of the products (TcStep): its buffer and phase.
-    // A group waits for its last output product only where it needs the outputs. That cannot be
-    // one phase off: a score product waited for the output product NB places before it, output
-    // products are in order, and behind this group's tile t there are fewer than NB of the other's
-    // before the group's next (at the end too: tile 1 has at most 128 / BN key tiles more).
-    auto place = [&](int t) { return min(t, n[0]) + min(t, n[1]) + (w & (t < n[0] ? 1 : 0)); };
     auto output_done = [&](int t) {
-      const int q = place(t);
-      if (ok) ok = mbar_wait(&o_done[q % NB], (q / NB) & 1, DEV_TIMEOUT_ACC);
+      const Place at(w, t, n[0], n[1]);
+      if (ok) ok = mbar_wait(&o_done[at.buffer], at.parity, DEV_TIMEOUT_ACC);
       __syncwarp();
       tc_fence_after();
     };
-
-    for (int t = 0; t < n_w; t++) {
-      const int q = place(t), b = q % NB;
-      const uint32_t ts = lanes + b * BN;
-      const float* kp = pos + (t & 1) * S2S_MAX_AXES * BN;
-      if (!PLAIN && A.axes) {
-        if (r < BN)
+    // the outputs of this warp's rows so far, times `keep` (the lane's row)
+    auto scale_outputs = [&](int t, float keep) {
+      output_done(t - 1);  // this tile's waits for the weights
+      for (int c = 0; c < ksteps * 16; c += 16) {
+        uint32_t o[16];
+        tmem_ld16(to + c, o);
 #pragma unroll
-          for (int a = 0; a < S2S_MAX_AXES; a++)
-            if (a < A.axes)
-              const_cast<float*>(kp)[a * BN + r] = slope[a] * (float)(int)((unsigned)kraw[a] - (unsigned)ref[a]);
-        group_sync(1 + w);
-        if (t + 1 < n_w) key_positions(t + 1);
+        for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+        tmem_st16(to + c, o);
       }
-      // after a wait that gave up the group goes on without waiting, so that its four warps
-      // still meet at their barrier
-      if (ok) ok = mbar_wait(&s_full[b], (q / NB) & 1, DEV_TIMEOUT_ACC);
-      tc_fence_after();
-      uint32_t s[BN / 32][32];
-#pragma unroll
-      for (int c = 0; c < BN / 32; c++) tmem_ld32_nw(ts + c * 32, s[c]);
-      tc_wait_ld();
-#pragma unroll
-      for (int c = 0; c < BN / 32; c++) loaded(s[c]);
-      auto at = [&](int j) -> float { return __uint_as_float(s[j >> 5][j & 31]); };
-      auto set = [&](int j, float x) { s[j >> 5][j & 31] = __float_as_uint(x); };
-
-      if (!PLAIN) {
-        if (A.cap > 0.0f) {
-#pragma unroll
-          for (int c = 0; c < BN / 32; c++) capped(reinterpret_cast<float (&)[32]>(s[c]), to_cap, raw_cap);
-        }
-#pragma unroll
-        for (int a = 0; a < S2S_MAX_AXES; a++)
-          if (a < A.axes) {
-            const F2 q2 = f2_both(-qf[a]);
-#pragma unroll
-            for (int j = 0; j < BN; j += 4) {
-              const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(kp + a * BN + j);
-              const float2 x = f2_unpack(f2_add(k.x, q2)), y = f2_unpack(f2_add(k.y, q2));
-              set(j, at(j) - fabsf(x.x));
-              set(j + 1, at(j + 1) - fabsf(x.y));
-              set(j + 2, at(j + 2) - fabsf(y.x));
-              set(j + 3, at(j + 3) - fabsf(y.y));
-            }
-          }
-      }
-      if ((t + 1) * BN > open) {
-        const int last = mine - t * BN;
-#pragma unroll
-        for (int j = 0; j < BN; j++)
-          if (j >= last) set(j, -INFINITY);
-      }
-      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int j = 0; j < BN; j += 2) top[(j >> 1) & 3] = max3(top[(j >> 1) & 3], at(j), at(j + 1));
-      const float high = fmaxf(max3(top[0], top[1], top[2]), top[3]) * unit;
-      if (t == 0) {
-        m = high;
-      } else if (__any_sync(0xffffffffu, high > m + 8.0f)) {
-        const float next = fmaxf(m, high), keep = next == -INFINITY ? 1.0f : ex2(m - next);
-        m = next;
-        l *= keep;
-        // the output product before this tile's is complete, this one waits for the weights
-        output_done(t - 1);
-        for (int c = 0; c < ksteps * 16; c += 16) {
-          uint32_t o[16];
-          tmem_ld16(to + c, o);
-#pragma unroll
-          for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-          tmem_st16(to + c, o);
-        }
-      }
-      const F2 base2 = f2_both(m == -INFINITY ? 0.0f : -m), unit2 = f2_both(unit);
-      F2 sum[2] = {0, 0};  // two zeros each
-#pragma unroll
-      for (int c = 0; c < BN / 64; c++) {
-        uint32_t p[32];
-#pragma unroll
-        for (int j = 0; j < 32; j++) {
-          F2 x = f2_fma(f2_pack(at(64 * c + 2 * j), at(64 * c + 2 * j + 1)), unit2, base2);
-          if (j % 4 == 3) {
-            x = ex2_poly(x);
-          } else {
-            const float2 xs = f2_unpack(x);
-            x = f2_pack(ex2(xs.x), ex2(xs.y));
-          }
-          sum[j & 1] = f2_add(sum[j & 1], x);
-          const float2 y = f2_unpack(x);
-          p[j] = pack2<T>(y.x, y.y);
-        }
-        tmem_st32(ts + c * 32, p);
-      }
-      const float2 total = f2_unpack(f2_add(sum[0], sum[1]));
-      l += total.x + total.y;
+    };
+    auto weights_done = [&](int b) {
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[b]);
+    };
+
+    if constexpr (MODE < 2) {
+      // a row a thread
+      for (int t = 0; t < n_w; t++) {
+        const Place at(w, t, n[0], n[1]);
+        const uint32_t ts = lanes + at.buffer * BN;
+        if (ok) ok = mbar_wait(&s_full[at.buffer], at.parity, DEV_TIMEOUT_ACC);
+        __syncwarp();
+        tc_fence_after();
+        uint32_t raw[BN / 32][32];
+#pragma unroll
+        for (int c = 0; c < BN / 32; c++) tmem_ld32_nw(ts + c * 32, raw[c]);
+        tc_wait_ld();
+#pragma unroll
+        for (int c = 0; c < BN / 32; c++) loaded(raw[c]);
+        float(&s)[BN] = reinterpret_cast<float(&)[BN]>(raw);
+        if constexpr (MODE == 1) capped(s, to_cap, raw_cap);
+        if ((t + 1) * BN > open) {
+          const int last = mine - t * BN;
+#pragma unroll
+          for (int j = 0; j < BN; j++)
+            if (j >= last) s[j] = -INFINITY;
+        }
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < BN; j += 2) top[(j >> 1) & 3] = max3(top[(j >> 1) & 3], s[j], s[j + 1]);
+        const float high = fmaxf(max3(top[0], top[1], top[2]), top[3]) * unit;
+        if (t == 0) {
+          m = high;
+        } else if (__any_sync(0xffffffffu, high > m + 8.0f)) {
+          const float next = fmaxf(m, high), keep = next == -INFINITY ? 1.0f : ex2(m - next);
+          m = next;
+          l *= keep;
+          scale_outputs(t, keep);
+        }
+        const F2 base2 = f2_both(m == -INFINITY ? 0.0f : -m);
+        F2 sum[2] = {0, 0};  // two zeros each
+#pragma unroll
+        for (int c = 0; c < BN / 64; c++) {
+          uint32_t p[32];
+#pragma unroll
+          for (int j = 0; j < 32; j++) {
+            const float2 x = f2_unpack(f2_fma(f2_pack(s[64 * c + 2 * j], s[64 * c + 2 * j + 1]), unit2, base2));
+            const float2 y = make_float2(ex2(x.x), ex2(x.y));
+            sum[j & 1] = f2_add(sum[j & 1], f2_pack(y.x, y.y));
+            p[j] = pack2<T>(y.x, y.y);
+          }
+          tmem_st32_nw(ts + c * 32, p);
+        }
+        const float2 total = f2_unpack(f2_add(sum[0], sum[1]));
+        l += total.x + total.y;
+        weights_done(at.buffer);
+      }
+    } else {
+      // Four rows a thread, g + 8 R, and of each eight keys the two of the lane's place in its quad:
+      // a key's positions then serve four scores. (With a row a thread every thread read all the
+      // tile's positions, and shared memory was what bound it.)
+      const int g = lane >> 2, t4 = lane & 3;
+      float rm[4], rl[4], qf[4][S2S_MAX_AXES], slope[S2S_MAX_AXES];
+      int rseen[4], ref[S2S_MAX_AXES], kraw[S2S_MAX_AXES];
+      float* pos = spos + w * 2 * S2S_MAX_AXES * BN;
+      // the positions of a tile's keys, times the slope, each loaded a tile ahead by one thread
+      auto key_positions = [&](int t) {
+        const int j = t * BN + r;
+        if (r < BN)
+#pragma unroll
+          for (int a = 0; a < S2S_MAX_AXES; a++)
+            if (a < A.axes) kraw[a] = j < D.nk ? A.kpos[(int64_t)a * A.kv_tokens + D.k0 + j] : ref[a];
+      };
+#pragma unroll
+      for (int R = 0; R < 4; R++) {
+        const int x = (warp & 3) * 32 + g + 8 * R;
+        rm[R] = -INFINITY;
+        rl[R] = 0.0f;
+        rseen[R] = x < rows_w ? seen(A, D, first + x) : 0;
+      }
+      if (n_w > 0) {
+#pragma unroll
+        for (int a = 0; a < S2S_MAX_AXES; a++)
+          if (a < A.axes) {
+            const int* qa = A.qpos + (int64_t)a * A.q_tokens + D.q0;
+            ref[a] = qa[i0];
+            slope[a] = fabsf(A.slopes[a * A.q_heads + h]) / A.scale;
+#pragma unroll
+            for (int R = 0; R < 4; R++) {
+              const int x = (warp & 3) * 32 + g + 8 * R;
+              qf[R][a] = -slope[a] * (float)(int)((unsigned)qa[x < rows_w ? first + x : i0] - (unsigned)ref[a]);
+            }
+          }
+        key_positions(0);
+      }
+      for (int t = 0; t < n_w; t++) {
+        const Place at(w, t, n[0], n[1]);
+        const uint32_t ts = lanes + at.buffer * BN;
+        float* kp = pos + (t & 1) * S2S_MAX_AXES * BN;
+        if (r < BN)
+#pragma unroll
+          for (int a = 0; a < S2S_MAX_AXES; a++)
+            if (a < A.axes) kp[a * BN + r] = slope[a] * (float)(int)((unsigned)kraw[a] - (unsigned)ref[a]);
+        group_sync(1 + w);
+        if (t + 1 < n_w) key_positions(t + 1);
+        if (ok) ok = mbar_wait(&s_full[at.buffer], at.parity, DEV_TIMEOUT_ACC);
+        __syncwarp();
+        tc_fence_after();
+        // [half][64 keys]: value 4 k + e is key 8 k + 2 t4 + (e & 1) of row R = 2 half + (e >> 1)
+        uint32_t raw[2][BN / 64][32];
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+          for (int c = 0; c < BN / 64; c++) tmem_ld_frag(ts + ((uint32_t)x << 20) + c * 64, raw[x][c]);
+        tc_wait_ld();
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+          for (int c = 0; c < BN / 64; c++) loaded(raw[x][c]);
+        float(&s)[2][BN / 64][32] = reinterpret_cast<float(&)[2][BN / 64][32]>(raw);
+        if (A.cap > 0.0f) capped(reinterpret_cast<float(&)[BN]>(raw), to_cap, raw_cap);
+#pragma unroll
+        for (int a = 0; a < S2S_MAX_AXES; a++)
+          if (a < A.axes) {
+#pragma unroll
+            for (int c = 0; c < BN / 64; c++)
+#pragma unroll
+              for (int k = 0; k < 8; k++) {
+                const F2 k2 = *reinterpret_cast<const F2*>(kp + a * BN + 64 * c + 8 * k + 2 * t4);
+#pragma unroll
+                for (int R = 0; R < 4; R++) {
+                  const float2 d = f2_unpack(f2_add(k2, f2_both(qf[R][a])));
+                  s[R >> 1][c][4 * k + 2 * (R & 1)] -= fabsf(d.x);
+                  s[R >> 1][c][4 * k + 2 * (R & 1) + 1] -= fabsf(d.y);
+                }
+              }
+          }
+        if ((t + 1) * BN > open) {
+          const int j0 = t * BN + 2 * t4;
+#pragma unroll
+          for (int c = 0; c < BN / 64; c++)
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+#pragma unroll
+              for (int R = 0; R < 4; R++)
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                  if (j0 + 64 * c + 8 * k + e >= rseen[R]) s[R >> 1][c][4 * k + 2 * (R & 1) + e] = -INFINITY;
+        }
+        float high[4];
+        bool more = false;
+#pragma unroll
+        for (int R = 0; R < 4; R++) {
+          float x = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < BN / 64; c++)
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+              x = max3(x, s[R >> 1][c][4 * k + 2 * (R & 1)], s[R >> 1][c][4 * k + 2 * (R & 1) + 1]);
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+          high[R] = x * unit;
+          if (t == 0) rm[R] = high[R];
+          more = more || high[R] > rm[R] + 8.0f;
+        }
+        if (t > 0 && __any_sync(0xffffffffu, more)) {
+          float keep[4], mine4 = 1.0f;
+#pragma unroll
+          for (int R = 0; R < 4; R++) {
+            const float next = fmaxf(rm[R], high[R]);
+            keep[R] = next == -INFINITY ? 1.0f : ex2(rm[R] - next);
+            rm[R] = next;
+            rl[R] *= keep[R];
+            const float x = __shfl_sync(0xffffffffu, keep[R], (lane & 7) * 4);
+            if (lane >> 3 == R) mine4 = x;
+          }
+          scale_outputs(t, mine4);
+        }
+        F2 base2[4], sum[4];
+#pragma unroll
+        for (int R = 0; R < 4; R++) {
+          base2[R] = f2_both(rm[R] == -INFINITY ? 0.0f : -rm[R]);
+          sum[R] = 0;  // two zeros
+        }
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+          for (int c = 0; c < BN / 64; c++) {
+            uint32_t p[16];
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+              const int R = 2 * x + (k & 1);
+              const float2 z = f2_unpack(f2_fma(f2_pack(s[x][c][2 * k], s[x][c][2 * k + 1]), unit2, base2[R]));
+              const float2 y = make_float2(ex2(z.x), ex2(z.y));
+              sum[R] = f2_add(sum[R], f2_pack(y.x, y.y));
+              p[k] = pack2<T>(y.x, y.y);
+            }
+            tmem_st_frag(ts + ((uint32_t)x << 20) + c * 32, p);
+          }
+#pragma unroll
+        for (int R = 0; R < 4; R++) {
+          const float2 total = f2_unpack(sum[R]);
+          rl[R] += total.x + total.y;
+        }
+        weights_done(at.buffer);
+      }
+      // to the row of the lane
+#pragma unroll
+      for (int R = 0; R < 4; R++) {
+        rl[R] += __shfl_xor_sync(0xffffffffu, rl[R], 1);
+        rl[R] += __shfl_xor_sync(0xffffffffu, rl[R], 2);
+        const float x = __shfl_sync(0xffffffffu, rm[R], (lane & 7) * 4);
+        const float y = __shfl_sync(0xffffffffu, rl[R], (lane & 7) * 4);
+        if (lane >> 3 == R) {
+          m = x;
+          l = y;
+        }
+      }
     }
 
     // ------------------------------------------------------------------- output
@@ -560,11 +701,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
-template <typename T, int NP, bool PLAIN>
+template <typename T, int NP, int MODE>
 cudaError_t launch_attention_tc(AttnArgs& A, cudaStream_t st) {
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   using C = TcCfg<NP>;
-  auto kernel = k_attention_tc<T, NP, PLAIN>;
+  auto kernel = k_attention_tc<T, NP, MODE>;
   static LaunchSetup setup;
   int ctas = 0;
   const cudaError_t err = resident_ctas(setup, kernel, kTcThreads, C::SMEM, &ctas);
@@ -582,10 +723,13 @@ cudaError_t launch_attention_tc(AttnArgs& A, cudaStream_t st) {
 
 template <typename T>
 cudaError_t launch_attention_tc(AttnArgs& A, cudaStream_t st) {
-  const bool plain = A.cap == 0.0f && A.axes == 0;
   if (A.head_dim <= 64)
-    return plain ? launch_attention_tc<T, 1, true>(A, st) : launch_attention_tc<T, 1, false>(A, st);
-  return plain ? launch_attention_tc<T, 2, true>(A, st) : launch_attention_tc<T, 2, false>(A, st);
+    return A.axes         ? launch_attention_tc<T, 1, 2>(A, st)
+           : A.cap > 0.0f ? launch_attention_tc<T, 1, 1>(A, st)
+                          : launch_attention_tc<T, 1, 0>(A, st);
+  return A.axes         ? launch_attention_tc<T, 2, 2>(A, st)
+         : A.cap > 0.0f ? launch_attention_tc<T, 2, 1>(A, st)
+                        : launch_attention_tc<T, 2, 0>(A, st);
 }
 
 }  // namespace
