@@ -37,7 +37,7 @@ struct TcCfg {
   static constexpr int VRING = KRING + STAGES * KB;
   static constexpr int POS = VRING + STAGES * KB;
   static constexpr int BARS = POS + 2 * 2 * S2S_MAX_AXES * BN * 4;
-  static constexpr int NBARS = 4 * STAGES + 3 * NB + 5;
+  static constexpr int NBARS = 4 * STAGES + 3 * NB + 13;
   static constexpr int SMEM = BARS + NBARS * 8 + 16 + 1024;  // + alignment
 };
 
@@ -209,7 +209,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint64_t* o_done = p_full + NB;   // the output product that read the buffer's weights is complete
   uint64_t* q_full = o_done + NB;   // [tile]
   uint64_t* fin = q_full + 2;       // [issuing warp]: every product has retired
-  uint32_t* holder = reinterpret_cast<uint32_t*>(fin + 3);
+  uint64_t* turn = fin + 3;         // [softmax warp]: its exponentials of a tile are done
+  uint32_t* holder = reinterpret_cast<uint32_t*>(turn + 8);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
@@ -226,6 +227,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     for (int w = 0; w < 2; w++) mbar_init(&q_full[w], 1);
     for (int k = 0; k < 3; k++) mbar_init(&fin[k], 1);
+    for (int k = 0; k < 8; k++) mbar_init(&turn[k], 1);
     fence_barrier_init();
     tma_prefetch_desc(&mapQ);
     tma_prefetch_desc(&mapK);
@@ -259,6 +261,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     n[w] = (kend[w] + BN - 1) / BN;
   }
   const int kmax = max(kend[0], kend[1]);
+  // Key tiles from the first on. With a bias they begin where the queries are, near their nearest
+  // keys, and wrap around: scores that grew from tile to tile on the way there would have the
+  // outputs scaled again for each. Both row tiles then take all of them.
+  int start = 0;
+  if (MODE == 2) {
+    n[0] = rows[0] > 0 ? max(n[0], n[1]) : 0;
+    n[1] = rows[1] > 0 ? n[0] : 0;
+    start = max(0, min((i0 + D.nk - D.nq) / BN, n[0] - 1));
+  }
+  auto key_tile = [&](int step) { return start + step < n[0] || MODE < 2 ? start + step : start + step - n[0]; };
   const int ksteps = (A.head_dim + 15) / 16;
 
   // registers: 384 threads begin with 168 each; the softmax groups take what the third gives
@@ -279,12 +291,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int s = i % ST;
         if (i >= ST) ok = mbar_wait(&k_empty[s], ((i / ST) - 1) & 1, DEV_TIMEOUT_EMPTY);
         if (!ok) break;
-        load(kring + s * C::KB, C::KB, &mapK, &k_full[s], hk, D.k0 + i * BN);
+        load(kring + s * C::KB, C::KB, &mapK, &k_full[s], hk, D.k0 + key_tile(i) * BN);
         if (i == 0)
           for (int w = 0; w < 2; w++)
             if (n[w] > 0) load(sQ + w * C::QB, C::QB, &mapQ, &q_full[w], h, D.q0 + i0 + w * kTcTile);
         if (i >= ST) ok = mbar_wait(&v_empty[s], ((i / ST) - 1) & 1, DEV_TIMEOUT_EMPTY);
-        if (ok) load(vring + s * C::KB, C::KB, &mapV, &v_full[s], hk, D.k0 + i * BN);
+        if (ok) load(vring + s * C::KB, C::KB, &mapV, &v_full[s], hk, D.k0 + key_tile(i) * BN);
       }
       // no copy is in flight when the CTA ends, also where a wait gave up
       if (N > 0)
@@ -301,6 +313,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int keys = (int)__reduce_max_sync(0xffffffffu, (unsigned)kmax);
     const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
     const int last = max(n0, n1) - 1;
+    const int cut = MODE == 2 ? (int)__reduce_max_sync(0xffffffffu, (unsigned)(last - start)) : last;  // step of the last keys
     // after a wait that gave up the products go on without waiting, over whatever is there
     bool ok = true;
     auto wait = [&](uint64_t* bar, int phase, unsigned code) {
@@ -362,7 +375,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int i = 0, st = 0, ph = 0; i <= last; i++) {
         const int tail = keys - last * BN, steps = (tail + 15) / 16;
         wait(&v_full[st], ph, DEV_TIMEOUT_FULL);
-        if (i == last && tail % 16) {
+        if (i == cut && tail % 16) {
           // Keys that no row sees, and rows of other documents behind them, have zero weights:
           // what lies there must not reach the product, which takes keys by 16.
           for (int x = 0; x < NP; x++)
@@ -381,7 +394,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const uint32_t d = tm + C::OUT + w * 64 * NP, p = tm + at.buffer * BN;
             if (one) {
               mma_ts(d, p, v, id, i != 0);
-              if (i < last) {
+              if (i != cut) {
 #pragma unroll
                 for (int c = 1; c < BN / 16; c++) mma_ts(d, p + c * 8, v + c * (2048 >> 4), id);
               } else {
@@ -437,6 +450,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
         tmem_st16(to + c, o);
       }
+    };
+    // With a bias the two softmax warps of a scheduler (warp and warp ^ 4) take turns at the
+    // exponentials, so that one's keep the special function unit busy while the other is at its
+    // bias (12 heads, images of 3136 + 4096 + ...: 338 -> 308 us; without a bias turns cost more than
+    // they give, 193 -> 238 us at 37 heads of 64 x 4096^2).
+    auto my_turn = [&](int t) {
+      const int u = w ? t : t - 1;  // tile 0 first
+      if (ok && u >= 0 && u < (w ? n[0] : n[1])) ok = mbar_wait(&turn[warp ^ 4], u & 1, DEV_TIMEOUT_ACC);
+      __syncwarp();
+    };
+    auto turn_over = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&turn[warp]);
     };
     auto weights_done = [&](int b) {
       tc_wait_st();
@@ -507,7 +533,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       float* pos = spos + w * 2 * S2S_MAX_AXES * BN;
       // the positions of a tile's keys, times the slope, each loaded a tile ahead by one thread
       auto key_positions = [&](int t) {
-        const int j = t * BN + r;
+        const int j = key_tile(t) * BN + r;
         if (r < BN)
 #pragma unroll
           for (int a = 0; a < S2S_MAX_AXES; a++)
@@ -577,8 +603,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
               }
           }
-        if ((t + 1) * BN > open) {
-          const int j0 = t * BN + 2 * t4;
+        if ((key_tile(t) + 1) * BN > open) {
+          const int j0 = key_tile(t) * BN + 2 * t4;
 #pragma unroll
           for (int c = 0; c < BN / 64; c++)
 #pragma unroll
@@ -624,6 +650,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           base2[R] = f2_both(rm[R] == -INFINITY ? 0.0f : -rm[R]);
           sum[R] = 0;  // two zeros
         }
+        my_turn(t);
 #pragma unroll
         for (int x = 0; x < 2; x++)
 #pragma unroll
@@ -644,6 +671,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const float2 total = f2_unpack(sum[R]);
           rl[R] += total.x + total.y;
         }
+        turn_over();
         weights_done(at.buffer);
       }
       // to the row of the lane
