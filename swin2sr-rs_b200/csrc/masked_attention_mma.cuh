@@ -46,6 +46,23 @@ __device__ __forceinline__ void mma_tile<__nv_bfloat16>(float (&c)[4], const uin
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The same onto zeros.
+template <typename T>
+__device__ __forceinline__ void mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
 // ------------------------------------------------------------------------- clusters
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -293,37 +310,12 @@ __global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS>::CTAS)
   const int ntiles = (kend + C::TKEYS - 1) / C::TKEYS;
   const int tb = (int)((long long)ntiles * split / S), te = (int)((long long)ntiles * (split + 1) / S);
 
-  // this thread's two rows
-  int row_seen[2], row_q[2], row_h[2];
-  bool live[2];
-#pragma unroll
-  for (int e = 0; e < 2; e++) {
-    const int r = r0 + rw * 16 + g + 8 * e;
-    live[e] = r - r0 < nrows;
-    const int i = live[e] ? r / A.group : i_first;
-    row_q[e] = D.q0 + i;
-    row_h[e] = live[e] ? r - i * A.group : 0;  // within the key head
-    row_seen[e] = live[e] ? seen(A, D, i) : 0;
-  }
-
-  // bias: positions count from the tile's first query, so that near ones are exact
-  float qpos[2][S2S_MAX_AXES];
-  int ref[S2S_MAX_AXES];
-  if (A.axes) {
-#pragma unroll
-    for (int a = 0; a < S2S_MAX_AXES; a++)
-      if (a < A.axes) {
-        const int* qa = A.qpos + (int64_t)a * A.q_tokens;
-        ref[a] = qa[D.q0 + i_first];
-#pragma unroll
-        for (int e = 0; e < 2; e++) qpos[e][a] = (float)(int)((unsigned)qa[row_q[e]] - (unsigned)ref[a]);
-      }
-  }
-
-  // K and V tiles of head after head into the ring; the key positions of a tile, as fp32,
-  // through registers a tile later
+  // K and V tiles of head after head into the ring; the key positions of a tile, as fp32, through
+  // registers and into place a tile later. Where all tiles of a head have a place of their own the
+  // positions come once for all heads.
   int ft = tb, fh = hk0;  // the next tile to fetch
-  int kraw[2];
+  int kraw[2], ref[S2S_MAX_AXES];
+  const bool stay = te - tb <= kMmaStages;
   auto fetch = [&]() {
     if (fh >= hk1 || tb >= te) return;
     if (tid == 0) {
@@ -335,7 +327,7 @@ __global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS>::CTAS)
         tma_load_3d(dst + C::TILE + p * C::PANEL, &mapV, &full[fstage], p * C::PV, fh, D.k0 + ft * C::TKEYS);
       }
     }
-    if (A.axes)
+    if (A.axes && (!stay || fh == hk0))
 #pragma unroll
       for (int x = 0; x < 2; x++) {
         const int u = tid + x * C::THREADS, a = u / C::TKEYS, j = ft * C::TKEYS + u % C::TKEYS;
@@ -344,8 +336,8 @@ __global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS>::CTAS)
   };
   auto fetched = [&]() {  // the positions of the tile last fetched
     if (fh >= hk1 || tb >= te) return;
-    if (A.axes) {
-      float* kp = spos + fstage * (S2S_MAX_AXES * C::TKEYS);
+    if (A.axes && (!stay || fh == hk0)) {
+      float* kp = spos + (stay ? ft - tb : fstage) * (S2S_MAX_AXES * C::TKEYS);
 #pragma unroll
       for (int x = 0; x < 2; x++) {
         const int u = tid + x * C::THREADS, a = u / C::TKEYS;
@@ -361,6 +353,34 @@ __global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS>::CTAS)
       fh++;
     }
   };
+  fetch();
+
+  // this thread's two rows
+  int row_seen[2], row_q[2], row_h[2];
+  bool live[2];
+#pragma unroll
+  for (int e = 0; e < 2; e++) {
+    const int r = r0 + rw * 16 + g + 8 * e;
+    live[e] = r - r0 < nrows;
+    const int i = live[e] ? r / A.group : i_first;
+    row_q[e] = D.q0 + i;
+    row_h[e] = live[e] ? r - i * A.group : 0;  // within the key head
+    row_seen[e] = live[e] ? seen(A, D, i) : 0;
+  }
+
+  // bias: positions count from the tile's first query, so that near ones are exact
+  float qpos[2][S2S_MAX_AXES];
+  if (A.axes) {
+#pragma unroll
+    for (int a = 0; a < S2S_MAX_AXES; a++)
+      if (a < A.axes) {
+        const int* qa = A.qpos + (int64_t)a * A.q_tokens;
+        ref[a] = qa[D.q0 + i_first];
+#pragma unroll
+        for (int e = 0; e < 2; e++) qpos[e][a] = (float)(int)((unsigned)qa[row_q[e]] - (unsigned)ref[a]);
+      }
+  }
+
   // Q fragments of a head straight from global memory
   uint32_t qf[DK][4], qnext[DK][4];
   auto load_q = [&](int hk) {
@@ -377,28 +397,36 @@ __global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS>::CTAS)
         }
     }
   };
-  __syncthreads();  // the barriers are set up, the ring is free
-  load_q(hk0);
+  const float per_scale = 1.0f / A.scale;
+  float slope[2][S2S_MAX_AXES], snext[2][S2S_MAX_AXES];
+  auto load_slopes = [&](int hk) {
 #pragma unroll
-  for (int s = 0; s < kMmaStages - 1; s++) {
-    fetch();
-    fetched();
-  }
+    for (int a = 0; a < S2S_MAX_AXES; a++)
+      if (a < A.axes)
+#pragma unroll
+        for (int e = 0; e < 2; e++) snext[e][a] = A.slopes[a * A.q_heads + hk * A.group + row_h[e]];
+  };
+  load_q(hk0);
+  load_slopes(hk0);
+  fetched();
+  fetch();
+  __syncthreads();  // the barriers are set up
 
   for (int hk = hk0; hk < hk1; hk++) {
 #pragma unroll
     for (int kk = 0; kk < DK; kk++)
 #pragma unroll
       for (int e = 0; e < 4; e++) qf[kk][e] = qnext[kk][e];
-    if constexpr (KW == 1)
-      if (hk + 1 < hk1) load_q(hk + 1);
-    float slope[2][S2S_MAX_AXES];
 #pragma unroll
     for (int a = 0; a < S2S_MAX_AXES; a++)
       if (a < A.axes)
 #pragma unroll
-        for (int e = 0; e < 2; e++)
-          slope[e][a] = fabsf(A.slopes[a * A.q_heads + hk * A.group + row_h[e]]) / A.scale;
+        for (int e = 0; e < 2; e++) slope[e][a] = fabsf(snext[e][a]) * per_scale;
+    if constexpr (KW == 1)
+      if (hk + 1 < hk1) {
+        load_q(hk + 1);
+        load_slopes(hk + 1);
+      }
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
     float o[DN][4];
 #pragma unroll
@@ -418,25 +446,29 @@ __global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS>::CTAS)
         fence_proxy_async_smem();
       }
       __syncthreads();  // everyone has left the stage that is filled now
+      fetched();
       fetch();
       const uint32_t ks = smem_u32(smem + stage * 2 * C::TILE), vs = ks + C::TILE;
       const int j0 = t * C::TKEYS + kw * C::KEYS;
       if (KW == 1 || j0 < kend) {  // some key of this warp is seen
         float s[NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-#pragma unroll
         for (int kk = 0; kk < DK; kk++)
 #pragma unroll
           for (int n = 0; n < NT; n += 2) {
             uint32_t b0, b1, b2, b3;
             ldsm_x4(ks + (kk / PK) * C::PANEL + n * 8 * C::PV * 2 + (kat ^ (kk % PK * 32)), b0, b1, b2, b3);
-            mma_tile<T>(s[n], qf[kk], b0, b1);
-            mma_tile<T>(s[n + 1], qf[kk], b2, b3);
+            if (kk == 0) {
+              mma_first<T>(s[n], qf[kk], b0, b1);
+              mma_first<T>(s[n + 1], qf[kk], b2, b3);
+            } else {
+              mma_tile<T>(s[n], qf[kk], b0, b1);
+              mma_tile<T>(s[n + 1], qf[kk], b2, b3);
+            }
           }
         if (A.cap > 0.0f) capped(reinterpret_cast<float (&)[NT * 4]>(s), to_cap, raw_cap);
         if (A.axes) {
-          const float* kp = spos + stage * (S2S_MAX_AXES * C::TKEYS) + kw * C::KEYS + 2 * t4;
+          const float* kp = spos + (stay ? t - tb : stage) * (S2S_MAX_AXES * C::TKEYS) + kw * C::KEYS + 2 * t4;
 #pragma unroll
           for (int a = 0; a < S2S_MAX_AXES; a++)
             if (a < A.axes) {
@@ -516,7 +548,6 @@ __global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS>::CTAS)
           }
         }
       }
-      fetched();
       if (++stage == kMmaStages) {
         stage = 0;
         phase ^= 1;
