@@ -93,7 +93,7 @@ __device__ __forceinline__ float4 cluster_load4(uint32_t addr, uint32_t rank) {
   return v;
 }
 
-template <int DP, int RW, int WARPS>
+template <int DP, int RW, int WARPS, int NA = S2S_MAX_AXES>
 struct MmaCfg {
   static constexpr int THREADS = 32 * WARPS;
   static constexpr int TKEYS = 16 * WARPS;       // keys of a tile
@@ -111,8 +111,13 @@ struct MmaCfg {
   static constexpr int BARS = BODY + kMmaStages * POS;
   static constexpr int ENDS = BARS + kMmaStages * 8 + 8;   // maxima and sums, flags
   static constexpr int SMEM = ENDS + WARPS * 16 * 8 + ROWS * 12 + 1024;  // + alignment
-  // resident CTAs that the registers are cut to: the more, the more loads are in flight
-  static constexpr int CTAS = (DP == 32 ? 4 : DP == 64 ? 3 : 2) * 4 / WARPS;
+  // Resident CTAs that the registers are cut to: the more, the more loads are in flight, but what
+  // spills costs more (1271 windows of 64, six heads of 32, two axes: 3 CTAs 55 us, 4 67 us; 32
+  // single queries over 3000 keys, eight heads of 64: 4 CTAs 44 us, 3 49 us).
+  static constexpr int CTAS = (RW < 4   ? (DP == 128 ? 2 : 4)
+                               : DP == 32 ? 3
+                               : DP == 64 ? (NA ? 2 : 3)
+                                          : 2) * 4 / WARPS;
 };
 
 // Where lane `lane` finds, in a tile, chunk `b` (16 bytes) of row `r`; chunk b + 2k of the same
@@ -123,39 +128,62 @@ __device__ __forceinline__ uint32_t tile_at(int r, int b) {
                   : (uint32_t)(r * 128 + ((b ^ (r & 7)) << 4));
 }
 
-// Outputs of a head from the warps that have their rows to themselves.
+// Outputs of a head from the warps that have their rows to themselves; `op`: this lane's place in
+// its two rows. Whether one of them is NaN or infinite (in causal order, where it matters).
 template <typename T, int DN>
-__device__ __forceinline__ void write_rows(const AttnArgs& A, const Doc& D, int hk, const float (&o)[DN][4],
-                                           const float (&m)[2], const float (&l)[2], const int (&row_q)[2],
-                                           const int (&row_h)[2], const int (&row_seen)[2],
-                                           const bool (&live)[2], int kend, int lane) {
-  const int t4 = lane & 3;
+__device__ __forceinline__ bool write_rows(const AttnArgs& A, int hk, const float (&o)[DN][4],
+                                           const float (&m)[2], const float (&l)[2], T* const (&op)[2],
+                                           const int (&row_q)[2], const int (&row_h)[2],
+                                           const bool (&live)[2], int lane) {
+  float check = 0.0f;
 #pragma unroll
   for (int e = 0; e < 2; e++) {
     const bool none = m[e] == -INFINITY;
-    const float inv = none ? 0.0f : 1.0f / l[e];
-    const int h = hk * A.group + row_h[e];
-    float check = 0.0f;  // NaN where an output is NaN or infinite
-    T* op = static_cast<T*>(A.out.data) + (int64_t)row_q[e] * A.out.token + (int64_t)h * A.out.head + 2 * t4;
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(l[e]));
+    if (none) inv = 0.0f;
+    if (live[e]) {
 #pragma unroll
-    for (int n = 0; n < DN; n++) {
-      const float x = o[n][2 * e] * inv, y = o[n][2 * e + 1] * inv;
-      check = fmaf(x, 0.0f, fmaf(y, 0.0f, check));
-      if (live[e] && n * 8 < A.head_dim) *reinterpret_cast<uint32_t*>(op + n * 8) = pack2<T>(x, y);
+      for (int n = 0; n < DN; n++)
+        if (n * 8 < A.head_dim)
+          *reinterpret_cast<uint32_t*>(op[e] + n * 8) = pack2<T>(o[n][2 * e] * inv, o[n][2 * e + 1] * inv);
+      if ((lane & 3) == 0 && A.lse)
+        A.lse[(int64_t)(hk * A.group + row_h[e]) * A.q_tokens + row_q[e]] =
+            none ? -INFINITY : (m[e] + log2f(l[e])) * kLn2;
     }
-    if (live[e] && t4 == 0 && A.lse)
-      A.lse[(int64_t)h * A.q_tokens + row_q[e]] = none ? -INFINITY : (m[e] + log2f(l[e])) * kLn2;
-    // keys that the row does not see were multiplied by zero weights: a NaN or infinity among
-    // their values shows here, and the row is done again without them
-    unsigned redo = __ballot_sync(0xffffffffu, check != 0.0f && live[e] && row_seen[e] < kend);
-    __syncwarp();
-    while (redo) {
-      const int src = __ffs(redo) - 1;
-      redo &= ~(15u << (src & ~3));
-      const int i = __shfl_sync(0xffffffffu, row_q[e], src) - D.q0;
-      attend_row<T>(A, D, i, __shfl_sync(0xffffffffu, h, src), lane);
-    }
+    if (A.causal)
+#pragma unroll
+      for (int n = 0; n < DN; n++) check = fmaf(o[n][2 * e] * inv, 0.0f, fmaf(o[n][2 * e + 1] * inv, 0.0f, check));
   }
+  return check != 0.0f;  // true for NaN
+}
+
+// Keys that a row does not see are multiplied by zero weights: a NaN or infinity among their values
+// shows in the row's outputs. Such rows of this warp are done again without those keys; `op` as it
+// was for the first head. Behind the heads' loop, as a call in it costs registers there.
+template <typename T, int DN>
+__device__ __forceinline__ void mend_rows(const AttnArgs& A, const Doc& D, int hk0, int hk1, T* (&op)[2],
+                                          const int (&row_q)[2], const int (&row_h)[2],
+                                          const int (&row_seen)[2], const bool (&live)[2], int kend, int lane) {
+  for (int hk = hk0; hk < hk1; hk++)
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      float check = 0.0f;
+      if (live[e] && row_seen[e] < kend)
+        for (int n = 0; n * 8 < A.head_dim; n++) {
+          const uint32_t u = *reinterpret_cast<const uint32_t*>(op[e] + n * 8);
+          const T* x = reinterpret_cast<const T*>(&u);
+          check = fmaf(to_f32(x[0]), 0.0f, fmaf(to_f32(x[1]), 0.0f, check));
+        }
+      op[e] += (int64_t)A.group * A.out.head;
+      unsigned redo = __ballot_sync(0xffffffffu, check != 0.0f);
+      while (redo) {
+        const int src = __ffs(redo) - 1;
+        redo &= ~(15u << (src & ~3));
+        const int i = __shfl_sync(0xffffffffu, row_q[e], src) - D.q0;
+        attend_row<T>(A, D, i, hk * A.group + __shfl_sync(0xffffffffu, row_h[e], src), lane);
+      }
+    }
 }
 
 // Outputs of a head whose keys lie with several warps, and CTAs of a cluster: everything they
@@ -260,8 +288,10 @@ __device__ __forceinline__ void join_rows(const AttnArgs& A, const Doc& D, int h
   if (S > 1) cluster_sync();  // nobody leaves while its shared memory is read
 }
 
-template <typename T, int DP, int RW, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS>::CTAS)
+// NA: the most axes of a bias, CAP: whether there can be a cap. Where one warp has all keys of a tile
+// the registers for both are what limits the CTAs on an SM.
+template <typename T, int DP, int RW, int WARPS, int NA, bool CAP>
+__global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS, NA>::CTAS)
     k_attention_mma(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap mapK,
                     const __grid_constant__ CUtensorMap mapV) {
   using C = MmaCfg<DP, RW, WARPS>;
@@ -314,7 +344,7 @@ __global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS>::CTAS)
   // registers and into place a tile later. Where all tiles of a head have a place of their own the
   // positions come once for all heads.
   int ft = tb, fh = hk0;  // the next tile to fetch
-  int kraw[2], ref[S2S_MAX_AXES];
+  int kraw[2], ref[NA > 0 ? NA : 1];
   const bool stay = te - tb <= kMmaStages;
   auto fetch = [&]() {
     if (fh >= hk1 || tb >= te) return;
@@ -327,7 +357,7 @@ __global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS>::CTAS)
         tma_load_3d(dst + C::TILE + p * C::PANEL, &mapV, &full[fstage], p * C::PV, fh, D.k0 + ft * C::TKEYS);
       }
     }
-    if (A.axes && (!stay || fh == hk0))
+    if (NA > 0 && A.axes && (!stay || fh == hk0))
 #pragma unroll
       for (int x = 0; x < 2; x++) {
         const int u = tid + x * C::THREADS, a = u / C::TKEYS, j = ft * C::TKEYS + u % C::TKEYS;
@@ -336,13 +366,13 @@ __global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS>::CTAS)
   };
   auto fetched = [&]() {  // the positions of the tile last fetched
     if (fh >= hk1 || tb >= te) return;
-    if (A.axes && (!stay || fh == hk0)) {
+    if (NA > 0 && A.axes && (!stay || fh == hk0)) {
       float* kp = spos + (stay ? ft - tb : fstage) * (S2S_MAX_AXES * C::TKEYS);
 #pragma unroll
       for (int x = 0; x < 2; x++) {
         const int u = tid + x * C::THREADS, a = u / C::TKEYS;
         if (a < A.axes) {
-          const int rf = a == 0 ? ref[0] : a == 1 ? ref[1] : ref[2];
+          const int rf = a == 0 ? ref[0] : a == 1 || NA < 3 ? ref[NA > 1] : ref[NA > 2 ? 2 : 0];
           kp[u] = (float)(int)((unsigned)kraw[x] - (unsigned)rf);
         }
       }
@@ -369,10 +399,10 @@ __global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS>::CTAS)
   }
 
   // bias: positions count from the tile's first query, so that near ones are exact
-  float qpos[2][S2S_MAX_AXES];
-  if (A.axes) {
+  float qpos[2][NA > 0 ? NA : 1];
+  if (NA > 0 && A.axes) {
 #pragma unroll
-    for (int a = 0; a < S2S_MAX_AXES; a++)
+    for (int a = 0; a < NA; a++)
       if (a < A.axes) {
         const int* qa = A.qpos + (int64_t)a * A.q_tokens;
         ref[a] = qa[D.q0 + i_first];
@@ -381,50 +411,57 @@ __global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS>::CTAS)
       }
   }
 
-  // Q fragments of a head straight from global memory
+  // Q fragments of a head straight from global memory (rows behind the last read the first)
   uint32_t qf[DK][4], qnext[DK][4];
-  auto load_q = [&](int hk) {
+  const T* qp[2];
+  T* op[2];
+#pragma unroll
+  for (int e = 0; e < 2; e++) {
+    const int h = hk0 * A.group + row_h[e];
+    qp[e] = static_cast<const T*>(A.q.data) + (int64_t)row_q[e] * A.q.token + (int64_t)h * A.q.head + 2 * t4;
+    op[e] = static_cast<T*>(A.out.data) + (int64_t)row_q[e] * A.out.token + (int64_t)h * A.out.head + 2 * t4;
+  }
+  auto load_q = [&]() {
 #pragma unroll
     for (int e = 0; e < 2; e++) {
-      const T* qp = static_cast<const T*>(A.q.data) + (int64_t)row_q[e] * A.q.token +
-                    (int64_t)(hk * A.group + row_h[e]) * A.q.head;
 #pragma unroll
       for (int kk = 0; kk < DK; kk++)
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
-          const int d = kk * 16 + 2 * t4 + x * 8;
-          qnext[kk][e + 2 * x] = live[e] && d < hd ? *reinterpret_cast<const uint32_t*>(qp + d) : 0u;
-        }
+        for (int x = 0; x < 2; x++)
+          qnext[kk][e + 2 * x] =
+              kk * 16 + x * 8 < hd ? *reinterpret_cast<const uint32_t*>(qp[e] + kk * 16 + x * 8) : 0u;
+      qp[e] += (int64_t)A.group * A.q.head;
     }
   };
   const float per_scale = 1.0f / A.scale;
-  float slope[2][S2S_MAX_AXES], snext[2][S2S_MAX_AXES];
+  float slope[2][NA > 0 ? NA : 1], snext[2][NA > 0 ? NA : 1];
   auto load_slopes = [&](int hk) {
 #pragma unroll
-    for (int a = 0; a < S2S_MAX_AXES; a++)
+    for (int a = 0; a < NA; a++)
       if (a < A.axes)
 #pragma unroll
         for (int e = 0; e < 2; e++) snext[e][a] = A.slopes[a * A.q_heads + hk * A.group + row_h[e]];
   };
-  load_q(hk0);
+  load_q();
   load_slopes(hk0);
   fetched();
   fetch();
   __syncthreads();  // the barriers are set up
 
+  bool mend = false;
   for (int hk = hk0; hk < hk1; hk++) {
 #pragma unroll
     for (int kk = 0; kk < DK; kk++)
 #pragma unroll
       for (int e = 0; e < 4; e++) qf[kk][e] = qnext[kk][e];
 #pragma unroll
-    for (int a = 0; a < S2S_MAX_AXES; a++)
+    for (int a = 0; a < NA; a++)
       if (a < A.axes)
 #pragma unroll
         for (int e = 0; e < 2; e++) slope[e][a] = fabsf(snext[e][a]) * per_scale;
     if constexpr (KW == 1)
       if (hk + 1 < hk1) {
-        load_q(hk + 1);
+        load_q();
         load_slopes(hk + 1);
       }
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
@@ -466,11 +503,11 @@ __global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS>::CTAS)
               mma_tile<T>(s[n + 1], qf[kk], b2, b3);
             }
           }
-        if (A.cap > 0.0f) capped(reinterpret_cast<float (&)[NT * 4]>(s), to_cap, raw_cap);
-        if (A.axes) {
+        if (CAP && A.cap > 0.0f) capped(reinterpret_cast<float (&)[NT * 4]>(s), to_cap, raw_cap);
+        if (NA > 0 && A.axes) {
           const float* kp = spos + (stay ? t - tb : stage) * (S2S_MAX_AXES * C::TKEYS) + kw * C::KEYS + 2 * t4;
 #pragma unroll
-          for (int a = 0; a < S2S_MAX_AXES; a++)
+          for (int a = 0; a < NA; a++)
             if (a < A.axes) {
               // |slope| |q - k| as |slope q - slope k|
               const F2 s0 = f2_both(-slope[0][a]), s1 = f2_both(-slope[1][a]);
@@ -559,16 +596,23 @@ __global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS>::CTAS)
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
     }
     if (KW == 1 && S == 1)
-      write_rows<T, DN>(A, D, hk, o, m, l, row_q, row_h, row_seen, live, kend, lane);
+      mend |= write_rows<T, DN>(A, hk, o, m, l, op, row_q, row_h, live, lane);
     else  // one head (cta_heads is 1)
       join_rows<T, DP, RW, WARPS>(A, D, hk, smem, o, m, l, r0, nrows, kend, S, split);
+#pragma unroll
+    for (int e = 0; e < 2; e++) op[e] += (int64_t)A.group * A.out.head;
+  }
+  if (KW == 1 && S == 1 && __any_sync(0xffffffffu, mend)) {
+#pragma unroll
+    for (int e = 0; e < 2; e++) op[e] -= (int64_t)(hk1 - hk0) * A.group * A.out.head;
+    mend_rows<T, DN>(A, D, hk0, hk1, op, row_q, row_h, row_seen, live, kend, lane);
   }
 }
 
-template <typename T, int DP, int RW, int WARPS>
+template <typename T, int DP, int RW, int WARPS, int NA = S2S_MAX_AXES, bool CAP = true>
 cudaError_t launch_attention_mma(AttnArgs& A, cudaStream_t st) {
   using C = MmaCfg<DP, RW, WARPS>;
-  auto kernel = k_attention_mma<T, DP, RW, WARPS>;
+  auto kernel = k_attention_mma<T, DP, RW, WARPS, NA, CAP>;
   static LaunchSetup setup;
   int ctas = 0;
   cudaError_t err = resident_ctas(setup, kernel, C::THREADS, C::SMEM, &ctas);
@@ -639,7 +683,13 @@ cudaError_t launch_attention_mma(AttnArgs& A, cudaStream_t st) {
   if (mean <= 16 || ctas(32) < 148)
     return wide ? launch_attention_mma<T, DP, 1, 8>(A, st) : launch_attention_mma<T, DP, 1, 4>(A, st);
   if (mean <= 32 || ctas(64) < 148) return launch_attention_mma<T, DP, 2, 4>(A, st);
-  return launch_attention_mma<T, DP, 4, 4>(A, st);
+  if (A.cap > 0.0f)
+    return A.axes == 0   ? launch_attention_mma<T, DP, 4, 4, 0, true>(A, st)
+           : A.axes <= 2 ? launch_attention_mma<T, DP, 4, 4, 2, true>(A, st)
+                         : launch_attention_mma<T, DP, 4, 4, 3, true>(A, st);
+  return A.axes == 0   ? launch_attention_mma<T, DP, 4, 4, 0, false>(A, st)
+         : A.axes <= 2 ? launch_attention_mma<T, DP, 4, 4, 2, false>(A, st)
+                       : launch_attention_mma<T, DP, 4, 4, 3, false>(A, st);
 }
 
 template <typename T>
