@@ -291,10 +291,23 @@ inline bool make_map_heads(CUtensorMap* map, const Rows& x, bool bf16, int64_t t
 namespace s2s {
 namespace {
 
+// Which of the two kernels, by what they measured (B200, cycles): a tcgen05 CTA takes 256 queries
+// over a key in 22 and 10000 besides, whatever the head; the mma.sync tiles take 0.25, 0.34 or 0.59
+// of an SM for each pair of query and key (head_dim up to 32, 64, 128), in as many CTAs as fill the
+// device. At eight heads of 64 and 8192 tokens in all, documents of 192: 23 us by mma.sync, 27 by
+// tcgen05; of 256: 26 and 22; of 512: 41 and 24. With 345 queries, 16 heads of 128 and 9000 keys
+// in three documents (48 tcgen05 CTAs): 62 and 96. S2S_MASKED_ATTN=mma or tcgen05 in the environment
+// (a validation switch, read at every call) takes that one.
 template <typename T>
 cudaError_t launch_attention(AttnArgs& A, cudaStream_t st) {
-  const bool many = A.q_tokens / A.documents >= 128 && A.kv_tokens > 0;
-  return many ? launch_attention_tc<T>(A, st) : launch_attention_mma<T>(A, st);
+  const double queries = (double)A.q_tokens / A.documents, keys = (double)A.kv_tokens / A.documents;
+  const double ctas = std::ceil(queries / (2 * kTcTile)) * A.documents * A.q_heads;
+  const double tc = std::ceil(ctas / 148) * (keys * 22 + 10000);
+  const double pair = A.head_dim <= 32 ? 0.25 : A.head_dim <= 64 ? 0.34 : 0.59;
+  const double mma = (double)A.q_tokens * A.q_heads * keys * pair / 148;
+  bool large = tc < mma;
+  if (const char* e = getenv("S2S_MASKED_ATTN")) large = !strcmp(e, "tcgen05") || (large && strcmp(e, "mma"));
+  return A.kv_tokens > 0 && large ? launch_attention_tc<T>(A, st) : launch_attention_mma<T>(A, st);
 }
 
 }  // namespace

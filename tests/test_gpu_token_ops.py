@@ -156,6 +156,13 @@ def test_rotary_inverse_is_the_gradient():
 
 
 # ---------------------------------------------------------------------------- attention
+@pytest.fixture(params=["mma", "tcgen05"])
+def kernel(request, monkeypatch):
+    """Each of the two attention kernels, whatever the sizes would choose."""
+    monkeypatch.setenv("S2S_MASKED_ATTN", request.param)
+    return request.param
+
+
 class Problem:
     """Tensors of one call on the CPU, and what the definition says in 64 bits."""
 
@@ -295,7 +302,7 @@ CASES = {
 
 @pytest.mark.parametrize("dtype", HALVES)
 @pytest.mark.parametrize("name", list(CASES))
-def test_attention(name, dtype):
+def test_attention(name, dtype, kernel):
     dim, qh, kh, q, kv, more = CASES[name]
     P = Problem(dtype, dim, qh, kh, q, kv, **more)
     out, lse = P.run()
@@ -304,8 +311,20 @@ def test_attention(name, dtype):
     assert torch.equal(out, again)
 
 
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("dim,heads,q,kv,more", [
+    (64, 8, [700, 1, 1500], [700, 1, 1500], dict(causal=True)),
+    (128, 8, [900, 300], [1300, 300], dict(causal=True, cap=50.0, prefix=[700, 0])),
+    (32, 10, [1000, 1000], [1000, 1100], dict(axes=2)),
+    (128, 6, [1500], [1500], dict(causal=True, axes=1, sharp=6.0))])
+def test_attention_of_the_size_for_the_large_kernel(dim, heads, q, kv, more, dtype):
+    """Sizes for which the library chooses its tcgen05 kernel by itself."""
+    P = Problem(dtype, dim, heads, heads // 2, q, kv, **more)
+    P.check(*P.run())
+
+
 @pytest.mark.parametrize("name", ["odd-causal", "windows", "single", "long", "long-cap-bias"])
-def test_attention_masked_values_may_be_anything(name):
+def test_attention_masked_values_may_be_anything(name, kernel):
     """NaN and infinities behind the last document and at keys that a row does not see."""
     dim, qh, kh, q, kv, more = CASES[name]
     P = Problem("float16", dim, qh, kh, q, kv, tail=(3, 150), **more)
@@ -317,7 +336,7 @@ def test_attention_masked_values_may_be_anything(name):
 
 @pytest.mark.parametrize("dtype", HALVES)
 @pytest.mark.parametrize("n", [20, 300, 900])
-def test_attention_hidden_values_of_the_own_document(n, dtype):
+def test_attention_hidden_values_of_the_own_document(n, dtype, kernel):
     """A NaN value in the middle of a causal document reaches the rows that see it, no other."""
     P = Problem(dtype, 64, 4, 2, [n], [n], causal=True)
     want = P.expected()
@@ -336,7 +355,7 @@ def test_attention_hidden_values_of_the_own_document(n, dtype):
 
 
 @pytest.mark.parametrize("name", ["windows", "odd-causal", "single", "long"])
-def test_attention_strides(name):
+def test_attention_strides(name, kernel):
     """q, k, v as parts of one row per token and head, as [head][token] planes, and as rows
     with gaps; outputs into a plane, their neighbours untouched."""
     dim, qh, kh, q, kv, more = CASES[name]
@@ -362,7 +381,7 @@ def test_attention_strides(name):
     assert wide[:, 0].isnan().all() and wide[..., :8].isnan().all() and wide[..., 8 + dim:].isnan().all()
 
 
-def test_attention_on_the_library_qkv_rows():
+def test_attention_on_the_library_qkv_rows(kernel):
     """The rows [token][head][q|k|v][dp] that the forward's QKV product writes."""
     P = Problem("float16", 32, 6, 6, [64] * 12, [64] * 12, axes=2)
     plain, _ = P.run()
@@ -373,7 +392,7 @@ def test_attention_on_the_library_qkv_rows():
 
 
 @pytest.mark.parametrize("q,kv,n", [(64, 64, 9), (1, 700, 5), (300, 310, 3), (20, 20, 1)])
-def test_attention_documents_of_equal_length_need_no_offsets(q, kv, n):
+def test_attention_documents_of_equal_length_need_no_offsets(q, kv, n, kernel):
     P = Problem("bfloat16", 64, 4, 2, [q] * n, [kv] * n, causal=True)
     with_offsets = P.run()
     without = P.run(offsets=False)
@@ -383,12 +402,12 @@ def test_attention_documents_of_equal_length_need_no_offsets(q, kv, n):
 
 
 @pytest.mark.parametrize("q,kv", [([70, 30], [70, 30]), ([1, 1], [300, 80]), ([600, 300], [600, 300])])
-def test_attention_leaves_rows_behind_the_documents(q, kv):
+def test_attention_leaves_rows_behind_the_documents(q, kv, kernel):
     P = Problem("float16", 64, 2, 2, q, kv, tail=(90, 0))
     P.check(*P.run())
 
 
-def test_attention_offsets_outside_the_tokens_stay_inside():
+def test_attention_offsets_outside_the_tokens_stay_inside(kernel):
     """Offsets past the tokens, negative and falling ones: results mean nothing, but nothing
     outside the outputs is written."""
     C = binding()
@@ -406,7 +425,7 @@ def test_attention_offsets_outside_the_tokens_stay_inside():
 
 
 @pytest.mark.parametrize("name", ["windows", "odd-causal-bias", "few", "long-cap-bias"])
-def test_attention_in_streams_and_graphs(name):
+def test_attention_in_streams_and_graphs(name, kernel):
     """Another stream; two calls at once; captured, replayed on changed inputs."""
     dim, qh, kh, q, kv, more = CASES[name]
     P, R = (Problem("bfloat16", dim, qh, kh, q, kv, seed=s, **more) for s in (0, 1))
@@ -445,7 +464,7 @@ def test_host_memory_is_refused():
 
 # ----------------------------------------------------------------------------- together
 @pytest.mark.parametrize("dtype", HALVES)
-def test_rotary_then_attention(dtype):
+def test_rotary_then_attention(dtype, kernel):
     """Frames of two clips: q and k turned along time, height and width, then attended with
     the same positions for the bias, a prefix of each clip seen whole; one stream, and the
     whole run replayed as a graph."""
