@@ -193,6 +193,13 @@ __device__ __forceinline__ void capped(float (&s)[N], float to_cap, float raw_ca
   }
 }
 
+// Before a CTA ends after a wait that gave up: the copy on `bar` has landed, or half a second is over.
+__device__ __forceinline__ void wait_landed(uint64_t* bar, uint32_t phase) {
+  const uint64_t t0 = global_timer_ns();
+  while (!mbar_try_wait(smem_u32(bar), phase) && global_timer_ns() - t0 < 500000000ull) {
+  }
+}
+
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar,
                                             int c0, int c1, int c2) {
   asm volatile(
@@ -209,39 +216,61 @@ __device__ __forceinline__ float4 load4(const T* p) {
   return make_float4(to_f32(t[0]), to_f32(t[1]), to_f32(t[2]), to_f32(t[3]));
 }
 
-// One query row of one head by one warp, key after key: lane l has the values
-// 4l .. 4l + 3 of the head. For rows that a tile cannot do: it multiplies the values of
-// keys that a row does not see by zero weights, and zero times NaN or infinity is NaN.
+// A row whose outputs came out NaN or infinite, again by one warp: lane l has the values 4l .. 4l + 3
+// of the head. The tile kernels multiply the values of keys that a row does not see by zero weights,
+// and zero times NaN or infinity is NaN; `end`: the keys that the row's tile went through. Nothing is
+// to be done where those values are finite, or where each column that they reach has a NaN among the
+// keys that the row does see; only what is left is computed, key after key. The row's sum is right
+// as it is.
 template <typename T>
-__device__ __noinline__ void attend_row(const AttnArgs& A, const Doc D, int i, int h, int lane) {
+__device__ __noinline__ void attend_row(const AttnArgs& A, const Doc D, int i, int h, int end, int lane) {
   const int qrow = D.q0 + i, hk = h / A.group, d = lane * 4;
   const bool mine = d < A.head_dim;
-  const T* k = static_cast<const T*>(A.k.data) + (int64_t)hk * A.k.head + d;
-  const T* v = static_cast<const T*>(A.v.data) + (int64_t)hk * A.v.head + d;
+  const T* k = static_cast<const T*>(A.k.data) + (int64_t)D.k0 * A.k.token + (int64_t)hk * A.k.head + d;
+  const T* v = static_cast<const T*>(A.v.data) + (int64_t)D.k0 * A.v.token + (int64_t)hk * A.v.head + d;
+  const int n = seen(A, D, i);
+  float reached[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // NaN: by a hidden NaN or infinity
+  if (mine)
+    for (int j = n; j < min(end, D.nk); j++) {
+      const float4 x = load4(v + (int64_t)j * A.v.token);
+      reached[0] = fmaf(x.x, 0.0f, reached[0]);
+      reached[1] = fmaf(x.y, 0.0f, reached[1]);
+      reached[2] = fmaf(x.z, 0.0f, reached[2]);
+      reached[3] = fmaf(x.w, 0.0f, reached[3]);
+    }
+  bool open = reached[0] != 0.0f || reached[1] != 0.0f || reached[2] != 0.0f || reached[3] != 0.0f;
+  for (int j = 0; __any_sync(0xffffffffu, open) && j < n; j++) {
+    if (!open) continue;
+    const float4 x = load4(v + (int64_t)j * A.v.token);
+    if (x.x != x.x) reached[0] = 0.0f;
+    if (x.y != x.y) reached[1] = 0.0f;
+    if (x.z != x.z) reached[2] = 0.0f;
+    if (x.w != x.w) reached[3] = 0.0f;
+    open = reached[0] != 0.0f || reached[1] != 0.0f || reached[2] != 0.0f || reached[3] != 0.0f;
+  }
+  if (!__any_sync(0xffffffffu, open)) return;
+
   float4 q = make_float4(0, 0, 0, 0), o = q;
   if (mine)
-    q = load4(static_cast<const T*>(A.q.data) + (int64_t)qrow * A.q.token +
-              (int64_t)h * A.q.head + d);
-  const int n = seen(A, D, i);
+    q = load4(static_cast<const T*>(A.q.data) + (int64_t)qrow * A.q.token + (int64_t)h * A.q.head + d);
   float m = -INFINITY, l = 0.0f;
   for (int j = 0; j < n; j++) {
-    const int64_t row = D.k0 + j;
     float s = 0.0f;
     if (mine) {
-      const float4 x = load4(k + row * A.k.token);
+      const float4 x = load4(k + (int64_t)j * A.k.token);
       s = q.x * x.x + q.y * x.y + q.z * x.z + q.w * x.w;
     }
 #pragma unroll
     for (int w = 16; w; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
     float z = s * A.scale;
     if (A.cap > 0.0f) z = A.cap * tanhf(z / A.cap);
-    z = z * kLog2e + distance_bias(A, h, qrow, (int)row);
+    z = z * kLog2e + distance_bias(A, h, qrow, D.k0 + j);
     if (z == -INFINITY) continue;
     const float top = fmaxf(m, z), keep = ex2(m - top), p = ex2(z - top);
     m = top;
     l = l * keep + p;
     if (mine) {
-      const float4 x = load4(v + row * A.v.token);
+      const float4 x = load4(v + (int64_t)j * A.v.token);
       o.x = o.x * keep + p * x.x;
       o.y = o.y * keep + p * x.y;
       o.z = o.z * keep + p * x.z;
@@ -259,8 +288,6 @@ __device__ __noinline__ void attend_row(const AttnArgs& A, const Doc D, int i, i
     *reinterpret_cast<uint2*>(static_cast<T*>(A.out.data) + (int64_t)qrow * A.out.token +
                               (int64_t)h * A.out.head + d) = u;
   }
-  if (A.lse && lane == 0)
-    A.lse[(int64_t)h * A.q_tokens + qrow] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 // Rows of heads as a [tokens][heads][head_dim] tensor, in boxes of `rows` tokens, one head and

@@ -138,7 +138,7 @@ __device__ __forceinline__ bool write_rows(const AttnArgs& A, int hk, const floa
   float check = 0.0f;
 #pragma unroll
   for (int e = 0; e < 2; e++) {
-    const bool none = m[e] == -INFINITY;
+    const bool none = m[e] == -INFINITY && l[e] == 0.0f;  // a sum that is NaN is kept
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(l[e]));
     if (none) inv = 0.0f;
@@ -181,7 +181,7 @@ __device__ __forceinline__ void mend_rows(const AttnArgs& A, const Doc& D, int h
         const int src = __ffs(redo) - 1;
         redo &= ~(15u << (src & ~3));
         const int i = __shfl_sync(0xffffffffu, row_q[e], src) - D.q0;
-        attend_row<T>(A, D, i, hk * A.group + __shfl_sync(0xffffffffu, row_h[e], src), lane);
+        attend_row<T>(A, D, i, hk * A.group + __shfl_sync(0xffffffffu, row_h[e], src), kend, lane);
       }
     }
 }
@@ -266,7 +266,7 @@ __device__ __forceinline__ void join_rows(const AttnArgs& A, const Doc& D, int h
       total = mlc[r].y;
     }
     const int i = (r0 + r) / A.group, h = hk * A.group + r0 + r - i * A.group;
-    const bool none = top == -INFINITY;
+    const bool none = top == -INFINITY && total == 0.0f;  // a sum that is NaN is kept
     const float inv = none ? 0.0f : 1.0f / total;
     const float4 x = none ? make_float4(0, 0, 0, 0)
                           : make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
@@ -283,7 +283,7 @@ __device__ __forceinline__ void join_rows(const AttnArgs& A, const Doc& D, int h
   for (int r = warp; r < C::ROWS; r += WARPS)
     if (flag[r]) {
       const int i = (r0 + r) / A.group;
-      attend_row<T>(A, D, i, hk * A.group + r0 + r - i * A.group, lane);
+      attend_row<T>(A, D, i, hk * A.group + r0 + r - i * A.group, kend, lane);
     }
   if (S > 1) cluster_sync();  // nobody leaves while its shared memory is read
 }
@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS, NA>::CTAS)
   pdl_wait();
   // the stages that are filled and computed next, the phase of the latter; a wait that gave up is
   // not followed by others, but the CTA's barriers are met all the same
-  int fstage = 0, stage = 0;
+  int fstage = 0, stage = 0, flying = 0;  // copies that are not waited for yet (thread 0)
   uint32_t phase = 0;
   bool ok = true;
 
@@ -348,7 +348,8 @@ __global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS, NA>::CTAS)
   const bool stay = te - tb <= kMmaStages;
   auto fetch = [&]() {
     if (fh >= hk1 || tb >= te) return;
-    if (tid == 0) {
+    if (tid == 0 && ok) {
+      flying++;
       uint8_t* dst = smem + fstage * 2 * C::TILE;
       mbar_arrive_expect_tx(&full[fstage], 2 * C::TILE);
 #pragma unroll
@@ -470,7 +471,13 @@ __global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS, NA>::CTAS)
     for (int n = 0; n < DN; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
 
     for (int t = tb; t < te; t++) {
-      if (ok) ok = mbar_wait(&full[stage], phase, DEV_TIMEOUT_FULL);
+      if (ok) {
+        ok = mbar_wait(&full[stage], phase, DEV_TIMEOUT_FULL);
+        if (ok) flying--;
+        else if (tid == 0)  // nothing is fetched after this
+          for (int k = 0; k < flying; k++)
+            wait_landed(&full[(stage + k) % kMmaStages], stage + k >= kMmaStages ? phase ^ 1 : phase);
+      }
       const int tail = kend - t * C::TKEYS;  // keys of the tile that some row sees
       if (tail < C::TKEYS) {
         // behind them lie other documents' rows, or none: zero weights must not meet what is

@@ -301,10 +301,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // no copy is in flight when the CTA ends, also where a wait gave up
       if (N > 0)
         for (int w = 0; w < 2; w++)
-          if (n[w] > 0) mbar_wait(&q_full[w], 0, DEV_TIMEOUT_FULL);
+          if (n[w] > 0) wait_landed(&q_full[w], 0);
       for (int k = max(0, i - ST); k < i; k++) {
-        mbar_wait(&k_full[k % ST], (k / ST) & 1, DEV_TIMEOUT_FULL);
-        if (ok || k < i - 1) mbar_wait(&v_full[k % ST], (k / ST) & 1, DEV_TIMEOUT_FULL);
+        wait_landed(&k_full[k % ST], (k / ST) & 1);
+        if (ok || k < i - 1) wait_landed(&v_full[k % ST], (k / ST) & 1);
       }
     }
     // values that steer the products, from reductions, which give uniform registers
@@ -690,7 +690,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
     // ------------------------------------------------------------------- output
     if (n_w > 0) output_done(n_w - 1);
-    const bool none = m == -INFINITY;
+    const bool none = m == -INFINITY && l == 0.0f;  // a sum that is NaN is kept
     const float inv = none ? 0.0f : 1.0f / l;
     float check = 0.0f;  // NaN where an output is NaN or infinite
     T* out = static_cast<T*>(A.out.data) + (int64_t)(D.q0 + i) * A.out.token + (int64_t)h * A.out.head;
@@ -713,14 +713,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
     if (live && A.lse)
       A.lse[(int64_t)h * A.q_tokens + D.q0 + i] = none ? -INFINITY : (m + log2f(l)) * kLn2;
-    // keys of the document that this row does not see had zero weights: a NaN or infinity
-    // among their values shows here, and the row is done again without them
+    // keys of the document that this row does not see had zero weights: a NaN or infinity among
+    // their values shows here
     unsigned redo = __ballot_sync(0xffffffffu, check != 0.0f && live && mine < kmax);
     __syncwarp();
     while (redo) {
       const int src = __ffs(redo) - 1;
       redo &= redo - 1;
-      attend_row<T>(A, D, i0 + w * kTcTile + (warp & 3) * 32 + src, h, lane);
+      attend_row<T>(A, D, first + (warp & 3) * 32 + src, h, kmax, lane);
     }
   }
   tc_fence_before();

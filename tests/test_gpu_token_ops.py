@@ -354,6 +354,36 @@ def test_attention_hidden_values_of_the_own_document(n, dtype, kernel):
     assert here.all()
 
 
+@pytest.mark.parametrize("what", ["all", "channel", "first", "query"])
+def test_attention_values_that_are_nan_for_good(what, kernel):
+    """NaN wherever the definition has it and nowhere else, at the size where a row done again
+    key after key would show in the time: all values, one channel, the first key, one query."""
+    n = 3000
+    P = Problem("bfloat16", 64, 4, 2, [n], [n], causal=True)
+    want = P.expected()
+    if what == "all":
+        P.v[:] = float("nan")
+    elif what == "channel":
+        P.v[:, :, 7] = float("nan")
+    elif what == "first":
+        P.v[0] = float("nan")
+    else:
+        P.q[100] = float("nan")
+    out, lse = P.run()
+    got = out.cpu().double()
+    nan = torch.zeros(n, 4, 64, dtype=torch.bool)
+    if what in ("all", "first"):
+        nan[:] = True
+    elif what == "channel":
+        nan[..., 7] = True
+    else:
+        nan[100] = True
+    assert torch.equal(got.isnan(), nan)
+    assert ((got - want[0]).abs() <= want[2])[~nan].all()
+    rows = torch.arange(n) != (100 if what == "query" else -1)
+    assert ((lse.cpu().double() - want[1]).abs() <= want[3])[:, rows].all()
+
+
 @pytest.mark.parametrize("name", ["windows", "odd-causal", "single", "long"])
 def test_attention_strides(name, kernel):
     """q, k, v as parts of one row per token and head, as [head][token] planes, and as rows
