@@ -333,8 +333,11 @@ int s2s_rotary_apply(const s2s_rotary* r, int dtype, int head_dim, int tokens, c
  * and key j is seen if causal == 0, or j <= i + nk - nq, or j < d_prefix[d] (NULL: none).
  * out_i = sum of softmax(z)_j v_j over the keys seen, d_lse = log sum exp(z) in fp32; a row
  * that sees no key (or only scores of minus infinity) gives zeros and minus infinity.
- * Values at keys that no mask of the row lets through never reach it, NaN and infinities
- * included. Rows of no document are left as they were. */
+ * Values at keys that a row does not see never reach it, NaN and infinities included. Rows
+ * of no document are left as they were. out and d_lse may not overlap each other or an
+ * input. Two positions of a document lie less than 2^31 apart. The result of a call does not
+ * depend on what else runs; a bounded wait that gives up (s2s_device_status) leaves it
+ * undefined. */
 typedef struct s2s_attention {
   int dtype;     /* S2S_F16 or S2S_BF16, of q, k, v and out */
   int head_dim;  /* a multiple of 8, at most 128 */
