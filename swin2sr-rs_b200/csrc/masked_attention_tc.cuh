@@ -191,13 +191,14 @@ struct TcPlace {
   }
 };
 
-// MODE 0: no cap, no bias; 1: a cap; 2: a bias, with or without a cap.
+// MODE 0: no cap, no bias; 1: a cap; 2: a bias of one or two axes, 3: of three, with or without a cap.
 template <typename T, int NP, int MODE>
 __global__ void __launch_bounds__(kTcThreads, 1)
     k_attention_tc(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap mapQ,
                    const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV) {
   using C = TcCfg<NP>;
   constexpr int BN = C::BN, NB = C::NB, ST = C::STAGES;
+  constexpr int NA = MODE == 2 ? 2 : S2S_MAX_AXES;  // the most axes of a bias
   using Place = TcPlace<NB>;
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ uint8_t smem_raw[];
@@ -271,7 +272,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   // keys, and wrap around: scores that grew from tile to tile on the way there would have the
   // outputs scaled again for each. Both row tiles then take all of them.
   int start = 0;
-  if (MODE == 2) {
+  if (MODE >= 2) {
     n[0] = rows[0] > 0 ? max(n[0], n[1]) : 0;
     n[1] = rows[1] > 0 ? n[0] : 0;
     start = max(0, min((i0 + D.nk - D.nq) / BN, n[0] - 1));
@@ -280,9 +281,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int ksteps = (A.head_dim + 15) / 16;
 
   // registers: 384 threads begin with 168 each; the softmax groups take what the third gives
-  // (2 * 128 * 200 + 128 * 96 = 63488 of 64512)
+  // (2 * 128 * 208 + 128 * 80 or 2 * 128 * 216 + 128 * 64, 63488 of 64512; with a bias 200 took 5 %
+  // more time, with a cap 208 6 %)
+  constexpr int kSoftmaxRegisters = MODE == 1 ? 216 : 208, kOtherRegisters = MODE == 1 ? 64 : 80;
   if (warp >= 8) {
-    fewer_registers<96>();
+    fewer_registers<kOtherRegisters>();
     if (warp == 8 && lane == 0) {
       // ------------------------------------------------------------------ loads
       auto load = [&](uint8_t* dst, int bytes, const CUtensorMap* map, uint64_t* bar, int head, int row) {
@@ -319,7 +322,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int keys = (int)__reduce_max_sync(0xffffffffu, (unsigned)kmax);
     const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
     const int last = max(n0, n1) - 1;
-    const int cut = MODE == 2 ? (int)__reduce_max_sync(0xffffffffu, (unsigned)(last - start)) : last;  // step of the last keys
+    const int cut = MODE >= 2 ? (int)__reduce_max_sync(0xffffffffu, (unsigned)(last - start)) : last;  // step of the last keys
     // after a wait that gave up the products go on without waiting, over whatever is there
     bool ok = true;
     auto wait = [&](uint64_t* bar, int phase, unsigned code) {
@@ -422,7 +425,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_wait(&fin[2], 0, DEV_TIMEOUT_ACC);
     }
   } else {
-    more_registers<200>();
+    more_registers<kSoftmaxRegisters>();
     // ------------------------------------------------------------------ softmax
     const int w = warp >> 2, r = tid & 127;
     const int rows_w = w ? rows[1] : rows[0], n_w = w ? n[1] : n[0];
@@ -534,15 +537,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // a key's positions then serve four scores. (With a row a thread every thread read all the
       // tile's positions, and shared memory was what bound it.)
       const int g = lane >> 2, t4 = lane & 3;
-      float rm[4], rl[4], qf[4][S2S_MAX_AXES], slope[S2S_MAX_AXES];
-      int rseen[4], ref[S2S_MAX_AXES], kraw[S2S_MAX_AXES];
+      float rm[4], rl[4], qf[4][NA], slope[NA];
+      int rseen[4], ref[NA], kraw[NA];
       float* pos = spos + w * 2 * S2S_MAX_AXES * BN;
       // the positions of a tile's keys, times the slope, each loaded a tile ahead by one thread
       auto key_positions = [&](int t) {
         const int j = key_tile(t) * BN + r;
         if (r < BN)
 #pragma unroll
-          for (int a = 0; a < S2S_MAX_AXES; a++)
+          for (int a = 0; a < NA; a++)
             if (a < A.axes) kraw[a] = j < D.nk ? A.kpos[(int64_t)a * A.kv_tokens + D.k0 + j] : ref[a];
       };
 #pragma unroll
@@ -554,7 +557,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       if (n_w > 0) {
 #pragma unroll
-        for (int a = 0; a < S2S_MAX_AXES; a++)
+        for (int a = 0; a < NA; a++)
           if (a < A.axes) {
             const int* qa = A.qpos + (int64_t)a * A.q_tokens + D.q0;
             ref[a] = qa[i0];
@@ -573,7 +576,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         float* kp = pos + (t & 1) * S2S_MAX_AXES * BN;
         if (r < BN)
 #pragma unroll
-          for (int a = 0; a < S2S_MAX_AXES; a++)
+          for (int a = 0; a < NA; a++)
             if (a < A.axes) kp[a * BN + r] = slope[a] * (float)(int)((unsigned)kraw[a] - (unsigned)ref[a]);
         group_sync(1 + w);
         if (t + 1 < n_w) key_positions(t + 1);
@@ -594,7 +597,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         float(&s)[2][BN / 64][32] = reinterpret_cast<float(&)[2][BN / 64][32]>(raw);
         if (A.cap > 0.0f) capped(reinterpret_cast<float(&)[BN]>(raw), to_cap, raw_cap);
 #pragma unroll
-        for (int a = 0; a < S2S_MAX_AXES; a++)
+        for (int a = 0; a < NA; a++)
           if (a < A.axes) {
 #pragma unroll
             for (int c = 0; c < BN / 64; c++)
@@ -758,10 +761,12 @@ cudaError_t launch_attention_tc(AttnArgs& A, cudaStream_t st) {
 template <typename T>
 cudaError_t launch_attention_tc(AttnArgs& A, cudaStream_t st) {
   if (A.head_dim <= 64)
-    return A.axes         ? launch_attention_tc<T, 1, 2>(A, st)
+    return A.axes > 2     ? launch_attention_tc<T, 1, 3>(A, st)
+           : A.axes       ? launch_attention_tc<T, 1, 2>(A, st)
            : A.cap > 0.0f ? launch_attention_tc<T, 1, 1>(A, st)
                           : launch_attention_tc<T, 1, 0>(A, st);
-  return A.axes         ? launch_attention_tc<T, 2, 2>(A, st)
+  return A.axes > 2     ? launch_attention_tc<T, 2, 3>(A, st)
+         : A.axes       ? launch_attention_tc<T, 2, 2>(A, st)
          : A.cap > 0.0f ? launch_attention_tc<T, 2, 1>(A, st)
                         : launch_attention_tc<T, 2, 0>(A, st);
 }
