@@ -1,18 +1,18 @@
 // The attention of masked_attention.cu on mma.sync tiles, for short documents, few queries
 // and small work.
 //
-// A CTA of four warps takes 16 * RW rows of one document and key head - a row is a query and
-// one of the query heads that share the key head, so K and V are read once for all of them -
-// and walks the keys in tiles of 64 through a ring of three stages that TMA fills. RW warps lie
-// along the rows, 4 / RW along the keys of a tile: one query of eight heads is one row tile,
-// whose keys the four warps share. Every warp keeps a running maximum, sum and output of its
-// own; they are joined once at the end, first within the CTA, then over the CTAs of a cluster
+// A CTA of four warps (eight where it has an SM for itself) takes 16 * RW rows of one document and
+// key head - a row is a query and one of the query heads that share the key head, so K and V are
+// read once for all of them - and walks the keys in tiles of 16 a warp through a ring of three
+// stages that TMA fills. RW warps lie along the rows, the others along the keys of a tile: one
+// query of eight heads is one row tile, whose keys the warps share. Every warp keeps a running
+// maximum, sum and output of its own; they are joined once at the end, first within the CTA, then over the CTAs of a cluster
 // among which the keys of the tile were split (through distributed shared memory: a call
 // needs no workspace, and the order of the sums is fixed).
 //
 // Bound: HBM where the keys are long (K and V are read once), else the latency of a tile's chain of
 // products, softmax and products, of which an SM has eight to sixteen warps' worth to hide. Measured
-// (B200): 24 single queries of 32 heads over 111 000 keys of 8 x 128, 444 MB: 101 us, 4.4 TB/s
+// (B200): 24 single queries of 32 heads over 111 000 keys of 8 x 128, 444 MB: 102 us, 4.3 TB/s
 // (68 us at the measured copy rate); 1271 windows of 64, six heads of 32, two axes: 54 us (45
 // without a bias, 19 for the bytes); 5 queries of 16 heads over 40001 keys of 2 x 128: 30 us.
 #pragma once

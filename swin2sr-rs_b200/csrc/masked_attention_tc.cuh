@@ -19,9 +19,10 @@
 //
 // Bound: for head_dim <= 64 the special function unit (16 exponentials a cycle and SM: 2048 cycles
 // for 256 x 128 pairs, of 2900), beyond it the tensor core with its 64-key score products (2560 of
-// 3000). Measured (B200, non-causal, 37 heads, 4096 x 4096): 192 us at head 64, 825 TFLOP/s; 285 us
-// at head 128, 1110 TFLOP/s, 0.68 of the measured bf16 rate; causal 16384, eight heads of 128: 445
-// us, 1230 TFLOP/s. With a cap of 50: 350 and 387 us; with one axis of bias 310 and 369.
+// 3000). Measured (B200, non-causal, 37 heads, 4096 x 4096): 195 us at head 64, 811 TFLOP/s; 281 us
+// at head 128, 1130 TFLOP/s, 0.69 of the measured bf16 rate; causal 16384, eight heads of 128: 434-447
+// us, 1230 TFLOP/s. With a cap of 50: 331 and 398 us; with one axis of bias 288 and 372; with two
+// axes at head 64 334.
 #pragma once
 
 namespace s2s {
@@ -462,8 +463,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     };
     // With a bias the two softmax warps of a scheduler (warp and warp ^ 4) take turns at the
     // exponentials, so that one's keep the special function unit busy while the other is at its
-    // bias (12 heads, images of 3136 + 4096 + ...: 338 -> 308 us; without a bias turns cost more than
-    // they give, 193 -> 238 us at 37 heads of 64 x 4096^2).
+    // bias (12 heads of 64, six images of up to 4096 tokens: 338 -> 308 us when they were added,
+    // 292 with today's registers; without a bias turns cost more than they give, 193 -> 238 us at 37
+    // heads of 64 x 4096^2).
     auto my_turn = [&](int t) {
       const int u = w ? t : t - 1;  // tile 0 first
       if (ok && u >= 0 && u < (w ? n[0] : n[1])) ok = mbar_wait(&turn[warp ^ 4], u & 1, DEV_TIMEOUT_ACC);
