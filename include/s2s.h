@@ -335,7 +335,8 @@ int s2s_rotary_apply(const s2s_rotary* r, int dtype, int head_dim, int tokens, c
  * that sees no key (or only scores of minus infinity) gives zeros and minus infinity.
  * Values at keys that a row does not see never reach it, NaN and infinities included. Rows
  * of no document are left as they were. out and d_lse may not overlap each other or an
- * input. Two positions of a document lie less than 2^31 apart. The result of a call does not
+ * input. Two positions of a document lie less than 2^31 apart (distances are exact while the
+ * queries' own positions lie less than 2^24 apart, else rounded to 2^-23 of that). The result of a call does not
  * depend on what else runs; a bounded wait that gives up (s2s_device_status) leaves it
  * undefined. */
 typedef struct s2s_attention {

@@ -120,6 +120,7 @@ __device__ __forceinline__ float distance_bias(const AttnArgs& A, int h, int qro
 
 using F2 = unsigned long long;  // two fp32 lanes of the packed operations
 __device__ __forceinline__ F2 f2_both(float x) { return f2_pack(x, x); }
+__device__ __forceinline__ F2 f2_abs(F2 x) { return x & 0x7fffffff7fffffffull; }
 
 // The larger and the smaller of three.
 __device__ __forceinline__ float max3(float a, float b, float c) {

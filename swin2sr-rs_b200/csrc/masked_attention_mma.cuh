@@ -13,7 +13,7 @@
 // Bound: HBM where the keys are long (K and V are read once), else the latency of a tile's chain of
 // products, softmax and products, of which an SM has eight to sixteen warps' worth to hide. Measured
 // (B200): 24 single queries of 32 heads over 111 000 keys of 8 x 128, 444 MB: 102 us, 4.3 TB/s
-// (68 us at the measured copy rate); 1271 windows of 64, six heads of 32, two axes: 54 us (45
+// (68 us at the measured copy rate); 1271 windows of 64, six heads of 32, two axes: 55 us (45
 // without a bias, 19 for the bytes); 5 queries of 16 heads over 40001 keys of 2 x 128: 30 us.
 #pragma once
 
@@ -520,17 +520,17 @@ __global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS, NA>::CTAS)
 #pragma unroll
           for (int a = 0; a < NA; a++)
             if (a < A.axes) {
-              // |slope| |q - k| as |slope q - slope k|
               const F2 s0 = f2_both(-slope[0][a]), s1 = f2_both(-slope[1][a]);
-              const F2 q0 = f2_both(slope[0][a] * qpos[0][a]), q1 = f2_both(slope[1][a] * qpos[1][a]);
+              const F2 q0 = f2_both(-qpos[0][a]), q1 = f2_both(-qpos[1][a]);
 #pragma unroll
               for (int n = 0; n < NT; n++) {
                 const F2 k2 = *reinterpret_cast<const F2*>(kp + a * C::TKEYS + n * 8);
-                const float2 d0 = f2_unpack(f2_fma(k2, s0, q0)), d1 = f2_unpack(f2_fma(k2, s1, q1));
-                s[n][0] -= fabsf(d0.x);
-                s[n][1] -= fabsf(d0.y);
-                s[n][2] -= fabsf(d1.x);
-                s[n][3] -= fabsf(d1.y);
+                const float2 z0 = f2_unpack(f2_fma(f2_abs(f2_add(k2, q0)), s0, f2_pack(s[n][0], s[n][1])));
+                const float2 z1 = f2_unpack(f2_fma(f2_abs(f2_add(k2, q1)), s1, f2_pack(s[n][2], s[n][3])));
+                s[n][0] = z0.x;
+                s[n][1] = z0.y;
+                s[n][2] = z1.x;
+                s[n][3] = z1.y;
               }
             }
         }

@@ -167,6 +167,17 @@ __device__ __forceinline__ void fewer_registers() {
 __device__ __forceinline__ void group_sync(int id) {
   asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
 }
+// Whether x holds for any thread of the group.
+__device__ __forceinline__ bool group_any(int id, bool x) {
+  uint32_t y;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(y)
+      : "r"((uint32_t)x), "r"(id)
+      : "memory");
+  return y != 0;
+}
 
 // Where the products of key tile i and row tile w have their place: score buffer and the parity of
 // its use. Three buffers are taken in the order of the products, tile 0 and 1 in turn and at the
@@ -464,7 +475,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // With a bias the two softmax warps of a scheduler (warp and warp ^ 4) take turns at the
     // exponentials, so that one's keep the special function unit busy while the other is at its
     // bias (12 heads of 64, six images of up to 4096 tokens: 338 -> 308 us when they were added,
-    // 292 with today's registers; without a bias turns cost more than they give, 193 -> 238 us at 37
+    // 304 now; without a bias turns cost more than they give, 193 -> 238 us at 37
     // heads of 64 x 4096^2).
     auto my_turn = [&](int t) {
       const int u = w ? t : t - 1;  // tile 0 first
@@ -542,7 +553,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       float rm[4], rl[4], qf[4][NA], slope[NA];
       int rseen[4], ref[NA], kraw[NA];
       float* pos = spos + w * 2 * S2S_MAX_AXES * BN;
-      // the positions of a tile's keys, times the slope, each loaded a tile ahead by one thread
+      // the positions of a tile's keys, each loaded a tile ahead by one thread
       auto key_positions = [&](int t) {
         const int j = key_tile(t) * BN + r;
         if (r < BN)
@@ -557,6 +568,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         rl[R] = 0.0f;
         rseen[R] = x < rows_w ? seen(A, D, first + x) : 0;
       }
+      // |slope| |q - k| as |slope q - slope k|, one operation a pair less, while that is right: the
+      // rounding of slope q is below 2^-14 of a score's power of two. (All tiles in the other form: 325
+      // us for the six images of up to 4096 tokens; the choice costs 292 -> 304.)
+      bool near = true, far = false;
       if (n_w > 0) {
 #pragma unroll
         for (int a = 0; a < NA; a++)
@@ -567,124 +582,146 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
             for (int R = 0; R < 4; R++) {
               const int x = (warp & 3) * 32 + g + 8 * R;
-              qf[R][a] = -slope[a] * (float)(int)((unsigned)qa[x < rows_w ? first + x : i0] - (unsigned)ref[a]);
+              qf[R][a] = -(float)(int)((unsigned)qa[x < rows_w ? first + x : i0] - (unsigned)ref[a]);
+              far |= fabsf(qf[R][a]) * slope[a] * unit >= 1024.0f;
             }
           }
-        key_positions(0);
-      }
-      for (int t = 0; t < n_w; t++) {
-        const Place at(w, t, n[0], n[1]);
-        const uint32_t ts = lanes + at.buffer * BN;
-        float* kp = pos + (t & 1) * S2S_MAX_AXES * BN;
-        if (r < BN)
+        near = !group_any(1 + w, far);
+        if (near)
 #pragma unroll
           for (int a = 0; a < NA; a++)
-            if (a < A.axes) kp[a * BN + r] = slope[a] * (float)(int)((unsigned)kraw[a] - (unsigned)ref[a]);
-        group_sync(1 + w);
-        if (t + 1 < n_w) key_positions(t + 1);
-        if (ok) ok = mbar_wait(&s_full[at.buffer], at.parity, DEV_TIMEOUT_ACC);
-        __syncwarp();
-        tc_fence_after();
-        // [half][64 keys]: value 4 k + e is key 8 k + 2 t4 + (e & 1) of row R = 2 half + (e >> 1)
-        uint32_t raw[2][BN / 64][32];
 #pragma unroll
-        for (int x = 0; x < 2; x++)
+            for (int R = 0; R < 4; R++) qf[R][a] *= a < A.axes ? slope[a] : 1.0f;
+        key_positions(0);
+      }
+      auto walk = [&](auto form) {
+        constexpr bool NEAR = decltype(form)::value;
+        for (int t = 0; t < n_w; t++) {
+          const Place at(w, t, n[0], n[1]);
+          const uint32_t ts = lanes + at.buffer * BN;
+          float* kp = pos + (t & 1) * S2S_MAX_AXES * BN;
+          if (r < BN)
 #pragma unroll
-          for (int c = 0; c < BN / 64; c++) tmem_ld_frag(ts + ((uint32_t)x << 20) + c * 64, raw[x][c]);
-        tc_wait_ld();
+            for (int a = 0; a < NA; a++)
+              if (a < A.axes) kp[a * BN + r] = (NEAR ? slope[a] : 1.0f) * (float)(int)((unsigned)kraw[a] - (unsigned)ref[a]);
+          group_sync(1 + w);
+          if (t + 1 < n_w) key_positions(t + 1);
+          if (ok) ok = mbar_wait(&s_full[at.buffer], at.parity, DEV_TIMEOUT_ACC);
+          __syncwarp();
+          tc_fence_after();
+          // [half][64 keys]: value 4 k + e is key 8 k + 2 t4 + (e & 1) of row R = 2 half + (e >> 1)
+          uint32_t raw[2][BN / 64][32];
 #pragma unroll
-        for (int x = 0; x < 2; x++)
+          for (int x = 0; x < 2; x++)
 #pragma unroll
-          for (int c = 0; c < BN / 64; c++) loaded(raw[x][c]);
-        float(&s)[2][BN / 64][32] = reinterpret_cast<float(&)[2][BN / 64][32]>(raw);
-        if (A.cap > 0.0f) capped(reinterpret_cast<float(&)[BN]>(raw), to_cap, raw_cap);
+            for (int c = 0; c < BN / 64; c++) tmem_ld_frag(ts + ((uint32_t)x << 20) + c * 64, raw[x][c]);
+          tc_wait_ld();
 #pragma unroll
-        for (int a = 0; a < NA; a++)
-          if (a < A.axes) {
+          for (int x = 0; x < 2; x++)
+#pragma unroll
+            for (int c = 0; c < BN / 64; c++) loaded(raw[x][c]);
+          float(&s)[2][BN / 64][32] = reinterpret_cast<float(&)[2][BN / 64][32]>(raw);
+          if (A.cap > 0.0f) capped(reinterpret_cast<float(&)[BN]>(raw), to_cap, raw_cap);
+#pragma unroll
+          for (int a = 0; a < NA; a++)
+            if (a < A.axes) {
+#pragma unroll
+              for (int c = 0; c < BN / 64; c++)
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                  const F2 k2 = *reinterpret_cast<const F2*>(kp + a * BN + 64 * c + 8 * k + 2 * t4);
+#pragma unroll
+                  for (int R = 0; R < 4; R++) {
+                    float* x = &s[R >> 1][c][4 * k + 2 * (R & 1)];
+                    if constexpr (NEAR) {
+                      const float2 d = f2_unpack(f2_add(k2, f2_both(qf[R][a])));
+                      x[0] -= fabsf(d.x);
+                      x[1] -= fabsf(d.y);
+                    } else {
+                      const F2 d = f2_abs(f2_add(k2, f2_both(qf[R][a])));
+                      const float2 z = f2_unpack(f2_fma(d, f2_both(-slope[a]), f2_pack(x[0], x[1])));
+                      x[0] = z.x;
+                      x[1] = z.y;
+                    }
+                  }
+                }
+            }
+          if ((key_tile(t) + 1) * BN > open) {
+            const int j0 = key_tile(t) * BN + 2 * t4;
 #pragma unroll
             for (int c = 0; c < BN / 64; c++)
 #pragma unroll
-              for (int k = 0; k < 8; k++) {
-                const F2 k2 = *reinterpret_cast<const F2*>(kp + a * BN + 64 * c + 8 * k + 2 * t4);
+              for (int k = 0; k < 8; k++)
 #pragma unroll
-                for (int R = 0; R < 4; R++) {
-                  const float2 d = f2_unpack(f2_add(k2, f2_both(qf[R][a])));
-                  s[R >> 1][c][4 * k + 2 * (R & 1)] -= fabsf(d.x);
-                  s[R >> 1][c][4 * k + 2 * (R & 1) + 1] -= fabsf(d.y);
-                }
-              }
+                for (int R = 0; R < 4; R++)
+#pragma unroll
+                  for (int e = 0; e < 2; e++)
+                    if (j0 + 64 * c + 8 * k + e >= rseen[R]) s[R >> 1][c][4 * k + 2 * (R & 1) + e] = -INFINITY;
           }
-        if ((key_tile(t) + 1) * BN > open) {
-          const int j0 = key_tile(t) * BN + 2 * t4;
-#pragma unroll
-          for (int c = 0; c < BN / 64; c++)
-#pragma unroll
-            for (int k = 0; k < 8; k++)
-#pragma unroll
-              for (int R = 0; R < 4; R++)
-#pragma unroll
-                for (int e = 0; e < 2; e++)
-                  if (j0 + 64 * c + 8 * k + e >= rseen[R]) s[R >> 1][c][4 * k + 2 * (R & 1) + e] = -INFINITY;
-        }
-        float high[4];
-        bool more = false;
-#pragma unroll
-        for (int R = 0; R < 4; R++) {
-          float x = -INFINITY;
-#pragma unroll
-          for (int c = 0; c < BN / 64; c++)
-#pragma unroll
-            for (int k = 0; k < 8; k++)
-              x = max3(x, s[R >> 1][c][4 * k + 2 * (R & 1)], s[R >> 1][c][4 * k + 2 * (R & 1) + 1]);
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-          high[R] = x * unit;
-          if (t == 0) rm[R] = high[R];
-          more = more || high[R] > rm[R] + 8.0f;
-        }
-        if (t > 0 && __any_sync(0xffffffffu, more)) {
-          float keep[4], mine4 = 1.0f;
+          float high[4];
+          bool more = false;
 #pragma unroll
           for (int R = 0; R < 4; R++) {
-            const float next = fmaxf(rm[R], high[R]);
-            keep[R] = next == -INFINITY ? 1.0f : ex2(rm[R] - next);
-            rm[R] = next;
-            rl[R] *= keep[R];
-            const float x = __shfl_sync(0xffffffffu, keep[R], (lane & 7) * 4);
-            if (lane >> 3 == R) mine4 = x;
+            float x = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < BN / 64; c++)
+#pragma unroll
+              for (int k = 0; k < 8; k++)
+                x = max3(x, s[R >> 1][c][4 * k + 2 * (R & 1)], s[R >> 1][c][4 * k + 2 * (R & 1) + 1]);
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+            high[R] = x * unit;
+            if (t == 0) rm[R] = high[R];
+            more = more || high[R] > rm[R] + 8.0f;
           }
-          scale_outputs(t, mine4);
-        }
-        F2 base2[4], sum[4];
+          if (t > 0 && __any_sync(0xffffffffu, more)) {
+            float keep[4], mine4 = 1.0f;
 #pragma unroll
-        for (int R = 0; R < 4; R++) {
-          base2[R] = f2_both(rm[R] == -INFINITY ? 0.0f : -rm[R]);
-          sum[R] = 0;  // two zeros
-        }
-        my_turn(t);
-#pragma unroll
-        for (int x = 0; x < 2; x++)
-#pragma unroll
-          for (int c = 0; c < BN / 64; c++) {
-            uint32_t p[16];
-#pragma unroll
-            for (int k = 0; k < 16; k++) {
-              const int R = 2 * x + (k & 1);
-              const float2 z = f2_unpack(f2_fma(f2_pack(s[x][c][2 * k], s[x][c][2 * k + 1]), unit2, base2[R]));
-              const float2 y = make_float2(ex2(z.x), ex2(z.y));
-              sum[R] = f2_add(sum[R], f2_pack(y.x, y.y));
-              p[k] = pack2<T>(y.x, y.y);
+            for (int R = 0; R < 4; R++) {
+              const float next = fmaxf(rm[R], high[R]);
+              keep[R] = next == -INFINITY ? 1.0f : ex2(rm[R] - next);
+              rm[R] = next;
+              rl[R] *= keep[R];
+              const float x = __shfl_sync(0xffffffffu, keep[R], (lane & 7) * 4);
+              if (lane >> 3 == R) mine4 = x;
             }
-            tmem_st_frag(ts + ((uint32_t)x << 20) + c * 32, p);
+            scale_outputs(t, mine4);
           }
+          F2 base2[4], sum[4];
 #pragma unroll
-        for (int R = 0; R < 4; R++) {
-          const float2 total = f2_unpack(sum[R]);
-          rl[R] += total.x + total.y;
+          for (int R = 0; R < 4; R++) {
+            base2[R] = f2_both(rm[R] == -INFINITY ? 0.0f : -rm[R]);
+            sum[R] = 0;  // two zeros
+          }
+          my_turn(t);
+#pragma unroll
+          for (int x = 0; x < 2; x++)
+#pragma unroll
+            for (int c = 0; c < BN / 64; c++) {
+              uint32_t p[16];
+#pragma unroll
+              for (int k = 0; k < 16; k++) {
+                const int R = 2 * x + (k & 1);
+                const float2 z = f2_unpack(f2_fma(f2_pack(s[x][c][2 * k], s[x][c][2 * k + 1]), unit2, base2[R]));
+                const float2 y = make_float2(ex2(z.x), ex2(z.y));
+                sum[R] = f2_add(sum[R], f2_pack(y.x, y.y));
+                p[k] = pack2<T>(y.x, y.y);
+              }
+              tmem_st_frag(ts + ((uint32_t)x << 20) + c * 32, p);
+            }
+#pragma unroll
+          for (int R = 0; R < 4; R++) {
+            const float2 total = f2_unpack(sum[R]);
+            rl[R] += total.x + total.y;
+          }
+          turn_over();
+          weights_done(at.buffer);
         }
-        turn_over();
-        weights_done(at.buffer);
-      }
+      };
+      if (__builtin_expect(near, 1))
+        walk(std::true_type());
+      else
+        walk(std::false_type());
       // to the row of the lane
 #pragma unroll
       for (int R = 0; R < 4; R++) {

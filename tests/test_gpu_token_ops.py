@@ -492,6 +492,30 @@ def test_host_memory_is_refused():
         run_rotary(plan, "float16", [(P.q, P.keep["q"])], torch.zeros(1, 4, dtype=torch.int32, device="cuda"))
 
 
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("dim,axes", [(32, 2), (64, 1), (64, 3), (128, 1), (128, 3)])
+def test_attention_positions_far_apart_in_a_tile(dtype, dim, axes, kernel):
+    """Neighbouring queries anywhere in 2^23, a key at each one's place and one beside it: distances
+    are exact whatever the others' are. Tolerance: differences of positions below 2^24 are exact in 32
+    bits, so a bias is off by 2^-23 of itself, and those that count (0 and a few slopes) are below 4;
+    the products as in Problem; one rounding of the weights and one of the output."""
+    n, g = 200, gen(dim + axes)
+    P = Problem(dtype, dim, 2, 2, [n, n], [2 * n, 2 * n], axes=axes)
+    P.slopes = 0.5 + torch.rand(axes, 2, generator=g)
+    place = torch.randint(-2 ** 22, 2 ** 22, (axes, 2, n), generator=g)
+    step = torch.randint(0, 2, (axes, 2, n), generator=g)
+    P.q_pos = place.flatten(1).to(torch.int32)
+    P.kv_pos = torch.cat([place, place + step], 2).flatten(1).to(torch.int32)
+    out, lse, _, _ = P.expected()
+    got, sums = P.run()
+    size = (P.q.abs().double().amax((0, 1)) @ P.k.abs().double().amax((0, 1))) * P.scale
+    e, u = 2.0 ** -20 * (1 + size + 4), unit(dtype)
+    tiny = 2 * n * 2.0 ** -25 if dtype == "float16" else 0.0
+    tol = u * out.abs() + (u + 2 * e + tiny) * P.v.abs().max()
+    assert ((got.cpu().double() - out).abs() <= tol).all()
+    assert ((sums.cpu().double() - lse).abs() <= e + 2.0 ** -20).all()
+
+
 # ----------------------------------------------------------------------------- together
 @pytest.mark.parametrize("dtype", HALVES)
 def test_rotary_then_attention(dtype, kernel):
