@@ -41,6 +41,15 @@ s2s_heads plain_strides(s2s_heads x, int64_t tokens) {
   return x;
 }
 
+// guarded_free for calls that leave no CUDA error behind: one that is reported here would else be
+// found by the next look at the runtime's last error, another library's included.
+template <typename F>
+int guarded_call(F&& f) {
+  const int rc = guarded_free(f);
+  if (rc == S2S_ERR_CUDA) cudaGetLastError();
+  return rc;
+}
+
 // For the lifetime of the object the device that holds the tensors is the current one.
 // Every pointer has to be memory of that device, the stream one of its streams.
 class DeviceScope {

@@ -345,7 +345,7 @@ extern "C" {
 
 int s2s_masked_attention(const s2s_attention* a, void* stream) {
   using namespace s2s;
-  return guarded_free([&] {
+  return guarded_call([&] {
     const std::string me = "s2s_masked_attention: ";
     if (!a) fail(S2S_ERR_INVALID, me + "null argument");
     if (a->dtype != S2S_F16 && a->dtype != S2S_BF16)
@@ -435,7 +435,7 @@ int s2s_masked_attention(const s2s_attention* a, void* stream) {
 
 int s2s_device_status(int device) {
   using namespace s2s;
-  return guarded_free([&] {
+  return guarded_call([&] {
     int before = 0;
     ck(cudaGetDevice(&before), "cudaGetDevice");
     struct Restore {

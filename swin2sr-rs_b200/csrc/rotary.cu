@@ -177,7 +177,7 @@ int s2s_rotary_apply(const s2s_rotary* r, int dtype, int head_dim, int tokens, c
                      int64_t pos_stride, const s2s_heads* x, const s2s_heads* y, int n,
                      int inverse, void* stream) {
   using namespace s2s;
-  return guarded_free([&] {
+  return guarded_call([&] {
     const std::string me = "s2s_rotary_apply: ";
     if (!r || !x || !y) fail(S2S_ERR_INVALID, me + "null argument");
     if (dtype != S2S_F16 && dtype != S2S_BF16 && dtype != S2S_F32)

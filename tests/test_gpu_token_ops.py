@@ -482,6 +482,14 @@ def test_attention_in_streams_and_graphs(name, kernel):
     assert torch.equal(out, other)
 
 
+def test_a_refused_device_leaves_no_error_behind():
+    C = binding()
+    with pytest.raises(C.S2SError):
+        C.device_status(99)
+    x = torch.ones(4, device="cuda") + 1  # looks at the last error after its launch
+    assert x.sum().item() == 8
+
+
 def test_host_memory_is_refused():
     C = binding()
     P = Problem("float16", 64, 2, 2, [4], [4])
