@@ -314,7 +314,8 @@ int s2s_rotary_init(s2s_rotary* r, int axes, const int* sections, double base, i
                     int interleaved);
 
 /* y[i] = x[i] turned, for i < n (1..4; q and k in one launch), `dtype` any of the three,
- * any strides. y[i] may be x[i] itself; otherwise no output may overlap anything else.
+ * any strides (heads of an output within a token's row, or tokens within a head's). y[i] may be
+ * x[i] itself; otherwise no output may overlap anything else.
  * d_pos: int32 [axes][tokens], an axis's tokens contiguous, axes pos_stride apart. With
  * `inverse` the turn is undone (the transposed rotation: also its gradient). Angles are
  * reduced in 64 bits, products and sums are 32-bit, rounded once. */
@@ -334,7 +335,8 @@ int s2s_rotary_apply(const s2s_rotary* r, int dtype, int head_dim, int tokens, c
  * out_i = sum of softmax(z)_j v_j over the keys seen, d_lse = log sum exp(z) in fp32; a row
  * that sees no key (or only scores of minus infinity) gives zeros and minus infinity.
  * Values at keys that a row does not see never reach it, NaN and infinities included. Rows
- * of no document are left as they were. out and d_lse may not overlap each other or an
+ * of no document are left as they were. Heads of out lie within a token's row, or tokens within
+ * a head's. out and d_lse may not overlap each other or an
  * input. Two positions of a document lie less than 2^31 apart (distances are exact while the
  * queries' own positions lie less than 2^24 apart, else rounded to 2^-23 of that). The result of a call does not
  * depend on what else runs; a bounded wait that gives up (s2s_device_status) leaves it

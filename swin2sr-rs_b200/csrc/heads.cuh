@@ -28,6 +28,13 @@ void check_heads(const char* what, const s2s_heads& x, int64_t tokens, int head_
   };
   if (tokens > 1) stride("token_stride", x.token_stride);
   if (x.heads > 1) stride("head_stride", x.head_stride);
+  if (out && tokens > 1 && x.heads > 1) {
+    const bool inner = x.head_stride <= x.token_stride;  // the heads lie within a token's row
+    const int64_t small = inner ? x.head_stride : x.token_stride, n = inner ? x.heads : tokens;
+    const int64_t large = inner ? x.token_stride : x.head_stride;
+    if ((double)small * (n - 1) + head_dim > (double)large)
+      fail(S2S_ERR_INVALID, w + ": its rows run into one another");
+  }
   // the last element's offset has to be a 64-bit number of bytes with room to spare
   const double last = (double)(tokens - 1) * (double)(tokens > 1 ? x.token_stride : 0) +
                       (double)(x.heads - 1) * (double)(x.heads > 1 ? x.head_stride : 0) + head_dim;

@@ -388,6 +388,10 @@ int s2s_masked_attention(const s2s_attention* a, void* stream) {
     if (a->axes && (!a->d_slopes || !a->d_q_pos || (!a->d_kv_pos && a->kv_tokens)))
       fail(S2S_ERR_INVALID, me + "axes need d_slopes, d_q_pos and d_kv_pos");
     const bool keys = a->kv_tokens > 0;
+    const void *o = a->out.data, *sums = a->d_lse;
+    if (o == a->q.data || o == sums || (keys && (o == a->k.data || o == a->v.data)) ||
+        (sums && (sums == a->q.data || (keys && (sums == a->k.data || sums == a->v.data)))))
+      fail(S2S_ERR_INVALID, me + "out and d_lse may not be an input or one another");
     DeviceScope scope({{"s2s_masked_attention: q", a->q.data},
                        {"s2s_masked_attention: k", keys ? a->k.data : nullptr},
                        {"s2s_masked_attention: v", keys ? a->v.data : nullptr},

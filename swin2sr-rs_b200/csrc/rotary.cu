@@ -213,6 +213,15 @@ int s2s_rotary_apply(const s2s_rotary* r, int dtype, int head_dim, int tokens, c
                v.head_stride % vec == 0;
       heads += a.heads;
     }
+    if (tokens > 0)
+      for (int i = 0; i < n; i++)
+        for (int j = 0; j < n; j++) {
+          const RotaryTensor &a = A.t[i], &b = A.t[j];
+          if (i != j && (a.y == b.y || a.y == b.x))
+            fail(S2S_ERR_INVALID, me + "an output is another tensor of the call");
+          if (i == j && a.y == a.x && (a.yt != a.xt || a.yh != a.xh))
+            fail(S2S_ERR_INVALID, me + "in place, x and y must have the same strides");
+        }
     if (heads * head_dim > (1 << 26)) fail(S2S_ERR_INVALID, me + "too many heads");
     if (tokens == 0) return;
     if (!d_pos || (uintptr_t)d_pos % 4) fail(S2S_ERR_INVALID, me + "d_pos must be 4-byte aligned");

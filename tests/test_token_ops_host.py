@@ -110,6 +110,27 @@ def test_attention_refusals(change, text):
     refused(attention, text, **change)
 
 
+@pytest.mark.parametrize("tensors,text", [
+    ([((1, 64, 16, 4), (2, 63, 16, 4))], "run into"), ([((1, 64, 16, 4), (2, 16, 159, 4))], "run into"),
+    ([((1, 64, 16, 4), (2, 16, 16, 4))], "run into"),
+    ([((1, 64, 16, 4), (2, 64, 16, 4)), ((3, 64, 16, 4), (2, 64, 16, 4))], "another tensor"),
+    ([((1, 64, 16, 4), (2, 64, 16, 4)), ((2, 64, 16, 4), (3, 64, 16, 4))], "another tensor"),
+    ([((1, 64, 16, 4), (1, 128, 16, 4))], "same strides")])
+def test_rotary_outputs_over_other_tensors(tensors, text):
+    C = binding()
+    rows = [tuple(C.heads(ADDR * x[0], *x[1:]) for x in pair) for pair in tensors]
+    refused(C.rotary, text, C.rotary_plan([4, 4]), "float16", 16, 10, ADDR, 10, rows)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(out=(2 * ADDR, 120, 32, 4)), "run into"), (dict(out=(2 * ADDR, 32, 312, 4)), "run into"),
+    (dict(out=(ADDR, 128, 32, 4)), "one another"), (dict(out=(2 * ADDR, 128, 32, 4), d_lse=ADDR), "one another"),
+    (dict(out=(2 * ADDR, 128, 32, 4), d_lse=2 * ADDR), "one another"),
+    (dict(q=(3 * ADDR, 128, 32, 4), out=(ADDR, 128, 32, 4)), "one another")])
+def test_attention_outputs_over_other_tensors(change, text):
+    refused(attention, text, **change)
+
+
 def test_nothing_to_do_is_no_error():
     C = binding()
     attention(q_tokens=0, kv_tokens=0)
