@@ -351,7 +351,7 @@ typedef struct s2s_attention {
   const int* d_kv_offsets; /* [documents + 1]; NULL only together with d_q_offsets */
   const int* d_prefix;     /* [documents], causal only */
   float scale;             /* 1e-12 .. 1e12 */
-  float cap;               /* 0: none */
+  float cap;               /* 0: none, or 1e-12 .. 1e12 */
   int axes;                /* of the distance bias, 0: none */
   const float* d_slopes;   /* [axes][q heads] */
   const int* d_q_pos;      /* [axes][q_tokens] */

@@ -362,8 +362,8 @@ int s2s_masked_attention(const s2s_attention* a, void* stream) {
     if (a->d_prefix && !a->causal) fail(S2S_ERR_INVALID, me + "a prefix needs causal order");
     if (!(a->scale >= 1e-12f && a->scale <= 1e12f))
       fail(S2S_ERR_INVALID, me + "scale must be between 1e-12 and 1e12");
-    if (!(a->cap >= 0.0f) || !std::isfinite(a->cap))
-      fail(S2S_ERR_INVALID, me + "cap must be 0 or positive and finite");
+    if (a->cap != 0.0f && !(a->cap >= 1e-12f && a->cap <= 1e12f))  // cap / scale and its inverse
+      fail(S2S_ERR_INVALID, me + "cap must be 0 or between 1e-12 and 1e12");
     if (a->axes < 0 || a->axes > S2S_MAX_AXES)
       fail(S2S_ERR_INVALID, me + "axes must be 0.." + std::to_string(S2S_MAX_AXES));
     check_heads("s2s_masked_attention: q", a->q, a->q_tokens, a->head_dim, a->dtype, 8, false);

@@ -21,8 +21,8 @@
 // for 256 x 128 pairs, of 2900), beyond it the tensor core with its 64-key score products (2560 of
 // 3000). Measured (B200, non-causal, 37 heads, 4096 x 4096): 195 us at head 64, 811 TFLOP/s; 281 us
 // at head 128, 1130 TFLOP/s, 0.69 of the measured bf16 rate; causal 16384, eight heads of 128: 434-447
-// us, 1230 TFLOP/s. With a cap of 50: 331 and 398 us; with one axis of bias 288 and 372; with two
-// axes at head 64 334.
+// us, 1230 TFLOP/s. With a cap of 50: 331 and 398 us; with one axis of bias 303 and 372; with two
+// axes at head 64 351.
 #pragma once
 
 namespace s2s {

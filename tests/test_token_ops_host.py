@@ -25,6 +25,11 @@ def refused(fn, text, *args, **kw):
     assert e.value.code == C.S2S_ERR_INVALID and text in str(e.value), str(e.value)
 
 
+@pytest.mark.parametrize("cap", [1e-30, 9e-13, 1.1e12, 3e38])
+def test_caps_whose_quotients_leave_32_bits(cap):
+    refused(attention, "cap must be", cap=cap, scale=1e12 if cap < 1 else 1e-12)
+
+
 def test_rotary_plan_series_and_axes():
     C = binding()
     r = C.rotary_plan([2, 3, 1], 100.0)
