@@ -353,7 +353,7 @@ typedef struct s2s_attention {
   float scale;             /* 1e-12 .. 1e12 */
   float cap;               /* 0: none, or 1e-12 .. 1e12 */
   int axes;                /* of the distance bias, 0: none */
-  const float* d_slopes;   /* [axes][q heads] */
+  const float* d_slopes;   /* [axes][q heads]; sizes / scale below 3e38 */
   const int* d_q_pos;      /* [axes][q_tokens] */
   const int* d_kv_pos;     /* [axes][kv_tokens] */
   s2s_heads q, k, v, out;  /* 16-byte aligned, strides multiples of 8 elements */
