@@ -344,7 +344,7 @@ int s2s_rotary_apply(const s2s_rotary* r, int dtype, int head_dim, int tokens, c
 typedef struct s2s_attention {
   int dtype;     /* S2S_F16 or S2S_BF16, of q, k, v and out */
   int head_dim;  /* a multiple of 8, at most 128 */
-  int q_tokens, kv_tokens;
+  int q_tokens, kv_tokens; /* 2^31 - 256 at most, q's times (q.heads / k.heads) */
   int documents;
   int causal;
   const int* d_q_offsets;  /* [documents + 1] */

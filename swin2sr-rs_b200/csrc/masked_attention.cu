@@ -374,8 +374,11 @@ int s2s_masked_attention(const s2s_attention* a, void* stream) {
       fail(S2S_ERR_INVALID, me + "k and v, and q and out, must have the same heads, q's a "
                                  "multiple of k's");
     if (a->q.heads > 65535) fail(S2S_ERR_INVALID, me + "at most 65535 heads");
+    // what is added to a row's or a key's place (a tile at most) has to stay in 32 bits too
     if ((int64_t)a->q_tokens * (a->q.heads / a->k.heads) > 0x7fffff00)
       fail(S2S_ERR_INVALID, me + "q_tokens * (q heads / k heads) must stay below 2^31");
+    if (a->kv_tokens > 0x7fffff00)
+      fail(S2S_ERR_INVALID, me + "kv_tokens must be 2^31 - 256 at most");
     if (a->documents > 1 << 30) fail(S2S_ERR_INVALID, me + "at most 2^30 documents");
     for (const void* p : {(const void*)a->d_q_offsets, (const void*)a->d_kv_offsets,
                           (const void*)a->d_prefix, (const void*)a->d_slopes,
