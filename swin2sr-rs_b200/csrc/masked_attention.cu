@@ -10,7 +10,9 @@
 //   seen(i) = nk, or with causal order min(nk, max(prefix, i + 1 + nk - nq)).
 // Scores, maxima, sums and outputs are fp32 until the one rounding of o. The tile kernels hold
 // the scores as the products give them, caps and biases divided by `scale`; scale log2 e comes
-// in with the multiply-add in front of the exponential, which is one of base 2.
+// in with the difference to the row's maximum, in front of the exponential, which is one of base 2.
+// That difference is made before the product where scores may be large: a rounded product with the
+// maximum alone is off by 2^4 and more from scores of 2^28 on, out of the weights' and the sums' range.
 #include "heads.cuh"
 
 namespace s2s {

@@ -136,7 +136,7 @@ __device__ __forceinline__ uint32_t tile_at(int r, int b) {
 // its two rows. Whether one of them is NaN or infinite (in causal order, where it matters).
 template <typename T, int DN>
 __device__ __forceinline__ bool write_rows(const AttnArgs& A, int hk, const float (&o)[DN][4],
-                                           const float (&m)[2], const float (&l)[2], T* const (&op)[2],
+                                           const float (&m)[2], const float (&l)[2], float unit, T* const (&op)[2],
                                            const int (&row_q)[2], const int (&row_h)[2],
                                            const bool (&live)[2], int lane) {
   float check = 0.0f;
@@ -153,7 +153,7 @@ __device__ __forceinline__ bool write_rows(const AttnArgs& A, int hk, const floa
           *reinterpret_cast<uint32_t*>(op[e] + n * 8) = pack2<T>(o[n][2 * e] * inv, o[n][2 * e + 1] * inv);
       if ((lane & 3) == 0 && A.lse)
         A.lse[(int64_t)(hk * A.group + row_h[e]) * A.q_tokens + row_q[e]] =
-            none ? -INFINITY : (m[e] + log2f(l[e])) * kLn2;
+            none ? -INFINITY : fmaf(m[e], unit, log2f(l[e])) * kLn2;
     }
     if (A.causal)
 #pragma unroll
@@ -195,8 +195,8 @@ __device__ __forceinline__ void mend_rows(const AttnArgs& A, const Doc& D, int h
 template <typename T, int DP, int RW, int WARPS>
 __device__ __forceinline__ void join_rows(const AttnArgs& A, const Doc& D, int hk, uint8_t* smem,
                                           const float (&o)[DP / 8][4], const float (&m)[2],
-                                          const float (&l)[2], int r0, int nrows, int kend, int S,
-                                          int split) {
+                                          const float (&l)[2], float unit, int r0, int nrows, int kend,
+                                          int S, int split) {
   using C = MmaCfg<DP, RW, WARPS>;
   constexpr int KW = C::KW, DN = DP / 8;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
@@ -228,7 +228,7 @@ __device__ __forceinline__ void join_rows(const AttnArgs& A, const Doc& D, int h
 #pragma unroll
     for (int k = 0; k < KW; k++) {
       const float2 x = ml[(k * RW + w) * 16 + rr];
-      const float f = ex2(x.x - b);
+      const float f = ex2((x.x - b) * unit);
       const float4 v = *reinterpret_cast<const float4*>(part + ((k * RW + w) * 16 + rr) * C::LD + c);
       total += x.y * f;
       sum.x += v.x * f;
@@ -256,7 +256,7 @@ __device__ __forceinline__ void join_rows(const AttnArgs& A, const Doc& D, int h
       sum = make_float4(0, 0, 0, 0);
       total = 0.0f;
       for (int k = 0; k < S; k++) {
-        const float f = ex2(cluster_load(mla, k) - b);
+        const float f = ex2((cluster_load(mla, k) - b) * unit);
         const float4 v = cluster_load4(pa, k);
         total += cluster_load(mla + 4, k) * f;
         sum.x += v.x * f;
@@ -278,7 +278,7 @@ __device__ __forceinline__ void join_rows(const AttnArgs& A, const Doc& D, int h
       *reinterpret_cast<uint2*>(static_cast<T*>(A.out.data) + (int64_t)(D.q0 + i) * A.out.token +
                                 (int64_t)h * A.out.head + c) = make_uint2(pack2<T>(x.x, x.y), pack2<T>(x.z, x.w));
     if (c == 0 && A.lse)
-      A.lse[(int64_t)h * A.q_tokens + D.q0 + i] = none ? -INFINITY : (top + log2f(total)) * kLn2;
+      A.lse[(int64_t)h * A.q_tokens + D.q0 + i] = none ? -INFINITY : fmaf(top, unit, log2f(total)) * kLn2;
     if (!(fabsf(x.x) < INFINITY && fabsf(x.y) < INFINITY && fabsf(x.z) < INFINITY && fabsf(x.w) < INFINITY) &&
         seen(A, D, i) < kend)
       flag[r] = 1;
@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS, NA>::CTAS)
             for (int e = 0; e < 4; e++)
               if (j0 + n * 8 + 2 * t4 + (e & 1) >= row_seen[e >> 1]) s[n][e] = -INFINITY;
         }
-        // running maximum and sum
+        // running maximum (of the scores as they are) and sum
         float keep[2], base[2];
 #pragma unroll
         for (int e = 0; e < 2; e++) {
@@ -550,17 +550,17 @@ __global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS, NA>::CTAS)
           for (int n = 0; n < NT; n++) top = max3(top, s[n][2 * e], s[n][2 * e + 1]);
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          top = fmaxf(top * unit, m[e]);
+          top = fmaxf(top, m[e]);
           base[e] = top == -INFINITY ? 0.0f : top;  // a row that has seen nothing yet
-          keep[e] = ex2(m[e] - base[e]);
+          keep[e] = ex2((m[e] - base[e]) * unit);
           m[e] = top;
         }
         const F2 u2 = f2_both(unit), b0 = f2_both(-base[0]), b1 = f2_both(-base[1]);
         F2 sum0 = 0, sum1 = 0;  // two zeros each
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-          const float2 x = f2_unpack(f2_fma(f2_pack(s[n][0], s[n][1]), u2, b0));
-          const float2 y = f2_unpack(f2_fma(f2_pack(s[n][2], s[n][3]), u2, b1));
+          const float2 x = f2_unpack(f2_mul(f2_add(f2_pack(s[n][0], s[n][1]), b0), u2));
+          const float2 y = f2_unpack(f2_mul(f2_add(f2_pack(s[n][2], s[n][3]), b1), u2));
           s[n][0] = ex2(x.x);
           s[n][1] = ex2(x.y);
           s[n][2] = ex2(y.x);
@@ -607,9 +607,9 @@ __global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS, NA>::CTAS)
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
     }
     if (KW == 1 && S == 1)
-      mend |= write_rows<T, DN>(A, hk, o, m, l, op, row_q, row_h, live, lane);
+      mend |= write_rows<T, DN>(A, hk, o, m, l, unit, op, row_q, row_h, live, lane);
     else  // one head (cta_heads is 1)
-      join_rows<T, DP, RW, WARPS>(A, D, hk, smem, o, m, l, r0, nrows, kend, S, split);
+      join_rows<T, DP, RW, WARPS>(A, D, hk, smem, o, m, l, unit, r0, nrows, kend, S, split);
 #pragma unroll
     for (int e = 0; e < 2; e++) op[e] += (int64_t)A.group * A.out.head;
   }

@@ -179,6 +179,16 @@ __device__ __forceinline__ bool group_any(int id, bool x) {
   return y != 0;
 }
 
+// Weights are 2^(s unit - m unit), in one multiply-add behind the rounded m unit, which all weights of a
+// row share. Beyond this size (in either direction), where that rounding passes the 2^-12 that a score has
+// itself, m is taken off first. (For all rows: images 307 -> 325 us, causal 16384 511 -> 539 back to back.)
+constexpr float kLargeScore = 4096.0f;
+// What a row's exponents lose when its maximum grows from m to `next`.
+__device__ __forceinline__ float growth(float m, float next, float unit) {
+  const float a = m * unit, b = next * unit;
+  return fmaxf(fabsf(a), fabsf(b)) < kLargeScore ? a - b : (m - next) * unit;
+}
+
 // Where the products of key tile i and row tile w have their place: score buffer and the parity of
 // its use. Three buffers are taken in the order of the products, tile 0 and 1 in turn and at the
 // end the one that has more (n0, n1: their key tiles); of four each tile has two.
@@ -495,56 +505,86 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
     if constexpr (MODE < 2) {
       // a row a thread
-      for (int t = 0; t < n_w; t++) {
-        const Place at(w, t, n[0], n[1]);
-        const uint32_t ts = lanes + at.buffer * BN;
-        if (ok) ok = mbar_wait(&s_full[at.buffer], at.parity, DEV_TIMEOUT_ACC);
-        __syncwarp();
-        tc_fence_after();
-        uint32_t raw[BN / 32][32];
+      float base = 0.0f;  // of the exponents
+      bool some_large = false;
+      auto new_base = [&]() {
+        base = m == -INFINITY ? 0.0f : -m * unit;
+        const bool large = fabsf(base) >= kLargeScore;
+        if (large) base = 0.0f;
+        some_large = __any_sync(0xffffffffu, large);
+      };
+      // Tiles from t on, until all are done or, where rows with large maxima are not taken, the first
+      // such row; that tile is begun again (its scores are still there). A loop of its own, as the
+      // branch cost 511 -> 566 us in the one for all (causal 16384).
+      auto walk = [&](auto form, int t) {
+        constexpr bool LARGE = decltype(form)::value;
+        for (; t < n_w; t++) {
+          const Place at(w, t, n[0], n[1]);
+          const uint32_t ts = lanes + at.buffer * BN;
+          if (ok) ok = mbar_wait(&s_full[at.buffer], at.parity, DEV_TIMEOUT_ACC);
+          __syncwarp();
+          tc_fence_after();
+          uint32_t raw[BN / 32][32];
 #pragma unroll
-        for (int c = 0; c < BN / 32; c++) tmem_ld32_nw(ts + c * 32, raw[c]);
-        tc_wait_ld();
+          for (int c = 0; c < BN / 32; c++) tmem_ld32_nw(ts + c * 32, raw[c]);
+          tc_wait_ld();
 #pragma unroll
-        for (int c = 0; c < BN / 32; c++) loaded(raw[c]);
-        float(&s)[BN] = reinterpret_cast<float(&)[BN]>(raw);
-        if constexpr (MODE == 1) capped(s, to_cap, raw_cap);
-        if ((t + 1) * BN > open) {
-          const int last = mine - t * BN;
+          for (int c = 0; c < BN / 32; c++) loaded(raw[c]);
+          float(&s)[BN] = reinterpret_cast<float(&)[BN]>(raw);
+          if constexpr (MODE == 1) capped(s, to_cap, raw_cap);
+          if ((t + 1) * BN > open) {
+            const int last = mine - t * BN;
 #pragma unroll
-          for (int j = 0; j < BN; j++)
-            if (j >= last) s[j] = -INFINITY;
-        }
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int j = 0; j < BN; j += 2) top[(j >> 1) & 3] = max3(top[(j >> 1) & 3], s[j], s[j + 1]);
-        const float high = fmaxf(max3(top[0], top[1], top[2]), top[3]) * unit;
-        if (t == 0) {
-          m = high;
-        } else if (__any_sync(0xffffffffu, high > m + 8.0f)) {
-          const float next = fmaxf(m, high), keep = next == -INFINITY ? 1.0f : ex2(m - next);
-          m = next;
-          l *= keep;
-          scale_outputs(t, keep);
-        }
-        const F2 base2 = f2_both(m == -INFINITY ? 0.0f : -m);
-        F2 sum[2] = {0, 0};  // two zeros each
-#pragma unroll
-        for (int c = 0; c < BN / 64; c++) {
-          uint32_t p[32];
-#pragma unroll
-          for (int j = 0; j < 32; j++) {
-            const float2 x = f2_unpack(f2_fma(f2_pack(s[64 * c + 2 * j], s[64 * c + 2 * j + 1]), unit2, base2));
-            const float2 y = make_float2(ex2(x.x), ex2(x.y));
-            sum[j & 1] = f2_add(sum[j & 1], f2_pack(y.x, y.y));
-            p[j] = pack2<T>(y.x, y.y);
+            for (int j = 0; j < BN; j++)
+              if (j >= last) s[j] = -INFINITY;
           }
-          tmem_st32_nw(ts + c * 32, p);
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int j = 0; j < BN; j += 2) top[(j >> 1) & 3] = max3(top[(j >> 1) & 3], s[j], s[j + 1]);
+          const float high = fmaxf(max3(top[0], top[1], top[2]), top[3]);
+          if (t == 0) {
+            m = high;
+            new_base();
+            if (!LARGE && some_large) return t;
+          } else if (__any_sync(0xffffffffu, (high - m) * unit > 8.0f)) {
+            const float next = fmaxf(m, high), keep = next == -INFINITY ? 1.0f : ex2(growth(m, next, unit));
+            m = next;
+            l *= keep;
+            new_base();
+            scale_outputs(t, keep);
+            if (!LARGE && some_large) return t;
+          }
+          if constexpr (LARGE) {
+            const F2 shift = f2_both(base == 0.0f && m != -INFINITY ? -m : 0.0f);
+#pragma unroll
+            for (int j = 0; j < BN; j += 2) {
+              const float2 x = f2_unpack(f2_add(f2_pack(s[j], s[j + 1]), shift));
+              s[j] = x.x;
+              s[j + 1] = x.y;
+            }
+          }
+          const F2 base2 = f2_both(base);
+          F2 sum[2] = {0, 0};  // two zeros each
+#pragma unroll
+          for (int c = 0; c < BN / 64; c++) {
+            uint32_t p[32];
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+              const float2 x = f2_unpack(f2_fma(f2_pack(s[64 * c + 2 * j], s[64 * c + 2 * j + 1]), unit2, base2));
+              const float2 y = make_float2(ex2(x.x), ex2(x.y));
+              sum[j & 1] = f2_add(sum[j & 1], f2_pack(y.x, y.y));
+              p[j] = pack2<T>(y.x, y.y);
+            }
+            tmem_st32_nw(ts + c * 32, p);
+          }
+          const float2 total = f2_unpack(f2_add(sum[0], sum[1]));
+          l += total.x + total.y;
+          weights_done(at.buffer);
         }
-        const float2 total = f2_unpack(f2_add(sum[0], sum[1]));
-        l += total.x + total.y;
-        weights_done(at.buffer);
-      }
+        return t;
+      };
+      const int from = walk(std::false_type(), 0);
+      if (__builtin_expect(from < n_w, 0)) walk(std::true_type(), from);
     } else {
       // Four rows a thread, g + 8 R, and of each eight keys the two of the lane's place in its quad:
       // a key's positions then serve four scores. (With a row a thread every thread read all the
@@ -670,16 +710,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 x = max3(x, s[R >> 1][c][4 * k + 2 * (R & 1)], s[R >> 1][c][4 * k + 2 * (R & 1) + 1]);
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-            high[R] = x * unit;
+            high[R] = x;
             if (t == 0) rm[R] = high[R];
-            more = more || high[R] > rm[R] + 8.0f;
+            more = more || (high[R] - rm[R]) * unit > 8.0f;
           }
           if (t > 0 && __any_sync(0xffffffffu, more)) {
             float keep[4], mine4 = 1.0f;
 #pragma unroll
             for (int R = 0; R < 4; R++) {
               const float next = fmaxf(rm[R], high[R]);
-              keep[R] = next == -INFINITY ? 1.0f : ex2(rm[R] - next);
+              keep[R] = next == -INFINITY ? 1.0f : ex2(growth(rm[R], next, unit));
               rm[R] = next;
               rl[R] *= keep[R];
               const float x = __shfl_sync(0xffffffffu, keep[R], (lane & 7) * 4);
@@ -688,11 +728,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             scale_outputs(t, mine4);
           }
           F2 base2[4], sum[4];
+          bool large = false;
 #pragma unroll
           for (int R = 0; R < 4; R++) {
-            base2[R] = f2_both(rm[R] == -INFINITY ? 0.0f : -rm[R]);
+            const float base = rm[R] == -INFINITY ? 0.0f : -rm[R] * unit;
+            large = large || fabsf(base) >= kLargeScore;
+            base2[R] = f2_both(base);
             sum[R] = 0;  // two zeros
           }
+          if (__any_sync(0xffffffffu, large))
+#pragma unroll
+            for (int R = 0; R < 4; R++)
+              if (fabsf(f2_unpack(base2[R]).x) >= kLargeScore) {
+                base2[R] = 0;
+#pragma unroll
+                for (int c = 0; c < BN / 64; c++)
+#pragma unroll
+                  for (int k = 0; k < 8; k++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) s[R >> 1][c][4 * k + 2 * (R & 1) + e] -= rm[R];
+              }
           my_turn(t);
 #pragma unroll
           for (int x = 0; x < 2; x++)
@@ -760,7 +815,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       }
     if (live && A.lse)
-      A.lse[(int64_t)h * A.q_tokens + D.q0 + i] = none ? -INFINITY : (m + log2f(l)) * kLn2;
+      A.lse[(int64_t)h * A.q_tokens + D.q0 + i] = none ? -INFINITY : fmaf(m, unit, log2f(l)) * kLn2;
     // keys of the document that this row does not see had zero weights: a NaN or infinity among
     // their values shows here
     unsigned redo = __ballot_sync(0xffffffffu, check != 0.0f && live && mine < kmax);
