@@ -124,6 +124,13 @@ using F2 = unsigned long long;  // two fp32 lanes of the packed operations
 __device__ __forceinline__ F2 f2_both(float x) { return f2_pack(x, x); }
 __device__ __forceinline__ F2 f2_abs(F2 x) { return x & 0x7fffffff7fffffffull; }
 
+// log sum exp of a row from its largest score m and the sum l of its weights, which are 2^LIFT times
+// exp(z - m).
+template <int LIFT>
+__device__ __forceinline__ float log_sum(float m, float unit, float l) {
+  return fmaf(m, unit, log2f(l * (1.0f / (1 << LIFT)))) * kLn2;
+}
+
 // The larger and the smaller of three.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;

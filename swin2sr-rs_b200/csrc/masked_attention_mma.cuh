@@ -22,6 +22,12 @@ namespace {
 
 constexpr int kMmaStages = 3;
 
+// Weights are at most 2^kMmaLift: in fp16, whose least value is 2^-24, those down to 2^-39 of the largest
+// then count in the second product. (At most 1, the 65535 keys that share 0.2 % of a row's sum at 2^-25
+// each were lost.)
+template <typename T>
+constexpr int kMmaLift = std::is_same<T, __half>::value ? 15 : 0;
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
@@ -153,7 +159,7 @@ __device__ __forceinline__ bool write_rows(const AttnArgs& A, int hk, const floa
           *reinterpret_cast<uint32_t*>(op[e] + n * 8) = pack2<T>(o[n][2 * e] * inv, o[n][2 * e + 1] * inv);
       if ((lane & 3) == 0 && A.lse)
         A.lse[(int64_t)(hk * A.group + row_h[e]) * A.q_tokens + row_q[e]] =
-            none ? -INFINITY : fmaf(m[e], unit, log2f(l[e])) * kLn2;
+            none ? -INFINITY : log_sum<kMmaLift<T>>(m[e], unit, l[e]);
     }
     if (A.causal)
 #pragma unroll
@@ -278,7 +284,7 @@ __device__ __forceinline__ void join_rows(const AttnArgs& A, const Doc& D, int h
       *reinterpret_cast<uint2*>(static_cast<T*>(A.out.data) + (int64_t)(D.q0 + i) * A.out.token +
                                 (int64_t)h * A.out.head + c) = make_uint2(pack2<T>(x.x, x.y), pack2<T>(x.z, x.w));
     if (c == 0 && A.lse)
-      A.lse[(int64_t)h * A.q_tokens + D.q0 + i] = none ? -INFINITY : fmaf(top, unit, log2f(total)) * kLn2;
+      A.lse[(int64_t)h * A.q_tokens + D.q0 + i] = none ? -INFINITY : log_sum<kMmaLift<T>>(top, unit, total);
     if (!(fabsf(x.x) < INFINITY && fabsf(x.y) < INFINITY && fabsf(x.z) < INFINITY && fabsf(x.w) < INFINITY) &&
         seen(A, D, i) < kend)
       flag[r] = 1;
@@ -555,12 +561,12 @@ __global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS, NA>::CTAS)
           keep[e] = ex2((m[e] - base[e]) * unit);
           m[e] = top;
         }
-        const F2 u2 = f2_both(unit), b0 = f2_both(-base[0]), b1 = f2_both(-base[1]);
+        const F2 u2 = f2_both(unit), lift = f2_both(kMmaLift<T>), b0 = f2_both(-base[0]), b1 = f2_both(-base[1]);
         F2 sum0 = 0, sum1 = 0;  // two zeros each
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-          const float2 x = f2_unpack(f2_mul(f2_add(f2_pack(s[n][0], s[n][1]), b0), u2));
-          const float2 y = f2_unpack(f2_mul(f2_add(f2_pack(s[n][2], s[n][3]), b1), u2));
+          const float2 x = f2_unpack(f2_fma(f2_add(f2_pack(s[n][0], s[n][1]), b0), u2, lift));
+          const float2 y = f2_unpack(f2_fma(f2_add(f2_pack(s[n][2], s[n][3]), b1), u2, lift));
           s[n][0] = ex2(x.x);
           s[n][1] = ex2(x.y);
           s[n][2] = ex2(y.x);

@@ -14,8 +14,8 @@
 // cycles) waited for its own two products and they for it, 3200-3400 cycles a round.
 //
 // The output is scaled again only when a row's maximum grows by more than 2^8 beyond the one its
-// weights refer to (weights then stay below 2^8, in the range of both types, and the sums are
-// 32-bit), which after the first tiles is rare; the group does it itself.
+// weights refer to, which after the first tiles is rare; the group does it itself. Weights then stay
+// below 2^8, in fp16 with its lift (kTcLift) below 2^15, and the sums are 32-bit.
 //
 // Bound: for head_dim <= 64 the special function unit (16 exponentials a cycle and SM: 2048 cycles
 // for 256 x 128 pairs, of 2900), beyond it the tensor core with its 64-key score products (2560 of
@@ -183,6 +183,10 @@ __device__ __forceinline__ bool group_any(int id, bool x) {
 // row share. Beyond this size (in either direction), where that rounding passes the 2^-12 that a score has
 // itself, m is taken off first. (For all rows: images 307 -> 325 us, causal 16384 511 -> 539 back to back.)
 constexpr float kLargeScore = 4096.0f;
+// In fp16 weights are 2^7 times as large, so that those down to 2^-31 of the largest count in the second
+// product (its least value is 2^-24; see kMmaLift).
+template <typename T>
+constexpr float kTcLift = std::is_same<T, __half>::value ? 7.0f : 0.0f;
 // What a row's exponents lose when its maximum grows from m to `next`.
 __device__ __forceinline__ float growth(float m, float next, float unit) {
   const float a = m * unit, b = next * unit;
@@ -508,9 +512,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       float base = 0.0f;  // of the exponents
       bool some_large = false;
       auto new_base = [&]() {
-        base = m == -INFINITY ? 0.0f : -m * unit;
-        const bool large = fabsf(base) >= kLargeScore;
-        if (large) base = 0.0f;
+        const float b = m == -INFINITY ? 0.0f : m * unit;
+        const bool large = fabsf(b) >= kLargeScore;
+        base = kTcLift<T> - (large ? 0.0f : b);
         some_large = __any_sync(0xffffffffu, large);
       };
       // Tiles from t on, until all are done or, where rows with large maxima are not taken, the first
@@ -555,7 +559,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (!LARGE && some_large) return t;
           }
           if constexpr (LARGE) {
-            const F2 shift = f2_both(base == 0.0f && m != -INFINITY ? -m : 0.0f);
+            const F2 shift = f2_both(base == kTcLift<T> && m != -INFINITY ? -m : 0.0f);
 #pragma unroll
             for (int j = 0; j < BN; j += 2) {
               const float2 x = f2_unpack(f2_add(f2_pack(s[j], s[j + 1]), shift));
@@ -731,16 +735,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           bool large = false;
 #pragma unroll
           for (int R = 0; R < 4; R++) {
-            const float base = rm[R] == -INFINITY ? 0.0f : -rm[R] * unit;
-            large = large || fabsf(base) >= kLargeScore;
-            base2[R] = f2_both(base);
+            const float b = rm[R] == -INFINITY ? 0.0f : rm[R] * unit;
+            large = large || fabsf(b) >= kLargeScore;
+            base2[R] = f2_both(kTcLift<T> - b);
             sum[R] = 0;  // two zeros
           }
           if (__any_sync(0xffffffffu, large))
 #pragma unroll
             for (int R = 0; R < 4; R++)
-              if (fabsf(f2_unpack(base2[R]).x) >= kLargeScore) {
-                base2[R] = 0;
+              if (rm[R] != -INFINITY && fabsf(rm[R] * unit) >= kLargeScore) {
+                base2[R] = f2_both(kTcLift<T>);
 #pragma unroll
                 for (int c = 0; c < BN / 64; c++)
 #pragma unroll
@@ -815,7 +819,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       }
     if (live && A.lse)
-      A.lse[(int64_t)h * A.q_tokens + D.q0 + i] = none ? -INFINITY : fmaf(m, unit, log2f(l)) * kLn2;
+      A.lse[(int64_t)h * A.q_tokens + D.q0 + i] = none ? -INFINITY : log_sum<(int)kTcLift<T>>(m, unit, l);
     // keys of the document that this row does not see had zero weights: a NaN or infinity among
     // their values shows here
     unsigned redo = __ballot_sync(0xffffffffu, check != 0.0f && live && mine < kmax);

@@ -74,3 +74,31 @@ def test_attention_distances_of_any_size(far, dtype, kernel):
     P.q_pos[:] = far // 2
     P.kv_pos[:] = far // 2 - far
     check(P)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("low", [12.0, 17.5, 18.5])
+@pytest.mark.parametrize("q_lens,keys", [([1], 65536), ([3], 20000), ([130], 65536)])
+def test_attention_many_small_weights(q_lens, keys, low, dtype, kernel):
+    """One key far above very many that share a part of the sum: small as each weight is (2^-25 of the
+    largest and less), together they count. Weights of 16 bits are right to u of themselves, or in fp16
+    to 2^-25 where the largest is 2^15 (mma) or 2^7 (tcgen05); those of the keys here err alike. Sums are
+    32-bit, off by 2^-24 of themselves for each tile of 64 keys or more and for each key of it that a
+    thread has."""
+    P = Problem(dtype, 64, 1, 1, q_lens, [keys], scale=0.5)
+    P.q.zero_()
+    P.k.zero_()
+    P.q[..., 0] = 1.0
+    P.k[..., 0] = -2 * low  # exact in both types
+    P.k[77] = 0.0
+    P.v[:] = 1.0
+    P.v[77] = 0.0
+    out, lse = P.run()
+    o, w = P.expected()[:2]
+    rest = keys * math.exp(-low)
+    tol = 2 * unit(dtype) * o + 2.0 ** -19 * rest
+    if dtype == "float16":
+        tol += keys * 2.0 ** (-40 if kernel == "mma" else -32)
+    got = out.cpu().double()
+    assert ((got - o).abs() <= tol).all(), (float(got.min()), float(o.min()))
+    assert ((lse.cpu().double() - w).abs() <= 2.0 ** -19 + (keys // 64 + 64) * 2.0 ** -24).all()
