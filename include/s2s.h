@@ -337,10 +337,12 @@ int s2s_rotary_apply(const s2s_rotary* r, int dtype, int head_dim, int tokens, c
  * Values at keys that a row does not see never reach it, NaN and infinities included. Rows
  * of no document are left as they were. Heads of out lie within a token's row, or tokens within
  * a head's. out and d_lse may not overlap each other or an
- * input. Two positions of a document lie less than 2^31 apart (distances are exact while the
- * queries' own positions lie less than 2^24 apart, else rounded to 2^-23 of that). The result of a call does not
- * depend on what else runs; a bounded wait that gives up (s2s_device_status) leaves it
- * undefined. */
+ * input. Two positions of a document lie less than 2^31 apart. Positions count, in 32-bit
+ * floating point, from a query less than 256 queries away: a distance is rounded once where both
+ * of its positions lie less than 2^24 from that one's, and is right to 2^-22 of itself while such
+ * queries lie less than 2^23 apart; beyond that it is off by up to 2^-23 of what they do. The
+ * result of a call does not depend on what else runs; a bounded wait that gives up
+ * (s2s_device_status) leaves it undefined. */
 typedef struct s2s_attention {
   int dtype;     /* S2S_F16 or S2S_BF16, of q, k, v and out */
   int head_dim;  /* a multiple of 8, at most 128 */

@@ -167,18 +167,6 @@ __device__ __forceinline__ void fewer_registers() {
 __device__ __forceinline__ void group_sync(int id) {
   asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
 }
-// Whether x holds for any thread of the group.
-__device__ __forceinline__ bool group_any(int id, bool x) {
-  uint32_t y;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 128, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(y)
-      : "r"((uint32_t)x), "r"(id)
-      : "memory");
-  return y != 0;
-}
-
 // Weights are 2^(s unit - m unit), in one multiply-add behind the rounded m unit, which all weights of a
 // row share. Beyond this size (in either direction), where that rounding passes the 2^-12 that a score has
 // itself, m is taken off first. (For all rows: images 307 -> 325 us, causal 16384 511 -> 539 back to back.)
@@ -217,14 +205,14 @@ struct TcPlace {
   }
 };
 
-// MODE 0: no cap, no bias; 1: a cap; 2: a bias of one or two axes, 3: of three, with or without a cap.
+// MODE 0: no cap, no bias; 1: a cap; 1 + axes: a bias of one to three axes, with or without a cap.
 template <typename T, int NP, int MODE>
 __global__ void __launch_bounds__(kTcThreads, 1)
     k_attention_tc(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap mapQ,
                    const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV) {
   using C = TcCfg<NP>;
   constexpr int BN = C::BN, NB = C::NB, ST = C::STAGES;
-  constexpr int NA = MODE == 2 ? 2 : S2S_MAX_AXES;  // the most axes of a bias
+  constexpr int NA = MODE < 2 ? 1 : MODE - 1;  // axes of a bias
   using Place = TcPlace<NB>;
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ uint8_t smem_raw[];
@@ -594,16 +582,42 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // a key's positions then serve four scores. (With a row a thread every thread read all the
       // tile's positions, and shared memory was what bound it.)
       const int g = lane >> 2, t4 = lane & 3;
-      float rm[4], rl[4], qf[4][NA], slope[NA];
+      float rm[4], rl[4], qf[4][NA];
       int rseen[4], ref[NA], kraw[NA];
       float* pos = spos + w * 2 * S2S_MAX_AXES * BN;
+      // The bias as slope (|d| + sum of other axes' |ratio d|), the axis with the largest slope first:
+      // distances come from the positions' differences, exact where both are near the tile's first
+      // query, and each further axis costs two packed operations and an absolute addition. (As
+      // |slope q - slope k| neighbours would be off by the rounding of products that grow along the
+      // tile; the difference times each axis' slope took 333 us for the six images, this takes 303. One
+      // axis alone, 37 heads of 64 x 4096^2: 331 us, two 337, three 453.)
+      int axis[NA];
+      float slope = 0.0f, ratio[NA];
+#pragma unroll
+      for (int a = 0; a < NA; a++) axis[a] = a;
+#pragma unroll
+      for (int a = 0; a < NA; a++)
+        if (n_w > 0) {
+          ratio[a] = fabsf(A.slopes[a * A.q_heads + h]);
+          if (!(ratio[a] <= slope)) {
+            if (a > 0) {
+              ratio[a] = slope;
+              axis[a] = axis[0];
+              axis[0] = a;
+            }
+            slope = fabsf(A.slopes[a * A.q_heads + h]);
+          }
+        }
+#pragma unroll
+      for (int a = 1; a < NA; a++) ratio[a] = slope > 0.0f ? ratio[a] / slope : slope;
+      slope /= A.scale;
       // the positions of a tile's keys, each loaded a tile ahead by one thread
       auto key_positions = [&](int t) {
         const int j = key_tile(t) * BN + r;
         if (r < BN)
 #pragma unroll
           for (int a = 0; a < NA; a++)
-            if (a < A.axes) kraw[a] = j < D.nk ? A.kpos[(int64_t)a * A.kv_tokens + D.k0 + j] : ref[a];
+            kraw[a] = j < D.nk ? A.kpos[(int64_t)axis[a] * A.kv_tokens + D.k0 + j] : ref[a];
       };
 #pragma unroll
       for (int R = 0; R < 4; R++) {
@@ -612,44 +626,41 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         rl[R] = 0.0f;
         rseen[R] = x < rows_w ? seen(A, D, first + x) : 0;
       }
-      // |slope| |q - k| as |slope q - slope k|, one operation a pair less, while that is right: the
-      // rounding of slope q is below 2^-14 of a score's power of two. (All tiles in the other form: 325
-      // us for the six images of up to 4096 tokens; the choice costs 292 -> 304.)
-      bool near = true, far = false;
       if (n_w > 0) {
 #pragma unroll
-        for (int a = 0; a < NA; a++)
-          if (a < A.axes) {
-            const int* qa = A.qpos + (int64_t)a * A.q_tokens + D.q0;
-            ref[a] = qa[i0];
-            slope[a] = fabsf(A.slopes[a * A.q_heads + h]) / A.scale;
+        for (int a = 0; a < NA; a++) {
+          const int* qa = A.qpos + (int64_t)axis[a] * A.q_tokens + D.q0;
+          ref[a] = qa[i0];
 #pragma unroll
-            for (int R = 0; R < 4; R++) {
-              const int x = (warp & 3) * 32 + g + 8 * R;
-              qf[R][a] = -(float)(int)((unsigned)qa[x < rows_w ? first + x : i0] - (unsigned)ref[a]);
-              far |= fabsf(qf[R][a]) * slope[a] * unit >= 1024.0f;
-            }
+          for (int R = 0; R < 4; R++) {
+            const int x = (warp & 3) * 32 + g + 8 * R;
+            qf[R][a] = -(float)(int)((unsigned)qa[x < rows_w ? first + x : i0] - (unsigned)ref[a]);
           }
-        near = !group_any(1 + w, far);
-        if (near)
-#pragma unroll
-          for (int a = 0; a < NA; a++)
-#pragma unroll
-            for (int R = 0; R < 4; R++) qf[R][a] *= a < A.axes ? slope[a] : 1.0f;
+        }
         key_positions(0);
       }
-      auto walk = [&](auto form) {
-        constexpr bool NEAR = decltype(form)::value;
-        for (int t = 0; t < n_w; t++) {
+      bool some_large = false;
+      auto look_for_large = [&]() {
+        bool large = false;
+#pragma unroll
+        for (int R = 0; R < 4; R++) large = large || (rm[R] != -INFINITY && fabsf(rm[R] * unit) >= kLargeScore);
+        some_large = __any_sync(0xffffffffu, large);
+      };
+      auto walk = [&](auto form, const int from) {  // as above
+        constexpr bool LARGE = decltype(form)::value;
+        int t = from;
+        for (; t < n_w; t++) {
           const Place at(w, t, n[0], n[1]);
           const uint32_t ts = lanes + at.buffer * BN;
           float* kp = pos + (t & 1) * S2S_MAX_AXES * BN;
-          if (r < BN)
+          if (!LARGE || t > from) {  // of a tile that is begun again they are there
+            if (r < BN)
 #pragma unroll
-            for (int a = 0; a < NA; a++)
-              if (a < A.axes) kp[a * BN + r] = (NEAR ? slope[a] : 1.0f) * (float)(int)((unsigned)kraw[a] - (unsigned)ref[a]);
-          group_sync(1 + w);
-          if (t + 1 < n_w) key_positions(t + 1);
+              for (int a = 0; a < NA; a++)
+                kp[a * BN + r] = (float)(int)((unsigned)kraw[a] - (unsigned)ref[a]);
+            group_sync(1 + w);
+            if (t + 1 < n_w) key_positions(t + 1);
+          }
           if (ok) ok = mbar_wait(&s_full[at.buffer], at.parity, DEV_TIMEOUT_ACC);
           __syncwarp();
           tc_fence_after();
@@ -666,29 +677,36 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             for (int c = 0; c < BN / 64; c++) loaded(raw[x][c]);
           float(&s)[2][BN / 64][32] = reinterpret_cast<float(&)[2][BN / 64][32]>(raw);
           if (A.cap > 0.0f) capped(reinterpret_cast<float(&)[BN]>(raw), to_cap, raw_cap);
+          const F2 by = f2_both(NA > 1 ? -slope : slope);
 #pragma unroll
-          for (int a = 0; a < NA; a++)
-            if (a < A.axes) {
+          for (int c = 0; c < BN / 64; c++)
 #pragma unroll
-              for (int c = 0; c < BN / 64; c++)
+            for (int k = 0; k < 8; k++) {
+              F2 k2[NA];
 #pragma unroll
-                for (int k = 0; k < 8; k++) {
-                  const F2 k2 = *reinterpret_cast<const F2*>(kp + a * BN + 64 * c + 8 * k + 2 * t4);
+              for (int a = 0; a < NA; a++)
+                k2[a] = *reinterpret_cast<const F2*>(kp + a * BN + 64 * c + 8 * k + 2 * t4);
 #pragma unroll
-                  for (int R = 0; R < 4; R++) {
-                    float* x = &s[R >> 1][c][4 * k + 2 * (R & 1)];
-                    if constexpr (NEAR) {
-                      const float2 d = f2_unpack(f2_add(k2, f2_both(qf[R][a])));
-                      x[0] -= fabsf(d.x);
-                      x[1] -= fabsf(d.y);
-                    } else {
-                      const F2 d = f2_abs(f2_add(k2, f2_both(qf[R][a])));
-                      const float2 z = f2_unpack(f2_fma(d, f2_both(-slope[a]), f2_pack(x[0], x[1])));
-                      x[0] = z.x;
-                      x[1] = z.y;
-                    }
+              for (int R = 0; R < 4; R++) {
+                float* x = &s[R >> 1][c][4 * k + 2 * (R & 1)];
+                if constexpr (NA == 1) {
+                  const float2 d = f2_unpack(f2_mul(f2_add(k2[0], f2_both(qf[R][0])), by));
+                  const float2 e = f2_unpack(f2_add(f2_pack(x[0], x[1]), f2_pack(-fabsf(d.x), -fabsf(d.y))));
+                  x[0] = e.x;
+                  x[1] = e.y;
+                } else {
+                  float2 d = f2_unpack(f2_add(k2[0], f2_both(qf[R][0])));
+#pragma unroll
+                  for (int a = 1; a < NA; a++) {
+                    const float2 y = f2_unpack(f2_mul(f2_add(k2[a], f2_both(qf[R][a])), f2_both(ratio[a])));
+                    d.x = fabsf(d.x) + fabsf(y.x);
+                    d.y = fabsf(d.y) + fabsf(y.y);
                   }
+                  const float2 z = f2_unpack(f2_fma(f2_pack(d.x, d.y), by, f2_pack(x[0], x[1])));
+                  x[0] = z.x;
+                  x[1] = z.y;
                 }
+              }
             }
           if ((key_tile(t) + 1) * BN > open) {
             const int j0 = key_tile(t) * BN + 2 * t4;
@@ -718,7 +736,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (t == 0) rm[R] = high[R];
             more = more || (high[R] - rm[R]) * unit > 8.0f;
           }
-          if (t > 0 && __any_sync(0xffffffffu, more)) {
+          if (t == 0) {
+            look_for_large();
+            if (!LARGE && some_large) return t;
+          } else if (__any_sync(0xffffffffu, more)) {
             float keep[4], mine4 = 1.0f;
 #pragma unroll
             for (int R = 0; R < 4; R++) {
@@ -729,21 +750,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               const float x = __shfl_sync(0xffffffffu, keep[R], (lane & 7) * 4);
               if (lane >> 3 == R) mine4 = x;
             }
+            look_for_large();
             scale_outputs(t, mine4);
+            if (!LARGE && some_large) return t;
           }
           F2 base2[4], sum[4];
-          bool large = false;
 #pragma unroll
           for (int R = 0; R < 4; R++) {
             const float b = rm[R] == -INFINITY ? 0.0f : rm[R] * unit;
-            large = large || fabsf(b) >= kLargeScore;
             base2[R] = f2_both(kTcLift<T> - b);
             sum[R] = 0;  // two zeros
-          }
-          if (__any_sync(0xffffffffu, large))
-#pragma unroll
-            for (int R = 0; R < 4; R++)
-              if (rm[R] != -INFINITY && fabsf(rm[R] * unit) >= kLargeScore) {
+            if constexpr (LARGE)
+              if (fabsf(b) >= kLargeScore) {
                 base2[R] = f2_both(kTcLift<T>);
 #pragma unroll
                 for (int c = 0; c < BN / 64; c++)
@@ -752,6 +770,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                     for (int e = 0; e < 2; e++) s[R >> 1][c][4 * k + 2 * (R & 1) + e] -= rm[R];
               }
+          }
           my_turn(t);
 #pragma unroll
           for (int x = 0; x < 2; x++)
@@ -776,11 +795,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           turn_over();
           weights_done(at.buffer);
         }
+        return t;
       };
-      if (__builtin_expect(near, 1))
-        walk(std::true_type());
-      else
-        walk(std::false_type());
+      const int from = walk(std::false_type(), 0);
+      if (__builtin_expect(from < n_w, 0)) walk(std::true_type(), from);
       // to the row of the lane
 #pragma unroll
       for (int R = 0; R < 4; R++) {
@@ -859,11 +877,13 @@ cudaError_t launch_attention_tc(AttnArgs& A, cudaStream_t st) {
 template <typename T>
 cudaError_t launch_attention_tc(AttnArgs& A, cudaStream_t st) {
   if (A.head_dim <= 64)
-    return A.axes > 2     ? launch_attention_tc<T, 1, 3>(A, st)
+    return A.axes > 2     ? launch_attention_tc<T, 1, 4>(A, st)
+           : A.axes > 1   ? launch_attention_tc<T, 1, 3>(A, st)
            : A.axes       ? launch_attention_tc<T, 1, 2>(A, st)
            : A.cap > 0.0f ? launch_attention_tc<T, 1, 1>(A, st)
                           : launch_attention_tc<T, 1, 0>(A, st);
-  return A.axes > 2     ? launch_attention_tc<T, 2, 3>(A, st)
+  return A.axes > 2     ? launch_attention_tc<T, 2, 4>(A, st)
+         : A.axes > 1   ? launch_attention_tc<T, 2, 3>(A, st)
          : A.axes       ? launch_attention_tc<T, 2, 2>(A, st)
          : A.cap > 0.0f ? launch_attention_tc<T, 2, 1>(A, st)
                         : launch_attention_tc<T, 2, 0>(A, st);

@@ -102,3 +102,47 @@ def test_attention_many_small_weights(q_lens, keys, low, dtype, kernel):
     got = out.cpu().double()
     assert ((got - o).abs() <= tol).all(), (float(got.min()), float(o.min()))
     assert ((lse.cpu().double() - w).abs() <= 2.0 ** -19 + (keys // 64 + 64) * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("dim,axes", [(64, 1), (64, 2), (128, 1), (128, 3)])
+@pytest.mark.parametrize("span", [40, 700, 2000, 30000])
+def test_attention_bias_between_neighbours(span, dim, axes, dtype, kernel):
+    """Queries spread over a tile, each with a key at its place or beside it, at slopes whose products
+    with the positions have no room in 32 bits: the bias is the distance's, not a difference of such
+    products. Scores are zero, so a bias is off by 2^-23 of itself, and those that count are below 4."""
+    n, g = 256, torch.Generator().manual_seed(span + dim)
+    P = Problem(dtype, dim, 2, 2, [n], [n], axes=axes)
+    P.q.zero_()
+    P.slopes = 0.7 + 0.1 * torch.rand(axes, 2, generator=g)
+    P.q_pos = torch.randint(0, span, (axes, n), generator=g).to(torch.int32)
+    P.kv_pos = P.q_pos + torch.randint(0, 2, (axes, n), generator=g).to(torch.int32)
+    out, lse = P.run()
+    o, w = P.expected()[:2]
+    u, big = unit(dtype), P.v.abs().max().double()
+    e = 2.0 ** -20  # of a score: the bias, its sum with the others, the exponential
+    assert ((lse.cpu().double() - w).abs() <= 2 * e).all(), float((lse.cpu().double() - w).abs().max())
+    assert ((out.cpu().double() - o).abs() <= u * o.abs() + (u + 2 * e + n * 2.0 ** -25) * big).all()
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("dim,axes", [(64, 1), (64, 2), (128, 3)])
+@pytest.mark.parametrize("reach", [2 ** 24 + 1, 2 ** 27 + 3, 2 ** 30 + 7])
+def test_attention_keys_far_from_queries_that_are_apart(reach, dim, axes, dtype, kernel):
+    """Queries anywhere in 2^23, keys up to `reach` from there, some beside a query: distances are right to
+    2^-22 of themselves, and the bias with its slope's and its own rounding to 2^-21. Scores are zero."""
+    n, g = 200, torch.Generator().manual_seed(reach % 1000 + axes)
+    P = Problem(dtype, dim, 2, 2, [n, 1], [n, 1], axes=axes)
+    P.q.zero_()
+    P.slopes = 2.0 ** 4 / reach * (0.5 + torch.rand(axes, 2, generator=g))
+    P.q_pos = torch.randint(0, 2 ** 23, (axes, n + 1), generator=g).to(torch.int32)
+    P.q_pos[:, :2] = torch.tensor([0, 2 ** 23 - 1])
+    P.kv_pos = torch.randint(-reach, reach + 1, (axes, n + 1), generator=g).to(torch.int32)
+    P.kv_pos[:, ::3] = P.q_pos[:, ::3] + 2
+    P.kv_pos[:, -1] = reach
+    out, lse = P.run()
+    o, w = P.expected()[:2]
+    u, big = unit(dtype), P.v.abs().max().double()
+    e = axes * 24 * 1.5 * 2.0 ** -21 + 2.0 ** -20  # slopes times distances are below 24 times 1.5 an axis
+    assert ((lse.cpu().double() - w).abs() <= 2 * e).all(), float((lse.cpu().double() - w).abs().max())
+    assert ((out.cpu().double() - o).abs() <= u * o.abs() + (u + 2 * e + n * 2.0 ** -25) * big).all()
