@@ -144,24 +144,25 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
 }
 
 // Capped scores, divided by the scale: s -> raw_cap tanh(s to_cap), where raw_cap to_cap = 1. For
-// arguments up to 1, tanh x = x P(x^2) with P the polynomial of least relative error on [0, 1] of
-// degree 6 (5e-8, by the exchange algorithm), up to 0.35 of degree 3 (3.5e-8); beyond 1,
-// 1 - 2 / (1 + e^{2x}). A warp takes the shortest form that is enough for all its scores: caps are
-// there for the exception, and the special function unit is busy with the exponentials.
+// arguments up to 1, tanh x = x (1 + x^2 Q(x^2)) with Q of least relative error of the whole on [0, 1],
+// six coefficients (5.7e-8 as they are rounded, by the exchange algorithm and a search of the last bits),
+// up to 0.35 three (4.1e-8); with the roundings of its evaluation 1.7e-7. Where x^2 is below 2^-24 that is x
+// itself. Beyond 1, 1 - 2 / (1 + e^{2x}). A warp takes the shortest form that is enough for all its scores:
+// caps are there for the exception, and the special function unit is busy with the exponentials.
 template <int DEGREE>
 __device__ __forceinline__ F2 tanh_over_x(F2 u) {
   F2 p;
   if (DEGREE == 6) {
-    p = f2_fma(f2_both(0.0010410225950181484f), u, f2_both(-0.006203379016369581f));
-    p = f2_fma(p, u, f2_both(0.020289979875087738f));
-    p = f2_fma(p, u, f2_both(-0.05345702916383743f));
-    p = f2_fma(p, u, f2_both(0.13325203955173492f));
-    p = f2_fma(p, u, f2_both(-0.33332839608192444f));
+    p = f2_fma(f2_both(0.0010582684772089124f), u, f2_both(-0.006259354762732983f));
+    p = f2_fma(p, u, f2_both(0.020359782502055168f));
+    p = f2_fma(p, u, f2_both(-0.053498707711696625f));
+    p = f2_fma(p, u, f2_both(0.13326406478881836f));
+    p = f2_fma(p, u, f2_both(-0.33332985639572144f));
   } else {
-    p = f2_fma(f2_both(-0.04895823076367378f), u, f2_both(0.13295799493789673f));
-    p = f2_fma(p, u, f2_both(-0.33332422375679016f));
+    p = f2_fma(f2_both(-0.04914923757314682f), u, f2_both(0.13299839198589325f));
+    p = f2_fma(p, u, f2_both(-0.33332663774490356f));
   }
-  return f2_fma(p, u, f2_both(0.9999999403953552f));
+  return f2_fma(p, u, f2_both(1.0f));
 }
 __device__ __forceinline__ float tanh_far(float x, float near) {
   float r;

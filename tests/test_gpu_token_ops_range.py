@@ -146,3 +146,13 @@ def test_attention_keys_far_from_queries_that_are_apart(reach, dim, axes, dtype,
     e = axes * 24 * 1.5 * 2.0 ** -21 + 2.0 ** -20  # slopes times distances are below 24 times 1.5 an axis
     assert ((lse.cpu().double() - w).abs() <= 2 * e).all(), float((lse.cpu().double() - w).abs().max())
     assert ((out.cpu().double() - o).abs() <= u * o.abs() + (u + 2 * e + n * 2.0 ** -25) * big).all()
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("dim,axes", [(32, 0), (64, 0), (64, 1), (128, 0), (128, 2)])
+def test_attention_a_cap_far_above_the_scores_changes_nothing(dim, axes, dtype, kernel):
+    """tanh x / x is 1 in 32 bits below 2^-12, so the outputs have the bits of a call without a cap."""
+    more = dict(causal=True, axes=axes)
+    plain, sums = Problem(dtype, dim, 4, 2, [300, 40], [300, 700], **more).run()
+    out, lse = Problem(dtype, dim, 4, 2, [300, 40], [300, 700], cap=2.0 ** 20, **more).run()
+    assert torch.equal(lse, sums) and torch.equal(out, plain)
