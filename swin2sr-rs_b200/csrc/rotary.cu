@@ -122,7 +122,8 @@ __global__ void __launch_bounds__(kRotaryThreads) k_rotary(const __grid_constant
 
 template <typename T, int VEC>
 cudaError_t launch_rotary(const RotaryArgs& A, bool interleaved, cudaStream_t st) {
-  const dim3 grid((unsigned)((A.tokens + A.per_cta - 1) / A.per_cta)), block(kRotaryThreads);
+  // in 64 bits: tokens go up to 2^31 - 1
+  const dim3 grid((unsigned)(((long long)A.tokens + A.per_cta - 1) / A.per_cta)), block(kRotaryThreads);
   return interleaved ? launch_pdl(k_rotary<T, VEC, true>, grid, block, 0, st, A)
                      : launch_pdl(k_rotary<T, VEC, false>, grid, block, 0, st, A);
 }
