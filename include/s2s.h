@@ -151,6 +151,12 @@ int64_t s2s_debug_read(s2s_handle* h, const char* buffer, float* host, int64_t c
  * S2S_ERR_TIMEOUT, and the handle stays usable. */
 int s2s_debug_halo_loopback(s2s_handle* h, int rows, int missing);
 
+/* Diagnostics of the masked attention's loads, on the host: the order in which a CTA of its
+ * tcgen05 kernel copies the key and value tiles of `tiles` steps, where the wait for a stage
+ * gives up after `waits` of them. copies[2 i] is key tile i, copies[2 i + 1] value tile i:
+ * 0 never copied, 1 copied, 2 its stage was waited for, 3 waited for at the end. */
+int s2s_debug_attention_loads(int tiles, int waits, int* copies);
+
 /* ---- Row-band sharding of one image across GPUs. No counterpart in the
  * reference, which runs an image on one GPU (src/gpu.rs:462-583 is the forward
  * each band repeats). The padded plane's window rows are split into contiguous

@@ -32,7 +32,8 @@ EXPORTS = ("s2s_create", "s2s_forward", "s2s_forward_batch", "s2s_forward_device
            "s2s_band_partition", "s2s_band_halo_ops", "s2s_png_header", "s2s_png_decode",
            "s2s_png_encode_rgb8", "s2s_png_encode_rows", "s2s_free", "s2s_adjust_device",
            "s2s_rgb8_device", "s2s_forward_image", "s2s_selftest", "s2s_rotary_init",
-           "s2s_rotary_apply", "s2s_masked_attention", "s2s_device_status")
+           "s2s_rotary_apply", "s2s_masked_attention", "s2s_device_status",
+           "s2s_debug_attention_loads")
 BAND_ID_BYTES = 128
 MAX_AXES, ROTARY_MAX_PAIRS = 3, 128
 # element types of the token operators
@@ -180,6 +181,8 @@ def load() -> ctypes.CDLL:
     L.s2s_masked_attention.restype = ctypes.c_int
     L.s2s_device_status.argtypes = [ctypes.c_int]
     L.s2s_device_status.restype = ctypes.c_int
+    L.s2s_debug_attention_loads.argtypes = [ctypes.c_int, ctypes.c_int, ip]
+    L.s2s_debug_attention_loads.restype = ctypes.c_int
     L.s2s_version.argtypes = []
     L.s2s_version.restype = ctypes.c_char_p
     _lib = L
@@ -535,6 +538,14 @@ def attention(dtype: str, head_dim: int, scale: float, q: S2SHeads, k: S2SHeads,
                      d_q_offsets, d_kv_offsets, d_prefix, scale, cap, axes, d_slopes, d_q_pos,
                      d_kv_pos, q, k, v, out, d_lse)
     _fail(L, L.s2s_masked_attention(a, stream or None))
+
+
+def debug_attention_loads(tiles: int, waits: int) -> list:
+    """s2s_debug_attention_loads: what becomes of each key and value copy, in turn."""
+    L = load()
+    copies = (ctypes.c_int * (2 * tiles))()
+    _fail(L, L.s2s_debug_attention_loads(tiles, waits, copies))
+    return list(copies)
 
 
 def device_status(device: int = 0) -> None:

@@ -450,6 +450,24 @@ int s2s_masked_attention(const s2s_attention* a, void* stream) {
   });
 }
 
+int s2s_debug_attention_loads(int tiles, int waits, int* copies) {
+  using namespace s2s;
+  return guarded_call([&] {
+    if (tiles < 0 || !copies) fail(S2S_ERR_INVALID, "s2s_debug_attention_loads: null argument");
+    memset(copies, 0, 2 * (size_t)tiles * sizeof(int));
+    constexpr int ST = TcCfg<1>::STAGES;
+    load_tiles<ST>(
+        tiles,
+        [&](bool value, int i) {
+          if (waits-- <= 0) return false;
+          copies[2 * (i - ST) + value] = 2;
+          return true;
+        },
+        [&](bool value, int i) { copies[2 * i + value] = 1; },
+        [&](bool value, int i) { copies[2 * i + value] += 2; });
+  });
+}
+
 int s2s_device_status(int device) {
   using namespace s2s;
   return guarded_call([&] {

@@ -205,6 +205,23 @@ struct TcPlace {
   }
 };
 
+// The loader's schedule: key and value tiles in turn through rings of STAGES each, `released` a wait for
+// the stage of an earlier tile, which may give up. At the end every copy that its stage's next tile did
+// not wait for is waited for, also then: none is in flight when the CTA ends.
+#pragma nv_exec_check_disable
+template <int STAGES, typename Released, typename Copy, typename Landed>
+__host__ __device__ __forceinline__ void load_tiles(int tiles, Released&& released, Copy&& copy, Landed&& landed) {
+  int n[2] = {0, 0};  // copies of keys, of values
+  for (int i = 0; i < 2 * tiles; i++) {
+    const bool value = i & 1;
+    if (i / 2 >= STAGES && !released(value, i / 2)) break;
+    copy(value, i / 2);
+    n[i & 1]++;
+  }
+  for (int v = 0; v < 2; v++)
+    for (int i = n[v] > STAGES ? n[v] - STAGES : 0; i < n[v]; i++) landed(v == 1, i);
+}
+
 // MODE 0: no cap, no bias; 1: a cap; 1 + axes: a bias of one to three axes, with or without a cap.
 template <typename T, int NP, int MODE>
 __global__ void __launch_bounds__(kTcThreads, 1)
@@ -308,27 +325,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int p = 0; p < NP; p++) tma_load_3d(dst + p * (bytes / NP), map, bar, p * 64, head, row);
       };
       const int N = max(n[0], n[1]);
-      bool ok = true;
-      int i = 0;
-      for (; i < N && ok; i++) {
-        const int s = i % ST;
-        if (i >= ST) ok = mbar_wait(&k_empty[s], ((i / ST) - 1) & 1, DEV_TIMEOUT_EMPTY);
-        if (!ok) break;
-        load(kring + s * C::KB, C::KB, &mapK, &k_full[s], hk, D.k0 + key_tile(i) * BN);
-        if (i == 0)
-          for (int w = 0; w < 2; w++)
-            if (n[w] > 0) load(sQ + w * C::QB, C::QB, &mapQ, &q_full[w], h, D.q0 + i0 + w * kTcTile);
-        if (i >= ST) ok = mbar_wait(&v_empty[s], ((i / ST) - 1) & 1, DEV_TIMEOUT_EMPTY);
-        if (ok) load(vring + s * C::KB, C::KB, &mapV, &v_full[s], hk, D.k0 + key_tile(i) * BN);
-      }
-      // no copy is in flight when the CTA ends, also where a wait gave up
-      if (N > 0)
-        for (int w = 0; w < 2; w++)
-          if (n[w] > 0) wait_landed(&q_full[w], 0);
-      for (int k = max(0, i - ST); k < i; k++) {
-        wait_landed(&k_full[k % ST], (k / ST) & 1);
-        if (ok || k < i - 1) wait_landed(&v_full[k % ST], (k / ST) & 1);
-      }
+      auto bar = [&](bool value, int i, bool full) {
+        return (full ? value ? v_full : k_full : value ? v_empty : k_empty) + i % ST;
+      };
+      load_tiles<ST>(
+          N, [&](bool value, int i) { return mbar_wait(bar(value, i, false), ((i / ST) - 1) & 1, DEV_TIMEOUT_EMPTY); },
+          [&](bool value, int i) {
+            load((value ? vring : kring) + i % ST * C::KB, C::KB, value ? &mapV : &mapK, bar(value, i, true), hk,
+                 D.k0 + key_tile(i) * BN);
+            if (i == 0 && !value)
+              for (int w = 0; w < 2; w++)
+                if (n[w] > 0) load(sQ + w * C::QB, C::QB, &mapQ, &q_full[w], h, D.q0 + i0 + w * kTcTile);
+          },
+          [&](bool value, int i) { wait_landed(bar(value, i, true), (i / ST) & 1); });
+      for (int w = 0; w < 2; w++)
+        if (n[w] > 0) wait_landed(&q_full[w], 0);
     }
     // values that steer the products, from reductions, which give uniform registers
     const int n0 = (int)__reduce_max_sync(0xffffffffu, (unsigned)n[0]);
