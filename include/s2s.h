@@ -370,9 +370,17 @@ typedef struct s2s_attention {
 
 int s2s_masked_attention(const s2s_attention* a, void* stream);
 
-/* Waits for `device` and says whether a bounded wait of any kernel on it has given up
- * since the last look (S2S_ERR_TIMEOUT; the synchronous forwards look by themselves). */
+/* Waits for `device` and says (S2S_ERR_TIMEOUT) whether a bounded wait of an attention call
+ * on it has given up since the last look, or one of a forward that no synchronous forward
+ * has reported yet; that report stays the forward's. Neither keeps the other's calls, or
+ * other attention calls, from their results. Replays of a captured attention call that gave up
+ * do not wait long again until this has been asked. Not to be called while a stream of the
+ * device is captured. */
 int s2s_device_status(int device);
+
+/* Diagnostics: a kernel on `device` whose wait nobody meets, so that it gives up after 20 ms,
+ * recorded as an attention call's or (`attention` 0) as a forward's. */
+int s2s_debug_wait_gives_up(int device, int attention);
 
 /* gpu::selftest (src/gpu.rs:889-1265; `--cuda-selftest`, src/main.rs:179-192): with the
  * same arguments as s2s_create, build handles on `device` and check the fast paths

@@ -33,7 +33,7 @@ EXPORTS = ("s2s_create", "s2s_forward", "s2s_forward_batch", "s2s_forward_device
            "s2s_png_encode_rgb8", "s2s_png_encode_rows", "s2s_free", "s2s_adjust_device",
            "s2s_rgb8_device", "s2s_forward_image", "s2s_selftest", "s2s_rotary_init",
            "s2s_rotary_apply", "s2s_masked_attention", "s2s_device_status",
-           "s2s_debug_attention_loads")
+           "s2s_debug_attention_loads", "s2s_debug_wait_gives_up")
 BAND_ID_BYTES = 128
 MAX_AXES, ROTARY_MAX_PAIRS = 3, 128
 # element types of the token operators
@@ -181,6 +181,8 @@ def load() -> ctypes.CDLL:
     L.s2s_masked_attention.restype = ctypes.c_int
     L.s2s_device_status.argtypes = [ctypes.c_int]
     L.s2s_device_status.restype = ctypes.c_int
+    L.s2s_debug_wait_gives_up.argtypes = [ctypes.c_int, ctypes.c_int]
+    L.s2s_debug_wait_gives_up.restype = ctypes.c_int
     L.s2s_debug_attention_loads.argtypes = [ctypes.c_int, ctypes.c_int, ip]
     L.s2s_debug_attention_loads.restype = ctypes.c_int
     L.s2s_version.argtypes = []
@@ -552,3 +554,9 @@ def device_status(device: int = 0) -> None:
     """s2s_device_status: waits for the device; raises if a bounded wait on it gave up."""
     L = load()
     _fail(L, L.s2s_device_status(device))
+
+
+def debug_wait_gives_up(device: int = 0, attention: bool = True) -> None:
+    """s2s_debug_wait_gives_up: leaves the report of a wait that gave up."""
+    L = load()
+    _fail(L, L.s2s_debug_wait_gives_up(device, int(attention)))

@@ -159,22 +159,32 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t phase) {
   return ok != 0;
 }
 
-// Wait for the barrier's phase `phase` to complete, for at most ~2 s of wall time.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t phase, unsigned code) {
+// Wait for the barrier's phase `phase` to complete, for at most `limit_ns` of wall time; after
+// that `gave_up` records it. `stop` says that a wait elsewhere did, so that this one need not
+// run out.
+template <typename GaveUp, typename Stop>
+__device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t phase, uint64_t limit_ns,
+                                                  GaveUp&& gave_up, Stop&& stop) {
   const uint32_t a = smem_u32(bar);
   if (mbar_try_wait(a, phase)) return true;
   const uint64_t t0 = global_timer_ns();
   for (uint32_t it = 0;; ++it) {
     if (mbar_try_wait(a, phase)) return true;
     if ((it & 255u) == 255u) {
-      if (global_timer_ns() - t0 > 2000000000ull) {
-        record_error(code);
+      if (global_timer_ns() - t0 > limit_ns) {
+        gave_up();
         return false;
       }
-      // Another block already gave up: do not wait out a full budget of our own.
-      if (*(volatile unsigned*)&g_s2s_err != 0u) return false;
+      if (stop()) return false;
     }
   }
+}
+
+// The same for ~2 s, on the library's error word: once another block gave up, no wait runs out
+// a full budget of its own.
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t phase, unsigned code) {
+  return mbar_wait_bounded(bar, phase, 2000000000ull, [&] { record_error(code); },
+                           [] { return *(volatile unsigned*)&g_s2s_err != 0u; });
 }
 
 // ---------------------------------------------------------------- TMA

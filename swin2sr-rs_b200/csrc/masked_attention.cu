@@ -35,12 +35,51 @@ struct AttnArgs {
   int slots;       // of row tiles (find_document)
   unsigned long long guess;  // documents per slot, 32.32 fixed point
   int cta_heads;   // key heads that a CTA takes, one after the other
+  unsigned launch;  // a number of the call's own
   float scale, cap;
 };
 
 constexpr int kMaxSplits = 16;  // the largest cluster
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+
+// Waits that gave up in these kernels, apart from the library's error word, so that neither side
+// stops the other's calls or takes its reports: the first one's code, for s2s_device_status
+// alone, and the call that had the last one, whose other waits then do not run out.
+struct GaveUp {
+  unsigned code, launch;
+};
+__device__ GaveUp g_attention_gave_up = {0, 0};
+
+__device__ __forceinline__ bool attn_wait(unsigned launch, uint64_t* bar, uint32_t phase, unsigned code,
+                                          uint64_t limit_ns = 2000000000ull) {
+  return mbar_wait_bounded(
+      bar, phase, limit_ns,
+      [&] {
+        atomicCAS(&g_attention_gave_up.code, 0u, code);
+        atomicExch(&g_attention_gave_up.launch, launch);
+      },
+      [&] { return *(volatile unsigned*)&g_attention_gave_up.launch == launch; });
+}
+
+// A wait that nobody meets, for `limit_ns`, recorded as a forward's or as an attention call's.
+__global__ void k_wait_gives_up(int attention, unsigned launch, uint64_t limit_ns) {
+  __shared__ uint64_t bar;
+  mbar_init(&bar, 1);
+  fence_barrier_init();
+  if (attention)
+    attn_wait(launch, &bar, 0, DEV_TIMEOUT_FULL, limit_ns);
+  else
+    mbar_wait_bounded(&bar, 0, limit_ns, [] { record_error(DEV_TIMEOUT_FULL); }, [] { return false; });
+}
+
+// 1, 2, ...
+inline unsigned next_launch() {
+  static std::atomic<unsigned> last{0};
+  unsigned n = ++last;
+  while (n == 0) n = ++last;
+  return n;
+}
 
 struct Doc {
   int q0, nq, k0, nk, prefix;
@@ -444,6 +483,7 @@ int s2s_masked_attention(const s2s_attention* a, void* stream) {
     A.head_dim = a->head_dim;
     A.scale = a->scale;
     A.cap = a->cap;
+    A.launch = next_launch();
     cudaStream_t st = (cudaStream_t)stream;
     ck(a->dtype == S2S_F16 ? launch_attention<__half>(A, st) : launch_attention<__nv_bfloat16>(A, st),
        "masked_attention");
@@ -479,7 +519,34 @@ int s2s_device_status(int device) {
     } restore{before};
     ck(cudaSetDevice(device), "cudaSetDevice");
     ck(cudaDeviceSynchronize(), "cudaDeviceSynchronize");
-    check_device_error(nullptr);
+    GaveUp e, none = {0, 0};
+    ck(cudaMemcpyFromSymbol(&e, g_attention_gave_up, sizeof e), "error word");
+    if (e.code != 0) {
+      ck(cudaMemcpyToSymbol(g_attention_gave_up, &none, sizeof none), "error word");
+      fail(S2S_ERR_TIMEOUT, "a wait of an attention call gave up (code " + std::to_string(e.code) +
+                                "); its outputs are undefined");
+    }
+    unsigned forward = 0;  // the next synchronous forward reports and clears it
+    ck(cudaMemcpyFromSymbol(&forward, g_s2s_err, sizeof forward), "error word");
+    if (forward != 0)
+      fail(S2S_ERR_TIMEOUT, "a wait of a forward gave up (code " + std::to_string(forward) +
+                                "), which no synchronous forward has reported yet");
+  });
+}
+
+int s2s_debug_wait_gives_up(int device, int attention) {
+  using namespace s2s;
+  return guarded_call([&] {
+    int before = 0;
+    ck(cudaGetDevice(&before), "cudaGetDevice");
+    struct Restore {
+      int d;
+      ~Restore() { cudaSetDevice(d); }
+    } restore{before};
+    ck(cudaSetDevice(device), "cudaSetDevice");
+    k_wait_gives_up<<<1, 1>>>(attention, next_launch(), 20000000ull);
+    ck(cudaGetLastError(), "wait_gives_up");
+    ck(cudaDeviceSynchronize(), "wait_gives_up");
   });
 }
 

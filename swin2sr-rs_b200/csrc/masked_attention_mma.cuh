@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(32 * WARPS, MmaCfg<DP, RW, WARPS, NA>::CTAS)
 
     for (int t = tb; t < te; t++) {
       if (ok) {
-        ok = mbar_wait(&full[stage], phase, DEV_TIMEOUT_FULL);
+        ok = attn_wait(A.launch, &full[stage], phase, DEV_TIMEOUT_FULL);
         if (ok) flying--;
         else if (tid == 0)  // nothing is fetched after this
           for (int k = 0; k < flying; k++)

@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         return (full ? value ? v_full : k_full : value ? v_empty : k_empty) + i % ST;
       };
       load_tiles<ST>(
-          N, [&](bool value, int i) { return mbar_wait(bar(value, i, false), ((i / ST) - 1) & 1, DEV_TIMEOUT_EMPTY); },
+          N, [&](bool value, int i) { return attn_wait(A.launch, bar(value, i, false), ((i / ST) - 1) & 1, DEV_TIMEOUT_EMPTY); },
           [&](bool value, int i) {
             load((value ? vring : kring) + i % ST * C::KB, C::KB, value ? &mapV : &mapK, bar(value, i, true), hk,
                  D.k0 + key_tile(i) * BN);
@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // after a wait that gave up the products go on without waiting, over whatever is there
     bool ok = true;
     auto wait = [&](uint64_t* bar, int phase, unsigned code) {
-      if (ok) ok = mbar_wait(bar, phase & 1, code);
+      if (ok) ok = attn_wait(A.launch, bar, phase & 1, code);
     };
     if (warp == 9 || (C::SW == 2 && warp == 11)) {
       // ----------------------------------------------------------- score products
@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       if (one) tc_commit(&fin[mine == 1]);
       __syncwarp();
-      mbar_wait(&fin[mine == 1], 0, DEV_TIMEOUT_ACC);
+      attn_wait(A.launch, &fin[mine == 1], 0, DEV_TIMEOUT_ACC);
     } else if (warp == 10) {
       // ---------------------------------------------------------- output products
       // V is read along its rows as the contraction (keys contract, values are the N extent):
@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       if (one) tc_commit(&fin[2]);
       __syncwarp();
-      mbar_wait(&fin[2], 0, DEV_TIMEOUT_ACC);
+      attn_wait(A.launch, &fin[2], 0, DEV_TIMEOUT_ACC);
     }
   } else {
     more_registers<kSoftmaxRegisters>();
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     float m = -INFINITY, l = 0.0f;
     auto output_done = [&](int t) {
       const Place at(w, t, n[0], n[1]);
-      if (ok) ok = mbar_wait(&o_done[at.buffer], at.parity, DEV_TIMEOUT_ACC);
+      if (ok) ok = attn_wait(A.launch, &o_done[at.buffer], at.parity, DEV_TIMEOUT_ACC);
       __syncwarp();
       tc_fence_after();
     };
@@ -492,7 +492,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // heads of 64 x 4096^2).
     auto my_turn = [&](int t) {
       const int u = w ? t : t - 1;  // tile 0 first
-      if (ok && u >= 0 && u < (w ? n[0] : n[1])) ok = mbar_wait(&turn[warp ^ 4], u & 1, DEV_TIMEOUT_ACC);
+      if (ok && u >= 0 && u < (w ? n[0] : n[1])) ok = attn_wait(A.launch, &turn[warp ^ 4], u & 1, DEV_TIMEOUT_ACC);
       __syncwarp();
     };
     auto turn_over = [&]() {
@@ -524,7 +524,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (; t < n_w; t++) {
           const Place at(w, t, n[0], n[1]);
           const uint32_t ts = lanes + at.buffer * BN;
-          if (ok) ok = mbar_wait(&s_full[at.buffer], at.parity, DEV_TIMEOUT_ACC);
+          if (ok) ok = attn_wait(A.launch, &s_full[at.buffer], at.parity, DEV_TIMEOUT_ACC);
           __syncwarp();
           tc_fence_after();
           uint32_t raw[BN / 32][32];
@@ -672,7 +672,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             group_sync(1 + w);
             if (t + 1 < n_w) key_positions(t + 1);
           }
-          if (ok) ok = mbar_wait(&s_full[at.buffer], at.parity, DEV_TIMEOUT_ACC);
+          if (ok) ok = attn_wait(A.launch, &s_full[at.buffer], at.parity, DEV_TIMEOUT_ACC);
           __syncwarp();
           tc_fence_after();
           // [half][64 keys]: value 4 k + e is key 8 k + 2 t4 + (e & 1) of row R = 2 half + (e >> 1)
