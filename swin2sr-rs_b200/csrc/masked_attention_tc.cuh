@@ -222,14 +222,17 @@ __host__ __device__ __forceinline__ void load_tiles(int tiles, Released&& releas
     for (int i = n[v] > STAGES ? n[v] - STAGES : 0; i < n[v]; i++) landed(v == 1, i);
 }
 
-// MODE 0: no cap, no bias; 1: a cap; 1 + axes: a bias of one to three axes, with or without a cap.
+// MODE 0: no cap, no bias; 1 + axes: a bias of one to three axes, with or without a cap; 1: a cap that keeps
+// scores below kLargeScore, 5: any cap. (With what large scores take, 37 heads of 64 x 4096^2 under a cap of
+// 50 are 353 us instead of 331.)
 template <typename T, int NP, int MODE>
 __global__ void __launch_bounds__(kTcThreads, 1)
     k_attention_tc(const __grid_constant__ AttnArgs A, const __grid_constant__ CUtensorMap mapQ,
                    const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV) {
   using C = TcCfg<NP>;
   constexpr int BN = C::BN, NB = C::NB, ST = C::STAGES;
-  constexpr int NA = MODE < 2 ? 1 : MODE - 1;  // axes of a bias
+  constexpr bool BIAS = MODE >= 2 && MODE <= 4, CAP = MODE == 1 || MODE == 5;
+  constexpr int NA = BIAS ? MODE - 1 : 1;  // axes of a bias
   using Place = TcPlace<NB>;
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ uint8_t smem_raw[];
@@ -303,18 +306,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   // keys, and wrap around: scores that grew from tile to tile on the way there would have the
   // outputs scaled again for each. Both row tiles then take all of them.
   int start = 0;
-  if (MODE >= 2) {
+  if (BIAS) {
     n[0] = rows[0] > 0 ? max(n[0], n[1]) : 0;
     n[1] = rows[1] > 0 ? n[0] : 0;
     start = max(0, min((i0 + D.nk - D.nq) / BN, n[0] - 1));
   }
-  auto key_tile = [&](int step) { return start + step < n[0] || MODE < 2 ? start + step : start + step - n[0]; };
+  auto key_tile = [&](int step) { return start + step < n[0] || !BIAS ? start + step : start + step - n[0]; };
   const int ksteps = (A.head_dim + 15) / 16;
 
   // registers: 384 threads begin with 168 each; the softmax groups take what the third gives
   // (2 * 128 * 208 + 128 * 80 or 2 * 128 * 216 + 128 * 64, 63488 of 64512; with a bias 200 took 5 %
   // more time, with a cap 208 6 %)
-  constexpr int kSoftmaxRegisters = MODE == 1 ? 216 : 208, kOtherRegisters = MODE == 1 ? 64 : 80;
+  constexpr int kSoftmaxRegisters = CAP ? 216 : 208, kOtherRegisters = CAP ? 64 : 80;
   if (warp >= 8) {
     fewer_registers<kOtherRegisters>();
     if (warp == 8 && lane == 0) {
@@ -347,7 +350,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int keys = (int)__reduce_max_sync(0xffffffffu, (unsigned)kmax);
     const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
     const int last = max(n0, n1) - 1;
-    const int cut = MODE >= 2 ? (int)__reduce_max_sync(0xffffffffu, (unsigned)(last - start)) : last;  // step of the last keys
+    const int cut = BIAS ? (int)__reduce_max_sync(0xffffffffu, (unsigned)(last - start)) : last;  // step of the last keys
     // after a wait that gave up the products go on without waiting, over whatever is there
     bool ok = true;
     auto wait = [&](uint64_t* bar, int phase, unsigned code) {
@@ -506,15 +509,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (lane == 0) mbar_arrive(&p_full[b]);
     };
 
-    if constexpr (MODE < 2) {
+    if constexpr (!BIAS) {
       // a row a thread
       float base = 0.0f;  // of the exponents
       bool some_large = false;
       auto new_base = [&]() {
         const float b = m == -INFINITY ? 0.0f : m * unit;
-        const bool large = fabsf(b) >= kLargeScore;
+        const bool large = MODE != 1 && fabsf(b) >= kLargeScore;
         base = kTcLift<T> - (large ? 0.0f : b);
-        some_large = __any_sync(0xffffffffu, large);
+        if (MODE != 1) some_large = __any_sync(0xffffffffu, large);
       };
       // Tiles from t on, until all are done or, where rows with large maxima are not taken, the first
       // such row; that tile is begun again (its scores are still there). A loop of its own, as the
@@ -534,7 +537,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
           for (int c = 0; c < BN / 32; c++) loaded(raw[c]);
           float(&s)[BN] = reinterpret_cast<float(&)[BN]>(raw);
-          if constexpr (MODE == 1) capped(s, to_cap, raw_cap);
+          if constexpr (CAP) capped(s, to_cap, raw_cap);
           if ((t + 1) * BN > open) {
             const int last = mine - t * BN;
 #pragma unroll
@@ -587,7 +590,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         return t;
       };
       const int from = walk(std::false_type(), 0);
-      if (__builtin_expect(from < n_w, 0)) walk(std::true_type(), from);
+      if constexpr (MODE != 1)
+        if (__builtin_expect(from < n_w, 0)) walk(std::true_type(), from);
     } else {
       // Four rows a thread, g + 8 R, and of each eight keys the two of the lane's place in its quad:
       // a key's positions then serve four scores. (With a row a thread every thread read all the
@@ -885,19 +889,19 @@ cudaError_t launch_attention_tc(AttnArgs& A, cudaStream_t st) {
   return launch_pdl(kernel, dim3((unsigned)grid), dim3(kTcThreads), C::SMEM, st, A, q, k, v);
 }
 
+template <typename T, int NP>
+cudaError_t launch_attention_tc(AttnArgs& A, cudaStream_t st) {
+  return A.axes > 2                     ? launch_attention_tc<T, NP, 4>(A, st)
+         : A.axes > 1                   ? launch_attention_tc<T, NP, 3>(A, st)
+         : A.axes                       ? launch_attention_tc<T, NP, 2>(A, st)
+         : A.cap == 0.0f                ? launch_attention_tc<T, NP, 0>(A, st)
+         : A.cap * kLog2e < kLargeScore ? launch_attention_tc<T, NP, 1>(A, st)
+                                        : launch_attention_tc<T, NP, 5>(A, st);
+}
+
 template <typename T>
 cudaError_t launch_attention_tc(AttnArgs& A, cudaStream_t st) {
-  if (A.head_dim <= 64)
-    return A.axes > 2     ? launch_attention_tc<T, 1, 4>(A, st)
-           : A.axes > 1   ? launch_attention_tc<T, 1, 3>(A, st)
-           : A.axes       ? launch_attention_tc<T, 1, 2>(A, st)
-           : A.cap > 0.0f ? launch_attention_tc<T, 1, 1>(A, st)
-                          : launch_attention_tc<T, 1, 0>(A, st);
-  return A.axes > 2     ? launch_attention_tc<T, 2, 4>(A, st)
-         : A.axes > 1   ? launch_attention_tc<T, 2, 3>(A, st)
-         : A.axes       ? launch_attention_tc<T, 2, 2>(A, st)
-         : A.cap > 0.0f ? launch_attention_tc<T, 2, 1>(A, st)
-                        : launch_attention_tc<T, 2, 0>(A, st);
+  return A.head_dim <= 64 ? launch_attention_tc<T, 1>(A, st) : launch_attention_tc<T, 2>(A, st);
 }
 
 }  // namespace

@@ -23,6 +23,8 @@ def softmax(P):
     out, lse, a, b = [], [], 0, 0
     for nq, nk in zip(P.q_lens, P.kv_lens):
         z = P.q[a:a + nq].double() @ P.k[b:b + nk, 0].double().T * P.scale  # [query][head][key]
+        if P.cap:
+            z = P.cap * torch.tanh(z / P.cap)
         for x in range(P.axes):
             far = (P.q_pos[x, a:a + nq, None].double() - P.kv_pos[x, None, b:b + nk].double()).abs()
             z = z - P.slopes[x].double().abs()[:, None] * far[:, None]
@@ -156,3 +158,18 @@ def test_attention_a_cap_far_above_the_scores_changes_nothing(dim, axes, dtype, 
     plain, sums = Problem(dtype, dim, 4, 2, [300, 40], [300, 700], **more).run()
     out, lse = Problem(dtype, dim, 4, 2, [300, 40], [300, 700], cap=2.0 ** 20, **more).run()
     assert torch.equal(lse, sums) and torch.equal(out, plain)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("cap", [2.0 ** 11, 2.0 ** 14, 2.0 ** 25, 2.0 ** 33])
+@pytest.mark.parametrize("q_lens,kv_lens", [([1], [5000]), ([300, 40], [300, 700])])
+def test_attention_large_scores_under_large_caps(q_lens, kv_lens, cap, dim, dtype, kernel):
+    """Scores of 1 to 3 quarters of the cap: each of the three capped ones is the same number for all its keys,
+    and they lie 2^8 and more apart, so that equal keys share a row as without a cap."""
+    P = Problem(dtype, dim, 2, 1, q_lens, kv_lens, scale=8.0 / dim, cap=cap)
+    a, g = int(math.log2(cap) - 3) // 2, torch.Generator().manual_seed(dim)
+    P.q[:] = 2.0 ** a
+    P.q[:, 1] = -(2.0 ** a)
+    P.k[:] = cap / 8 / 2.0 ** a / 4 * torch.randint(1, 4, P.k.shape[:2], generator=g)[..., None]
+    check(P)
