@@ -341,14 +341,17 @@ int s2s_rotary_apply(const s2s_rotary* r, int dtype, int head_dim, int tokens, c
  * out_i = sum of softmax(z)_j v_j over the keys seen, d_lse = log sum exp(z) in fp32; a row
  * that sees no key (or only scores of minus infinity) gives zeros and minus infinity.
  * Values at keys that a row does not see never reach it, NaN and infinities included. Rows
- * of no document are left as they were. Heads of out lie within a token's row, or tokens within
- * a head's. out and d_lse may not overlap each other or an
- * input. Two positions of a document lie less than 2^31 apart. Positions count, in 32-bit
- * floating point, from a query less than 256 queries away: a distance is rounded once where both
- * of its positions lie less than 2^24 from that one's, and is right to 2^-22 of itself while such
- * queries lie less than 2^23 apart; beyond that it is off by up to 2^-23 of what they do. The
- * result of a call does not depend on what else runs; a bounded wait that gives up
- * (s2s_device_status) leaves it undefined. */
+ * of no document are left as they were. Heads of out lie within a token's row, or tokens
+ * within a head's. out and d_lse may not overlap each other or an input.
+ * Scores (of any finite size), maxima, sums and outputs are 32-bit; the weights are rounded to
+ * `dtype` before they meet v (in fp16 those below 2^-31 of a row's largest may count as zero),
+ * the sum that divides them is not. Two positions of a document lie less than 2^31 apart.
+ * Positions count, in 32-bit floating point, from a query less than 256 queries away: a
+ * distance is right to 2^-22 of itself while such queries lie less than 2^23 apart, beyond that
+ * it is off by up to 2^-23 of what they do. The result of a call does not depend on what else
+ * runs; a bounded wait that gives up (s2s_device_status) leaves it undefined. The kernel is
+ * chosen by the documents' mean lengths: a long document with very many short ones can take
+ * several times as long as in a call of its own. */
 typedef struct s2s_attention {
   int dtype;     /* S2S_F16 or S2S_BF16, of q, k, v and out */
   int head_dim;  /* a multiple of 8, at most 128 */

@@ -372,9 +372,12 @@ namespace {
 // over a key in 22 and 10000 besides, whatever the head; the mma.sync tiles take 0.25, 0.34 or 0.59
 // of an SM for each pair of query and key (head_dim up to 32, 64, 128), in as many CTAs as fill the
 // device. At eight heads of 64 and 8192 tokens in all, documents of 192: 23 us by mma.sync, 27 by
-// tcgen05; of 256: 26 and 22; of 512: 41 and 24. With 345 queries, 16 heads of 128 and 9000 keys
-// in three documents (48 tcgen05 CTAs): 62 and 96. S2S_MASKED_ATTN=mma or tcgen05 in the environment
-// (a validation switch, read at every call) takes that one.
+// tcgen05; of 256: 26 and 22; of 512: 41 and 24. The lengths are on the device, so the costs are those of
+// documents of the mean length. Where lengths are mixed the choice can be the slower kernel: 196, 49
+// and 100 queries over 6272, 1813 and 900 keys, 16 heads of 128: mma.sync, 71 us of 98; three times 115 over
+// 3000: mma.sync, 63 of 36; one image of 4096 with 60 of 16, 12 heads of 64: mma.sync, 189 of 126; 16384 in
+// order with 200 of one, eight heads of 128: mma.sync, 2251 of 516. S2S_MASKED_ATTN=mma or tcgen05 in the
+// environment (a validation switch, read at every call) takes that one.
 template <typename T>
 cudaError_t launch_attention(AttnArgs& A, cudaStream_t st) {
   const double queries = (double)A.q_tokens / A.documents, keys = (double)A.kv_tokens / A.documents;

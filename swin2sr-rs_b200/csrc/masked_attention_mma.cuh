@@ -6,15 +6,16 @@
 // read once for all of them - and walks the keys in tiles of 16 a warp through a ring of three
 // stages that TMA fills. RW warps lie along the rows, the others along the keys of a tile: one
 // query of eight heads is one row tile, whose keys the warps share. Every warp keeps a running
-// maximum, sum and output of its own; they are joined once at the end, first within the CTA, then over the CTAs of a cluster
-// among which the keys of the tile were split (through distributed shared memory: a call
-// needs no workspace, and the order of the sums is fixed).
+// maximum, sum and output of its own; they are joined once at the end, first within the CTA, then over
+// the CTAs of a cluster among which the keys of the tile were split (through distributed shared memory:
+// a call needs no workspace, and the order of the sums is fixed).
 //
 // Bound: HBM where the keys are long (K and V are read once), else the latency of a tile's chain of
 // products, softmax and products, of which an SM has eight to sixteen warps' worth to hide. Measured
 // (B200): 24 single queries of 32 heads over 111 000 keys of 8 x 128, 444 MB: 102 us, 4.3 TB/s
 // (68 us at the measured copy rate); 1271 windows of 64, six heads of 32, two axes: 55 us (45
-// without a bias, 19 for the bytes); 5 queries of 16 heads over 40001 keys of 2 x 128: 30 us.
+// without a bias, 19 for the bytes; issue slots 0.43, no unit above 0.3); 5 queries of 16 heads over
+// 40001 keys of 2 x 128: 29 us.
 #pragma once
 
 namespace s2s {

@@ -17,12 +17,14 @@
 // weights refer to, which after the first tiles is rare; the group does it itself. Weights then stay
 // below 2^8, in fp16 with its lift (kTcLift) below 2^15, and the sums are 32-bit.
 //
-// Bound: for head_dim <= 64 the special function unit (16 exponentials a cycle and SM: 2048 cycles
-// for 256 x 128 pairs, of 2900), beyond it the tensor core with its 64-key score products (2560 of
-// 3000). Measured (B200, non-causal, 37 heads, 4096 x 4096): 195 us at head 64, 811 TFLOP/s; 281 us
-// at head 128, 1130 TFLOP/s, 0.69 of the measured bf16 rate; causal 16384, eight heads of 128: 434-447
-// us, 1230 TFLOP/s. With a cap of 50: 331 and 398 us; with one axis of bias 303 and 372; with two
-// axes at head 64 351.
+// Bound: without a cap or a bias, for head_dim <= 64 the special function unit (16 exponentials a cycle
+// and SM: 2048 cycles for 256 x 128 pairs, of 2900), beyond it the tensor core with its 64-key score
+// products. With either no unit is full (six images with two axes: exponentials 0.40, issue 0.48, tensor
+// 0.20 of the cycles): two softmax warps a scheduler, each a chain from scores to weights. Measured
+// (B200, bf16, non-causal, 37 heads, 4096 x 4096, replayed from a graph): 194 us at head 64, 820 TFLOP/s;
+// 288 us at head 128, 1100 TFLOP/s, 0.67 of the measured bf16 burst; with a cap of 50 340 and 406 us, with
+// one, two, three axes of bias 334, 333, 463 and 417, 424, 504. Causal 16384, eight heads of 128: 446-457
+// us in bursts, 1220 TFLOP/s, 530 back to back for seconds under the power cap, 1040 TFLOP/s.
 #pragma once
 
 namespace s2s {
@@ -169,7 +171,8 @@ __device__ __forceinline__ void group_sync(int id) {
 }
 // Weights are 2^(s unit - m unit), in one multiply-add behind the rounded m unit, which all weights of a
 // row share. Beyond this size (in either direction), where that rounding passes the 2^-12 that a score has
-// itself, m is taken off first. (For all rows: images 307 -> 325 us, causal 16384 511 -> 539 back to back.)
+// itself, m is taken off first. (Taken off first in all rows: six images 307 -> 325 us, causal 16384 511 ->
+// 539 back to back.)
 constexpr float kLargeScore = 4096.0f;
 // In fp16 weights are 2^7 times as large, so that those down to 2^-31 of the largest count in the second
 // product (its least value is 2^-24; see kMmaLift).
@@ -491,7 +494,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // With a bias the two softmax warps of a scheduler (warp and warp ^ 4) take turns at the
     // exponentials, so that one's keep the special function unit busy while the other is at its
     // bias (12 heads of 64, six images of up to 4096 tokens: 338 -> 308 us when they were added,
-    // 304 now; without a bias turns cost more than they give, 193 -> 238 us at 37
+    // 290 now; without a bias turns cost more than they give, 193 -> 238 us at 37
     // heads of 64 x 4096^2).
     auto my_turn = [&](int t) {
       const int u = w ? t : t - 1;  // tile 0 first
@@ -520,8 +523,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (MODE != 1) some_large = __any_sync(0xffffffffu, large);
       };
       // Tiles from t on, until all are done or, where rows with large maxima are not taken, the first
-      // such row; that tile is begun again (its scores are still there). A loop of its own, as the
-      // branch cost 511 -> 566 us in the one for all (causal 16384).
+      // such row; that tile is begun again (its scores are still there). A loop of its own: as a branch
+      // in one loop for all it cost 511 -> 566 us (causal 16384 back to back), as two loops 519.
       auto walk = [&](auto form, int t) {
         constexpr bool LARGE = decltype(form)::value;
         for (; t < n_w; t++) {
@@ -604,8 +607,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // distances come from the positions' differences, exact where both are near the tile's first
       // query, and each further axis costs two packed operations and an absolute addition. (As
       // |slope q - slope k| neighbours would be off by the rounding of products that grow along the
-      // tile; the difference times each axis' slope took 333 us for the six images, this takes 303. One
-      // axis alone, 37 heads of 64 x 4096^2: 331 us, two 337, three 453.)
+      // tile; the difference times each axis' slope took 333 us for the six images where this took 303.)
       int axis[NA];
       float slope = 0.0f, ratio[NA];
 #pragma unroll

@@ -10,8 +10,9 @@
 // position 1e6 a 32-bit product is off by 0.06 rad, this one by less than 1e-9. Sine and
 // cosine of the fraction, products and sums are 32-bit.
 //
-// Measured (B200): 50176 tokens of 16 + 4 heads of 128, bf16: 90 us, 5.7 TB/s (0.87 of the
-// measured copy); 81344 tokens of 6 + 6 heads of 32, fp16: 28 us, 4.5 TB/s. Fewer tokens a CTA
+// Measured (B200): 50176 tokens of 16 + 4 heads of 128, bf16: 97 us, 5.3 TB/s (0.81 of the
+// measured copy; 90 us where a replay finds a part of its inputs in L2); 81344 tokens of 6 + 6
+// heads of 32, fp16: 28 us, 4.5 TB/s. Fewer tokens a CTA
 // (8: 33 us at 12 heads of 32) repeat the set-up, two or four loads ahead of the angles take
 // the registers that the eight CTAs of an SM need (147 us instead of 90).
 #include "heads.cuh"
