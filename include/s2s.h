@@ -344,8 +344,8 @@ int s2s_rotary_apply(const s2s_rotary* r, int dtype, int head_dim, int tokens, c
  * of no document are left as they were. Heads of out lie within a token's row, or tokens
  * within a head's. out and d_lse may not overlap each other or an input.
  * Scores (of any finite size), maxima, sums and outputs are 32-bit; the weights are rounded to
- * `dtype` before they meet v (in fp16 those below 2^-31 of a row's largest may count as zero),
- * the sum that divides them is not. Two positions of a document lie less than 2^31 apart.
+ * `dtype` before they meet v (in fp16 those below 2^-31 of a row's largest may count as zero;
+ * with an infinite v that is NaN), the sum that divides them is not. Two positions of a document lie less than 2^31 apart.
  * Positions count, in 32-bit floating point, from a query less than 256 queries away: a
  * distance is right to 2^-22 of itself while such queries lie less than 2^23 apart, beyond that
  * it is off by up to 2^-23 of what they do. The result of a call does not depend on what else
